@@ -564,6 +564,157 @@ SAM3CU_API int sam3cu_neck_forward_async(sam3cu_neck *nk, const float *feat, int
 SAM3CU_API void *sam3cu_neck_stream(sam3cu_neck *nk);
 SAM3CU_API void sam3cu_neck_destroy(sam3cu_neck *nk);
 
+/* ------------------------- attention over an encoder's states (decoder side) */
+
+/*
+ * Rotary positions.  Pair i < rot_dim/2 of a head turns by turns[i] * p
+ * revolutions at position p; cosine and sine are multiplied by amplitude.
+ * SAM3CU_ROPE_INTERLEAVED pairs elements (2i, 2i+1), as cpu_rope.c:35-110
+ * does; SAM3CU_ROPE_HALF pairs (i, i + rot_dim/2).  Elements from rot_dim on
+ * are not rotated.
+ */
+enum sam3cu_rope_layout {
+	SAM3CU_ROPE_INTERLEAVED = 0,
+	SAM3CU_ROPE_HALF = 1,
+};
+
+/*
+ * How the angles theta^(-2i/rot_dim) are scaled for contexts of `factor`
+ * times the trained length:
+ *   LINEAR  every angle divided by factor
+ *   NTK     theta * factor^(rot_dim/(rot_dim-2)) in place of theta
+ *   YARN    pairs that turn more than beta_fast times over trained_len keep
+ *           their angle, those that turn less than beta_slow times have it
+ *           divided by factor, a ramp over the pair index between them;
+ *           amplitude 0.1 ln(factor) + 1
+ *   BANDS   pairs whose wavelength is below trained_len/high_freq keep their
+ *           angle, those above trained_len/low_freq have it divided by
+ *           factor, interpolated in trained_len/wavelength between them
+ */
+enum sam3cu_rope_scaling {
+	SAM3CU_ROPE_SCALE_NONE = 0,
+	SAM3CU_ROPE_SCALE_LINEAR = 1,
+	SAM3CU_ROPE_SCALE_NTK = 2,
+	SAM3CU_ROPE_SCALE_YARN = 3,
+	SAM3CU_ROPE_SCALE_BANDS = 4,
+};
+
+struct sam3cu_rope_config {
+	int rot_dim;          /* even, 2 .. 256 */
+	int layout;           /* enum sam3cu_rope_layout */
+	int scaling;          /* enum sam3cu_rope_scaling */
+	double theta;         /* > 1 (10000) */
+	double factor;        /* >= 1, for every scaling but NONE */
+	double trained_len;   /* > 0, YARN and BANDS */
+	double beta_fast, beta_slow;    /* YARN (32, 1): fast > slow > 0 */
+	double low_freq, high_freq;     /* BANDS (1, 4): high > low > 0 */
+	double amplitude;     /* 0: 1, or what YARN says */
+};
+
+#define SAM3CU_ROPE_MAX_PAIRS 128
+
+/* Angles in 64 bits, in revolutions per position: at position 10^6 a 32-bit
+ * angle is already off by 0.06 radians.  Host memory; every call that takes
+ * it copies it. */
+struct sam3cu_rope_freqs {
+	int n_pairs;          /* rot_dim / 2 */
+	int layout;
+	float amplitude;
+	double turns[SAM3CU_ROPE_MAX_PAIRS];
+};
+
+/* Fill the frequencies of a configuration.  Host only. */
+SAM3CU_API int sam3cu_rope_freqs_init(const struct sam3cu_rope_config *cfg,
+				      struct sam3cu_rope_freqs *out);
+
+/*
+ * Heads of one tensor, read at x and written at y (device, one type):
+ * element d of head h of token s of sequence b lies at
+ * x[b*x_strides[0] + s*x_strides[1] + h*x_strides[2] + d] (element strides,
+ * >= 0; y likewise).  y may be x with the same strides; x and y that overlap
+ * in any other way, and outputs that overlap each other or the other
+ * tensor's input, are not detected.  gamma, beta: device F32 [head_dim] or
+ * NULL (sam3cu_qk_norm_rope only).  heads may be 0 (pointers unused).
+ */
+struct sam3cu_head_view {
+	const void *x;
+	int64_t x_strides[3];
+	void *y;
+	int64_t y_strides[3];
+	int heads;
+	const float *gamma, *beta;
+};
+
+/*
+ * Rotate the heads of q and k (k NULL: q alone) by the positions of their
+ * tokens: positions[b*pos_stride + s] (device int64; pos_stride 0: the same
+ * for every sequence; negative positions turn backwards), or start + s where
+ * positions is NULL.  The angle is formed in 64 bits, the rotation in F32.
+ * dtype SAM3CU_F32, _F16 or _BF16; head_dim 2 .. 256, >= 2*n_pairs.  Heads
+ * whose head_dim and rot_dim are multiples of 16 and whose rows start on 16
+ * bytes take 16-byte accesses.
+ */
+SAM3CU_API int sam3cu_rope_pos(const struct sam3cu_head_view *q, const struct sam3cu_head_view *k,
+			       int dtype, int batch, int seq, int head_dim,
+			       const int64_t *positions, int64_t pos_stride, int64_t start,
+			       const struct sam3cu_rope_freqs *freqs, void *stream);
+
+enum sam3cu_head_norm {
+	SAM3CU_NORM_RMS = 1,   /* x / sqrt(mean(x^2) + eps) * gamma + beta */
+	SAM3CU_NORM_LAYER = 2, /* (x - mean) / sqrt(var + eps) * gamma + beta */
+};
+
+/*
+ * Normalise every head of q and k over its head_dim elements (statistics in
+ * F32; a NULL gamma is 1, a NULL beta 0), then rotate as sam3cu_rope_pos
+ * does (freqs NULL: no rotation), in one pass over the data with one
+ * rounding.  eps >= 0.
+ */
+SAM3CU_API int sam3cu_qk_norm_rope(const struct sam3cu_head_view *q,
+				   const struct sam3cu_head_view *k, int dtype, int batch, int seq,
+				   int head_dim, int norm, float eps, const int64_t *positions,
+				   int64_t pos_stride, int64_t start,
+				   const struct sam3cu_rope_freqs *freqs, void *stream);
+
+/*
+ * Attention of queries over an encoder's states of another length:
+ *   o[b,i,h] = sum_j p_j v[b,j,h/g],  g = q_heads / kv_heads,
+ *   p = softmax over j of scale * q[b,i,h].k[b,j,h/g] + bias[b,h,i,j]
+ * over the keys j < min(k_lens[b], sk) with key_mask[b,j] != 0.  A query
+ * without any such key (or whose every score is -inf) gives zeros.  K and V
+ * of keys that do not count are never used, whatever they hold.
+ *
+ * q, o [batch, sq, q_heads, head_dim], k, v [batch, sk, kv_heads, head_dim]:
+ * device, dtype SAM3CU_BF16 or _F16, addressed by element strides (batch,
+ * token, head) >= 0, head_dim elements contiguous; head_dim a multiple of 8,
+ * 8 .. 128; pointers on 16 bytes and strides multiples of 8 (a stride of 0
+ * shares the data: states common to a batch).  o must not overlap an input.
+ * k_lens: device int32 [batch] or NULL (values below 0 count as 0).
+ * key_mask: device bytes, row b at key_mask + b*mask_stride, or NULL.
+ * bias: device F32 [batch, q_heads, sq, sk] with strides (batch, head, query)
+ * >= 0, keys contiguous, or NULL; -inf removes a key for its query (the key's
+ * V still has to be finite); finite values, the lowest included, only add.
+ * scale 0: 1/sqrt(head_dim).  q_heads / kv_heads <= 128.  Scores, softmax
+ * and sums in F32, P rounded to dtype before P.V.
+ */
+struct sam3cu_cross_attention_args {
+	const void *q, *k, *v;
+	void *o;
+	int64_t q_strides[3], k_strides[3], v_strides[3], o_strides[3];
+	int dtype;
+	int batch, sq, sk;
+	int q_heads, kv_heads, head_dim;
+	float scale;
+	const int32_t *k_lens;
+	const uint8_t *key_mask;
+	int64_t mask_stride;
+	const float *bias;
+	int64_t bias_strides[3];
+};
+
+SAM3CU_API int sam3cu_cross_attention(const struct sam3cu_cross_attention_args *args,
+				      void *stream);
+
 /* ------------------------------------------------------ .sam3 weight files */
 
 /*

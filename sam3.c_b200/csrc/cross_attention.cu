@@ -1,0 +1,537 @@
+// cross_attention.cu - attention of queries over states of another length,
+// for few query rows or few keys (and the entry point of both kernels).
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(s_j - max s),
+//   s_j = scale q.k_j + bias_j, over the keys that count
+//
+// One pass over the keys with the running maximum and sum of each row.  With
+// few rows to a key head the call reads K and V once and does little with
+// them, with few keys it reads Q and writes O: HBM bounds both, and what
+// matters is that enough loads are under way on every SM.  So:
+//   * a warp computes 16 rows with m16n8k16 MMAs (fp32 accumulate); K and V
+//     tiles come by 16-byte cp.async through a ring in shared memory;
+//   * up to 16 rows: every warp of the CTA walks key tiles of its own (no
+//     CTA barrier in the loop); more: the CTA's four warps take 16 rows each
+//     of 64 and share the tiles;
+//   * where that leaves SMs idle the keys are split over the CTAs of a
+//     cluster, which exchange (max, sum, partial O) through distributed
+//     shared memory: no workspace, no second launch, a fixed order of sums.
+// A key that does not count is not read at all: its K and V rows are
+// zero-filled by the copy (so what they hold cannot reach the sums as 0 * NaN)
+// and its score is -inf.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <cmath>
+#include <cstdint>
+#include <cstring>
+
+#include "../../include/sam3cu.h"
+#include "cross_attention.cuh"
+#include "sam3cu_internal.h"
+#include "sm100_ptx.cuh"
+
+namespace s3 {
+
+namespace {
+
+constexpr int kThreads = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool pred) {
+  const int n = pred ? 16 : 0;  // zero fill
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr)
+               : "memory");
+}
+template <bool kBf16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (kBf16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if (kBf16) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+  __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+// kD: head_dim rounded up to 32, 64 or 128 (the copies fill the rest with
+// zeros).  kWM: row warps of the CTA (4 / kWM warps split the keys of a tile).
+template <int kD, int kWM>
+struct Cfg {
+  static constexpr int kRows = 16 * kWM;               // query rows of a CTA
+  static constexpr int kWK = 4 / kWM;                  // key warps
+  static constexpr int kKW = kWM == 4 ? 64 : 32;       // keys of a warp's tile
+  static constexpr int kKT = kKW * kWK;                // keys of the CTA's tile
+  static constexpr int kChunks = kD / 8;               // 16-byte pieces of a row
+  static constexpr int kTileBytes = kKT * kD * 2;      // K or V
+  static constexpr int kStages = kD == 32 ? 4 : kD == 64 ? 3 : 2;
+  static constexpr int kQBytes = kRows * kD * 2;
+  static constexpr int kOPitch = kD + 4;               // floats of a partial row
+  static constexpr int kPartBytes = kWK * kRows * kOPitch * 4;  // partial O of each key warp (over the ring)
+  static constexpr int kRing = 2 * kStages * kTileBytes;
+  static constexpr int kSmem = kQBytes + (kRing > kPartBytes ? kRing : kPartBytes);
+};
+
+// Byte offset of 16-byte piece c of row r in a tile of kChunks pieces a row,
+// permuted within each 128-byte line so that ldmatrix (8 rows, one piece)
+// and the copies (consecutive pieces) touch all banks.
+template <int kChunks>
+__device__ __forceinline__ uint32_t tile_at(int r, int c) {
+  const int at = r * kChunks + c;
+  const int key = kChunks == 4 ? (r >> 1) & 3 : r & 7;
+  return static_cast<uint32_t>((at ^ key) << 4);
+}
+
+template <bool kBf16, int kD, int kWM, bool kBias>
+__global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_constant__ CrossParams p, int row_tiles,
+                                                             int splits) {
+  using Cf = Cfg<kD, kWM>;
+  constexpr int kKW = Cf::kKW, kKT = Cf::kKT, kWK = Cf::kWK, kCh = Cf::kChunks, kStages = Cf::kStages;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float2 ml[kWK][Cf::kRows];  // (max, sum) of each row, by key warp; [0] then holds the CTA's
+  __shared__ float wgt[kWK][Cf::kRows];
+  const uint32_t sq = smem_u32(smem), ring = sq + Cf::kQBytes;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int wm = kWM == 4 ? warp : 0, wk = kWM == 4 ? 0 : warp;
+  const int split = blockIdx.x % splits, item = blockIdx.x / splits;
+  const int rt = item % row_tiles, bh = item / row_tiles;
+  const int kvh = bh % p.kv_heads, b = bh / p.kv_heads;
+  const int row0 = rt * Cf::kRows;
+  const int len = cross_len(p, b);
+  const uint16_t* kg = p.k + b * p.kb + kvh * p.kh;
+  const uint16_t* vg = p.v + b * p.vb + kvh * p.vh;
+  const uint8_t* mg = p.key_mask ? p.key_mask + b * p.mask_stride : nullptr;
+
+  const int n_tiles = (len + kKT - 1) / kKT;
+  const int t0 = static_cast<int>(static_cast<int64_t>(n_tiles) * split / splits);
+  const int t1 = static_cast<int>(static_cast<int64_t>(n_tiles) * (split + 1) / splits);
+
+  // the rows' queries, zero-filled past the last row and past head_dim
+  for (int i = tid; i < Cf::kRows * kCh; i += kThreads) {
+    const int r = i / kCh, c = i % kCh;
+    const bool ok = row0 + r < p.rows && c * 8 < p.head_dim;
+    const int s = ok ? (row0 + r) / p.group : 0, h = ok ? (row0 + r) % p.group : 0;
+    const uint16_t* src = p.q + b * p.qb + s * p.qs + static_cast<int64_t>(kvh * p.group + h) * p.qh + (ok ? c * 8 : 0);
+    cp_async16(sq + tile_at<kCh>(r, c), src, ok);
+  }
+  cp_async_commit();
+
+  // Tile t into its ring slot: by the whole CTA, or by each key warp its own
+  // keys (then only that warp waits for them).
+  auto load = [&](int t) {
+    const uint32_t sk = ring + (t % kStages) * 2 * Cf::kTileBytes, sv = sk + Cf::kTileBytes;
+    constexpr int kCopies = kKW * kCh / (kWM == 4 ? kThreads : 32);
+#pragma unroll 4
+    for (int i = 0; i < kCopies; ++i) {
+      const int idx = (kWM == 4 ? tid : lane) + i * (kWM == 4 ? kThreads : 32);
+      const int r = wk * kKW + idx / kCh, c = idx % kCh;
+      const int key = t * kKT + r;
+      bool ok = key < len && c * 8 < p.head_dim;
+      if (mg && ok) ok = mg[key] != 0;
+      const int64_t at = ok ? key : 0;
+      const int cc = ok ? c * 8 : 0;
+      cp_async16(sk + tile_at<kCh>(r, c), kg + at * p.ks + cc, ok);
+      cp_async16(sv + tile_at<kCh>(r, c), vg + at * p.vs + cc, ok);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    if (t0 + i < t1) load(t0 + i);
+    cp_async_commit();
+  }
+
+  float acc[kD / 8][4];
+#pragma unroll
+  for (int j = 0; j < kD / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+  uint32_t qf[kD / 16][4];
+  // with a bias the scores are in natural units (its lowest finite values
+  // would overflow in base 2), without one they stay unscaled dot products
+  const float to_log2 = kBias ? kLog2e : p.scale_log2;
+  const float* brow[2] = {nullptr, nullptr};
+  if (kBias) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = min(row0 + wm * 16 + (lane >> 2) + 8 * h, p.rows - 1);
+      brow[h] = p.bias + b * p.bb + static_cast<int64_t>(kvh * p.group + r % p.group) * p.bh + (r / p.group) * p.bs;
+    }
+  }
+
+  cp_async_wait<kStages - 1>();  // the queries
+  __syncthreads();
+#pragma unroll
+  for (int kk = 0; kk < kD / 16; ++kk) {
+    const int r = wm * 16 + (lane & 15);
+    ldsm_x4(sq + tile_at<kCh>(r, kk * 2 + (lane >> 4)), qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3]);
+  }
+
+  for (int t = t0; t < t1; ++t) {
+    cp_async_wait<kStages - 2>();
+    if (kWM == 4) __syncthreads();
+    else __syncwarp();
+    if (t + kStages - 1 < t1) load(t + kStages - 1);  // into the slot of tile t - 1, which all have left
+    cp_async_commit();
+    const uint32_t sk = ring + (t % kStages) * 2 * Cf::kTileBytes, sv = sk + Cf::kTileBytes;
+    const int key0 = t * kKT + wk * kKW;
+    if (key0 >= len) continue;
+
+    float bias[kBias ? kKW / 8 : 1][4];
+    if (kBias) {
+#pragma unroll
+      for (int j = 0; j < kKW / 8; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = key0 + j * 8 + (lane & 3) * 2 + (e & 1);
+          bias[kBias ? j : 0][e] = key < len ? __ldg(brow[e >> 1] + key) : 0.f;
+        }
+      }
+    }
+    float s[kKW / 8][4];
+#pragma unroll
+    for (int j = 0; j < kKW / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < kD / 16; ++kk) {
+#pragma unroll
+      for (int jp = 0; jp < kKW / 16; ++jp) {  // pairs of 8-key blocks
+        const int r = wk * kKW + jp * 16 + (lane & 7) + (lane >> 4) * 8;
+        uint32_t b0, b1, b2, b3;
+        ldsm_x4(sk + tile_at<kCh>(r, kk * 2 + ((lane >> 3) & 1)), b0, b1, b2, b3);
+        mma16816<kBf16>(s[2 * jp], qf[kk], b0, b1);
+        mma16816<kBf16>(s[2 * jp + 1], qf[kk], b2, b3);
+      }
+    }
+    if (kBias) {
+#pragma unroll
+      for (int j = 0; j < kKW / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[j][e] = fmaf(s[j][e], p.scale, bias[kBias ? j : 0][e]);
+    }
+    if (mg || key0 + kKW > len) {
+#pragma unroll
+      for (int j = 0; j < kKW / 8; ++j) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int key = key0 + j * 8 + (lane & 3) * 2 + e;
+          if (key >= len || (mg && mg[key] == 0)) s[j][e] = s[j][2 + e] = -INFINITY;
+        }
+      }
+    }
+    // online softmax: rows lane/4 and lane/4 + 8 of the warp's 16
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kKW / 8; ++j) mx = fmaxf(mx, fmaxf(s[j][2 * h], s[j][2 * h + 1]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float m_new = fmaxf(m_run[h], mx);
+      const float base = m_new == -INFINITY ? 0.f : m_new;  // nothing counted yet: every p is 0
+      const float corr = ex2((m_run[h] - base) * to_log2);
+      m_run[h] = m_new;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < kKW / 8; ++j) {
+        s[j][2 * h] = ex2((s[j][2 * h] - base) * to_log2);
+        s[j][2 * h + 1] = ex2((s[j][2 * h + 1] - base) * to_log2);
+        sum += s[j][2 * h] + s[j][2 * h + 1];
+      }
+      l_run[h] = l_run[h] * corr + sum;
+#pragma unroll
+      for (int j = 0; j < kD / 8; ++j) {
+        acc[j][2 * h] *= corr;
+        acc[j][2 * h + 1] *= corr;
+      }
+    }
+    // O += P V, P rounded to the operands' type
+#pragma unroll
+    for (int kk = 0; kk < kKW / 16; ++kk) {
+      uint32_t pa[4];
+      pa[0] = pack2<kBf16>(s[2 * kk][0], s[2 * kk][1]);
+      pa[1] = pack2<kBf16>(s[2 * kk][2], s[2 * kk][3]);
+      pa[2] = pack2<kBf16>(s[2 * kk + 1][0], s[2 * kk + 1][1]);
+      pa[3] = pack2<kBf16>(s[2 * kk + 1][2], s[2 * kk + 1][3]);
+#pragma unroll
+      for (int jp = 0; jp < kD / 16; ++jp) {  // pairs of 8-wide column blocks
+        const int r = wk * kKW + kk * 16 + (lane & 15);
+        uint32_t b0, b1, b2, b3;
+        ldsm_x4_t(sv + tile_at<kCh>(r, jp * 2 + (lane >> 4)), b0, b1, b2, b3);
+        mma16816<kBf16>(acc[2 * jp], pa, b0, b1);
+        mma16816<kBf16>(acc[2 * jp + 1], pa, b2, b3);
+      }
+    }
+  }
+
+  // Partial results into shared memory (over the ring, which nothing reads
+  // or fills any more).
+  cp_async_wait<0>();
+  __syncthreads();
+  float* part = reinterpret_cast<float*>(smem + Cf::kQBytes);
+  const int r_lo = wm * 16 + (lane >> 2);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float l = l_run[h];
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if ((lane & 3) == 0) ml[wk][r_lo + 8 * h] = make_float2(m_run[h], l);
+    float* dst = part + (wk * Cf::kRows + r_lo + 8 * h) * Cf::kOPitch + (lane & 3) * 2;
+#pragma unroll
+    for (int j = 0; j < kD / 8; ++j)
+      *reinterpret_cast<float2*>(dst + j * 8) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+  }
+  __syncthreads();
+  // The weight of each key warp's partial row against the row's maximum over
+  // this CTA, and over the cluster.
+  if (kWK > 1 || splits > 1) {
+    if (tid < Cf::kRows) {
+      float m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWK; ++w) m = fmaxf(m, ml[w][tid].x);
+      const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int w = 0; w < kWK; ++w) {
+        const float f = ex2((ml[w][tid].x - base) * to_log2);
+        wgt[w][tid] = f;
+        l = fmaf(f, ml[w][tid].y, l);
+      }
+      ml[0][tid] = make_float2(m, l);
+    }
+    if (kWK == 1) cluster_sync();
+    else __syncthreads();
+  }
+  if (kWK > 1 && splits > 1) {
+    // one partial tile per CTA for the others to read
+    for (int i = tid; i < Cf::kRows * kD / 4; i += kThreads) {
+      const int r = i / (kD / 4), c = (i % (kD / 4)) * 4;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWK; ++w) {
+        const float f = wgt[w][r];
+        const float4 x = *reinterpret_cast<const float4*>(part + (w * Cf::kRows + r) * Cf::kOPitch + c);
+        a.x = fmaf(f, x.x, a.x);
+        a.y = fmaf(f, x.y, a.y);
+        a.z = fmaf(f, x.z, a.z);
+        a.w = fmaf(f, x.w, a.w);
+      }
+      *reinterpret_cast<float4*>(part + r * Cf::kOPitch + c) = a;
+    }
+    cluster_sync();
+  }
+  // Rows to the output, 8 elements a thread; with a cluster each CTA sums a
+  // share of them over all CTAs, in rank order.
+  const int out_chunks = p.head_dim / 8;
+  const uint32_t part_s = smem_u32(part), ml_s = smem_u32(&ml[0][0]);
+  for (int i = tid + kThreads * split; i < Cf::kRows * out_chunks; i += kThreads * splits) {
+    const int r = i / out_chunks, c = (i % out_chunks) * 8;
+    if (row0 + r >= p.rows) break;
+    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f;
+    if (splits > 1) {
+      float m = -INFINITY;
+      for (int w = 0; w < splits; ++w) m = fmaxf(m, ld_cluster_f2(mapa_shared(ml_s + r * 8, w)).x);
+      const float base = m == -INFINITY ? 0.f : m;
+      for (int w = 0; w < splits; ++w) {
+        const float2 s = ld_cluster_f2(mapa_shared(ml_s + r * 8, w));
+        const float f = ex2((s.x - base) * to_log2);
+        l = fmaf(f, s.y, l);
+        const uint32_t src = mapa_shared(part_s + (r * Cf::kOPitch + c) * 4, w);
+        const float4 x = ld_cluster_f4(src), y = ld_cluster_f4(src + 16);
+        o[0] = fmaf(f, x.x, o[0]);
+        o[1] = fmaf(f, x.y, o[1]);
+        o[2] = fmaf(f, x.z, o[2]);
+        o[3] = fmaf(f, x.w, o[3]);
+        o[4] = fmaf(f, y.x, o[4]);
+        o[5] = fmaf(f, y.y, o[5]);
+        o[6] = fmaf(f, y.z, o[6]);
+        o[7] = fmaf(f, y.w, o[7]);
+      }
+    } else {
+      l = ml[0][r].y;
+#pragma unroll
+      for (int w = 0; w < kWK; ++w) {
+        const float f = kWK > 1 ? wgt[w][r] : 1.f;
+        const float* src = part + (w * Cf::kRows + r) * Cf::kOPitch + c;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = fmaf(f, src[e], o[e]);
+      }
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays NaN
+    const int row = row0 + r;
+    uint4 w4;
+    w4.x = pack2<kBf16>(o[0] * inv, o[1] * inv);
+    w4.y = pack2<kBf16>(o[2] * inv, o[3] * inv);
+    w4.z = pack2<kBf16>(o[4] * inv, o[5] * inv);
+    w4.w = pack2<kBf16>(o[6] * inv, o[7] * inv);
+    *reinterpret_cast<uint4*>(p.o + b * p.ob + (row / p.group) * p.os +
+                              static_cast<int64_t>(kvh * p.group + row % p.group) * p.oh + c) = w4;
+  }
+  if (splits > 1) cluster_sync();  // the others may still read this CTA's partial rows
+}
+
+template <bool kBf16, int kD, int kWM, bool kBias>
+int launch_variant(const CrossParams& p, cudaStream_t st) {
+  using Cf = Cfg<kD, kWM>;
+  const auto kernel = cross_mma_kernel<kBf16, kD, kWM, kBias>;
+  static std::atomic<uint64_t> ready{0};  // devices whose attributes are set
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return kErrCuda;
+  if (dev >= 64 || !(ready.load() >> dev & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::kSmem) != cudaSuccess)
+      return kErrCuda;
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  const int64_t row_tiles = (static_cast<int64_t>(p.rows) + Cf::kRows - 1) / Cf::kRows;
+  const int64_t items = row_tiles * p.kv_heads * p.batch;
+  const int key_tiles = (p.sk + Cf::kKT - 1) / Cf::kKT;
+  int splits = 1;
+  while (splits < 8 && items * splits * 2 <= 2 * num_sms() && key_tiles >= 2 * splits) splits *= 2;
+  if (items * splits > 0x7fffffffLL) return kErrShape;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(items * splits));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Cf::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  if (splits > 1) {
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = splits;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+  }
+  count_launches(1);
+  return cudaLaunchKernelEx(&cfg, kernel, p, static_cast<int>(row_tiles), splits) == cudaSuccess ? kOk : kErrLaunch;
+}
+
+template <bool kBf16, int kD>
+int launch_rows(const CrossParams& p, cudaStream_t st) {
+  if (p.rows <= 16)
+    return p.bias ? launch_variant<kBf16, kD, 1, true>(p, st) : launch_variant<kBf16, kD, 1, false>(p, st);
+  return p.bias ? launch_variant<kBf16, kD, 4, true>(p, st) : launch_variant<kBf16, kD, 4, false>(p, st);
+}
+
+}  // namespace
+
+int launch_cross_mma(const CrossParams& p, int dtype, cudaStream_t st) {
+  const bool bf = dtype == kBF16;
+  if (p.head_dim <= 32) return bf ? launch_rows<true, 32>(p, st) : launch_rows<false, 32>(p, st);
+  if (p.head_dim <= 64) return bf ? launch_rows<true, 64>(p, st) : launch_rows<false, 64>(p, st);
+  return bf ? launch_rows<true, 128>(p, st) : launch_rows<false, 128>(p, st);
+}
+
+}  // namespace s3
+
+using namespace s3;
+
+extern "C" int sam3cu_cross_attention(const struct sam3cu_cross_attention_args* a, void* stream) {
+  if (!a) return SAM3CU_EINVAL;
+  if (a->dtype != SAM3CU_BF16 && a->dtype != SAM3CU_F16) return SAM3CU_EDTYPE;
+  if (a->batch < 0 || a->sq < 0 || a->sk < 0 || a->q_heads < 0 || a->kv_heads < 1 || a->head_dim < 1)
+    return SAM3CU_EINVAL;
+  if (a->q_heads % a->kv_heads) return SAM3CU_EINVAL;
+  if (!(a->scale >= 0.f) || std::isinf(a->scale)) return SAM3CU_EINVAL;
+  if (a->head_dim % 8 || a->head_dim > 128) return SAM3CU_ESHAPE;
+  if (a->batch == 0 || a->sq == 0 || a->q_heads == 0) return SAM3CU_OK;
+  const int group = a->q_heads / a->kv_heads;
+  if (a->sk > 0x7fffff00) return SAM3CU_ESHAPE;
+  if (group > 128 || static_cast<int64_t>(a->sq) * group > 0x7fffff00LL) return SAM3CU_ESHAPE;
+  if (!a->q || !a->o || (a->sk > 0 && (!a->k || !a->v))) return SAM3CU_EINVAL;
+  CrossParams p;
+  memset(&p, 0, sizeof(p));
+  const int64_t* from[4] = {a->q_strides, a->k_strides, a->v_strides, a->o_strides};
+  int64_t* to[4][3] = {{&p.qb, &p.qs, &p.qh}, {&p.kb, &p.ks, &p.kh}, {&p.vb, &p.vs, &p.vh}, {&p.ob, &p.os, &p.oh}};
+  const void* base[4] = {a->q, a->k, a->v, a->o};
+  for (int t = 0; t < 4; ++t) {
+    const int extent[3] = {a->batch, t == 0 || t == 3 ? a->sq : a->sk, t == 0 || t == 3 ? a->q_heads : a->kv_heads};
+    if (reinterpret_cast<uintptr_t>(base[t]) & 15) return SAM3CU_ESHAPE;
+    for (int i = 0; i < 3; ++i) {
+      if (from[t][i] < 0) return SAM3CU_EINVAL;
+      if (extent[i] <= 1) continue;  // the stride of a single element says nothing
+      if (from[t][i] % 8) return SAM3CU_ESHAPE;
+      if (t == 3 && from[t][i] == 0) return SAM3CU_EINVAL;  // every output element has a place of its own
+      *to[t][i] = from[t][i];
+    }
+  }
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.k = static_cast<const uint16_t*>(a->k);
+  p.v = static_cast<const uint16_t*>(a->v);
+  p.o = static_cast<uint16_t*>(a->o);
+  p.batch = a->batch;
+  p.sq = a->sq;
+  p.sk = a->sk;
+  p.kv_heads = a->kv_heads;
+  p.group = group;
+  p.head_dim = a->head_dim;
+  p.rows = a->sq * group;
+  p.scale = a->scale > 0.f ? a->scale : 1.f / sqrtf(static_cast<float>(a->head_dim));
+  p.scale_log2 = p.scale * 1.4426950408889634f;
+  if (a->k_lens) {
+    if (reinterpret_cast<uintptr_t>(a->k_lens) & 3) return SAM3CU_EINVAL;
+    p.k_lens = a->k_lens;
+  }
+  if (a->key_mask) {
+    if (a->mask_stride < 0) return SAM3CU_EINVAL;
+    p.key_mask = a->key_mask;
+    p.mask_stride = a->mask_stride;
+  }
+  if (a->bias) {
+    if (reinterpret_cast<uintptr_t>(a->bias) & 3) return SAM3CU_EINVAL;
+    for (int i = 0; i < 3; ++i)
+      if (a->bias_strides[i] < 0) return SAM3CU_EINVAL;
+    p.bias = a->bias;
+    p.bb = a->bias_strides[0];
+    p.bh = a->bias_strides[1];
+    p.bs = a->bias_strides[2];
+  }
+  return launch_cross_mma(p, a->dtype, static_cast<cudaStream_t>(stream));
+}

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from typing import Optional
 
 import numpy as np
@@ -21,6 +22,9 @@ LIB_PATH = os.environ.get("SAM3CU_LIB") or os.path.join(HERE, "lib", "libsam3cu.
 F32, F16, BF16, Q8_0 = 0, 1, 2, 5
 ACT_NONE, ACT_GELU_TANH = 0, 1
 EMODEL, ENOENT = -5, -109
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_NTK, ROPE_SCALE_YARN, ROPE_SCALE_BANDS = range(5)
+NORM_RMS, NORM_LAYER = 1, 2
 
 EXPORTS = (
     "sam3cu_init", "sam3cu_strerror", "sam3cu_last_device_error",
@@ -38,6 +42,7 @@ EXPORTS = (
     "sam3cu_sam3_check", "sam3cu_sam3_find", "sam3cu_vit_create_from_sam3", "sam3cu_vit_get_config",
     "sam3cu_neck_create", "sam3cu_neck_forward", "sam3cu_neck_forward_async", "sam3cu_neck_out_size",
     "sam3cu_neck_stream", "sam3cu_neck_destroy",
+    "sam3cu_rope_freqs_init", "sam3cu_rope_pos", "sam3cu_qk_norm_rope", "sam3cu_cross_attention",
 )
 
 # sizeof(struct sam3_cuda_backend): {enum type; ops*} + int device + void *impl
@@ -115,6 +120,10 @@ def lib():
         L.sam3cu_tinyvit_encode.argtypes = [vp, vp, i32, vp, i32]
         L.sam3cu_tinyvit_grid.argtypes = [vp]
         L.sam3cu_tinyvit_destroy.argtypes = [vp]
+        L.sam3cu_rope_freqs_init.argtypes = [vp, vp]
+        L.sam3cu_rope_pos.argtypes = [vp, vp, i32, i32, i32, i32, vp, i64, i64, vp, vp]
+        L.sam3cu_qk_norm_rope.argtypes = [vp, vp, i32, i32, i32, i32, i32, C.c_float, vp, i64, i64, vp, vp]
+        L.sam3cu_cross_attention.argtypes = [vp, vp]
         _lib = L
     return _lib
 
@@ -257,6 +266,186 @@ def conv2d_nhwc_noalloc(x, w, bias=None, stride=1, pad=0, out=None):
     check(lib().sam3cu_conv2d_nhwc_noalloc(_ptr(x), _ptr(w), _f32(bias, 'bias'), _ptr(out),
                                            dtype_code(x), n, H, W, C, OC, kh, kw, stride, pad,
                                            _stream()), "sam3cu_conv2d_nhwc_noalloc")
+    return out
+
+
+# ------------------------- attention over an encoder's states (decoder side)
+_HEAD_VIEW = struct.Struct("P3qP3qi4xPP")          # struct sam3cu_head_view
+_CROSS_ARGS = struct.Struct("4P12q7ifPPqP3q")      # struct sam3cu_cross_attention_args
+
+
+class _RopeConfig(C.Structure):
+    _fields_ = ([(n, C.c_int) for n in ("rot_dim", "layout", "scaling")]
+                + [(n, C.c_double) for n in ("theta", "factor", "trained_len", "beta_fast", "beta_slow", "low_freq",
+                                             "high_freq", "amplitude")])
+
+
+class _RopeFreqs(C.Structure):
+    _fields_ = [("n_pairs", C.c_int), ("layout", C.c_int), ("amplitude", C.c_float), ("turns", C.c_double * 128)]
+
+
+class RopeFreqs:
+    """The angles of a rotary position encoding (sam3cu_rope_freqs_init):
+    rot_dim elements of each head rotate, in the ROPE_HALF or
+    ROPE_INTERLEAVED layout; scaling is one of ROPE_SCALE_*.  Host data, good
+    for every device; make it once."""
+
+    def __init__(self, rot_dim: int, layout: int = ROPE_HALF, scaling: int = ROPE_SCALE_NONE, theta: float = 10000.0,
+                 factor: float = 1.0, trained_len: float = 4096, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                 low_freq: float = 1.0, high_freq: float = 4.0, amplitude: float = 0.0):
+        cfg = _RopeConfig(rot_dim, layout, scaling, theta, factor, trained_len, beta_fast, beta_slow, low_freq,
+                          high_freq, amplitude)
+        self._c = _RopeFreqs()
+        check(lib().sam3cu_rope_freqs_init(C.byref(cfg), C.byref(self._c)), "sam3cu_rope_freqs_init")
+        self.ptr = C.addressof(self._c)
+        self.rot_dim = rot_dim
+
+    @property
+    def turns(self) -> np.ndarray:
+        """Revolutions per position of each pair, float64 [rot_dim / 2]."""
+        return np.array(self._c.turns[:self._c.n_pairs])
+
+    @property
+    def amplitude(self) -> float:
+        return self._c.amplitude
+
+
+def _here(device):
+    """The calls launch on the current device, where their tensors must be."""
+    import torch
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise ValueError(f"tensors must be on the current CUDA device, not on {device}")
+
+
+def _like(t, x, shape, what):
+    if t.dtype != x.dtype or t.device != x.device or t.shape != shape or (t.stride(-1) != 1 and shape[-1] > 1):
+        raise ValueError(f"{what} must be a {x.dtype} tensor of shape {tuple(shape)} on {x.device} with contiguous "
+                         f"last dimension")
+    return t
+
+
+def _head_param(t, x, what):
+    if t is None:
+        return 0
+    if t.shape != x.shape[-1:] or t.device != x.device:
+        raise ValueError(f"{what} must be [head_dim] on {x.device}")
+    return _f32(t, what)
+
+
+def _head_view(x, out, q, gamma, beta, what):
+    """x [batch, seq, heads, head_dim] like q, any strides but the last."""
+    import torch
+    if x.dim() != 4 or x.shape[:2] != q.shape[:2] or x.shape[3] != q.shape[3]:
+        raise ValueError("q and k must be [batch, seq, heads, head_dim], alike but in heads")
+    _like(x, q, x.shape, what)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        _like(out, q, x.shape, "the output of " + what)
+    xs, ys = x.stride(), out.stride()
+    return out, _HEAD_VIEW.pack(x.data_ptr(), xs[0], xs[1], xs[2], out.data_ptr(), ys[0], ys[1], ys[2], x.shape[2],
+                                _head_param(gamma, x, "gamma"), _head_param(beta, x, "beta"))
+
+
+def _positions(positions, x):
+    """Pointer and batch stride of int64 positions [seq], [1, seq] or [batch, seq]."""
+    import torch
+    if positions is None:
+        return None, 0
+    batch, seq = x.shape[:2]
+    if positions.dtype != torch.int64 or positions.device != x.device or positions.dim() not in (1, 2) \
+            or positions.shape[-1] != seq or (positions.stride(-1) != 1 and seq > 1):
+        raise ValueError(f"positions must be int64 [batch, seq] or [seq] on {x.device}, contiguous along seq")
+    if positions.dim() == 1 or positions.shape[0] == 1:
+        return positions.data_ptr(), 0
+    if positions.shape[0] != batch:
+        raise ValueError(f"positions for {positions.shape[0]} sequences, not {batch}")
+    return positions.data_ptr(), positions.stride(0)
+
+
+def rope_pos(q, freqs: RopeFreqs, positions=None, start: int = 0, k=None, out=None, k_out=None):
+    """Rotate the heads of q (and k) [batch, seq, heads, head_dim] by their
+    tokens' positions (int64 tensor [batch, seq] or [seq], else start,
+    start + 1, ...): sam3cu_rope_pos.  out / k_out may be q / k themselves.
+    Returns q's rotation, with k the pair."""
+    _here(q.device)
+    out, qv = _head_view(q, out, q, None, None, "q")
+    kv = None
+    if k is not None:
+        k_out, kv = _head_view(k, k_out, q, None, None, "k")
+    pos, stride = _positions(positions, q)
+    check(lib().sam3cu_rope_pos(qv, kv, dtype_code(q), q.shape[0], q.shape[1], q.shape[3], pos, stride, start,
+                                freqs.ptr, _stream()), "sam3cu_rope_pos")
+    return out if k is None else (out, k_out)
+
+
+def qk_norm_rope(q, k, q_gamma=None, k_gamma=None, q_beta=None, k_beta=None, norm: int = NORM_RMS, eps: float = 1e-6,
+                 freqs: Optional[RopeFreqs] = None, positions=None, start: int = 0, out=None, k_out=None):
+    """Normalise every head of q and k [batch, seq, heads, head_dim] (k may
+    be None) over its elements, then rotate as rope_pos does (freqs None: no
+    rotation), in one pass: sam3cu_qk_norm_rope.  gamma and beta: float32
+    [head_dim] or None."""
+    _here(q.device)
+    out, qv = _head_view(q, out, q, q_gamma, q_beta, "q")
+    kv = None
+    if k is not None:
+        k_out, kv = _head_view(k, k_out, q, k_gamma, k_beta, "k")
+    pos, stride = _positions(positions, q) if freqs is not None else (None, 0)
+    check(lib().sam3cu_qk_norm_rope(qv, kv, dtype_code(q), q.shape[0], q.shape[1], q.shape[3], norm, eps, pos, stride,
+                                    start, freqs.ptr if freqs is not None else None, _stream()),
+          "sam3cu_qk_norm_rope")
+    return out if k is None else (out, k_out)
+
+
+def cross_attention(q, k, v, k_lens=None, key_mask=None, bias=None, scale: float = 0.0, out=None):
+    """Attention of q [batch, sq, q_heads, head_dim] over k, v [batch, sk,
+    kv_heads, head_dim] (BF16 or F16, any strides but the last, expanded
+    dimensions included): sam3cu_cross_attention.
+
+    k_lens: int32 [batch], the keys of each sequence that count; key_mask:
+    bool or uint8 [batch or 1, sk], True where a key counts; bias: float32,
+    added to the scaled scores, of a shape that broadcasts to [batch, q_heads,
+    sq, sk] (its last dimension sk); scale 0: 1/sqrt(head_dim).  A query left
+    without keys gives zeros."""
+    import torch
+    _here(q.device)
+    if q.dim() != 4 or k.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError("q must be [batch, sq, q_heads, head_dim], k and v [batch, sk, kv_heads, head_dim]")
+    batch, sq, q_heads, head_dim = q.shape
+    sk, kv_heads = k.shape[1], k.shape[2]
+    _like(q, q, q.shape, "q")
+    _like(k, q, k.shape, "k")
+    _like(v, q, k.shape, "v")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _like(out, q, q.shape, "out")
+    lens = mask = bptr = 0
+    mask_stride, bs = 0, (0, 0, 0)
+    if k_lens is not None:
+        if k_lens.dtype != torch.int32 or k_lens.shape != (batch,) or k_lens.device != q.device \
+                or not k_lens.is_contiguous():
+            raise ValueError(f"k_lens must be a contiguous int32 [batch] tensor on {q.device}")
+        lens = k_lens.data_ptr()
+    if key_mask is not None:
+        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.dim() != 2 or key_mask.device != q.device \
+                or key_mask.shape[0] not in (1, batch) or key_mask.shape[1] != sk \
+                or (key_mask.stride(1) != 1 and sk > 1):
+            raise ValueError(f"key_mask must be a bool or uint8 [batch or 1, sk] tensor on {q.device}, contiguous "
+                             f"along sk")
+        mask, mask_stride = key_mask.data_ptr(), key_mask.stride(0) if key_mask.shape[0] > 1 else 0
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.device != q.device or bias.dim() > 4 or bias.dim() < 1 \
+                or bias.shape[-1] != sk or (bias.stride(-1) != 1 and sk > 1):
+            raise ValueError(f"bias must be a float32 tensor on {q.device} that broadcasts to [batch, q_heads, sq, "
+                             f"sk], contiguous along sk")
+        bs = bias.expand(batch, q_heads, sq, sk).stride()
+        bptr = bias.data_ptr()
+    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
+    args = _CROSS_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qs[0], qs[1], qs[2], ks[0],
+                            ks[1], ks[2], vs[0], vs[1], vs[2], os_[0], os_[1], os_[2], dtype_code(q), batch, sq, sk,
+                            q_heads, kv_heads, head_dim, scale, lens, mask, mask_stride, bptr, bs[0], bs[1], bs[2])
+    check(lib().sam3cu_cross_attention(args, _stream()), "sam3cu_cross_attention")
     return out
 
 
