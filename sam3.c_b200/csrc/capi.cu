@@ -5,6 +5,7 @@
 #include <mutex>
 
 #include "../../include/sam3cu.h"
+#include "cross_attention.cuh"
 #include "gemm_sm100.cuh"
 #include "misc.cuh"
 #include "sam3cu_internal.h"
@@ -156,8 +157,8 @@ const char* sam3cu_strerror(int s) {
 unsigned int sam3cu_last_device_error(void) {
   cudaDeviceSynchronize();
   unsigned int a = dev_error_gemm(), b = dev_error_attn(), c = dev_error_misc(), d = dev_error_attn_tc(),
-               e = dev_error_gemm2();
-  return a ? a : (b ? b : (c ? c : (d ? d : e)));
+               e = dev_error_gemm2(), f = dev_error_cross();
+  return a ? a : (b ? b : (c ? c : (d ? d : (e ? e : f))));
 }
 
 uint64_t sam3cu_launch_count(int reset) {

@@ -90,20 +90,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
-__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-  return v;
-}
-
 // kD: head_dim rounded up to 32, 64 or 128 (the copies fill the rest with
 // zeros).  kWM: row warps of the CTA (4 / kWM warps split the keys of a tile).
 template <int kD, int kWM>
@@ -533,5 +519,7 @@ extern "C" int sam3cu_cross_attention(const struct sam3cu_cross_attention_args* 
     p.bh = a->bias_strides[1];
     p.bs = a->bias_strides[2];
   }
-  return launch_cross_mma(p, a->dtype, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (cross_tc_takes(p) && p.rows > 64 && p.sk > 256) return launch_cross_tc(p, a->dtype, st);
+  return launch_cross_mma(p, a->dtype, st);
 }

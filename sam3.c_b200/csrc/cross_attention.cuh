@@ -32,6 +32,25 @@ __device__ __forceinline__ int cross_len(const CrossParams& p, int b) {
   return p.k_lens ? max(0, min(p.k_lens[b], p.sk)) : p.sk;
 }
 
+// Distributed shared memory of the cluster.
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
 int launch_cross_mma(const CrossParams& p, int dtype, cudaStream_t st);
+// cross_attention_sm100.cu: whether the tensor maps can describe the call.
+bool cross_tc_takes(const CrossParams& p);
+int launch_cross_tc(const CrossParams& p, int dtype, cudaStream_t st);
+unsigned int dev_error_cross();
 
 }  // namespace s3

@@ -1,0 +1,594 @@
+// cross_attention_sm100.cu - attention of many queries over states of another
+// length on the fifth-generation tensor cores.
+//
+//   S_j = Q K_j^T     tcgen05.mma 128 x 128 x D, accumulator in TMEM
+//   P_j = exp2(S_j c - m)   one thread per query row, 16-bit pairs to TMEM
+//   O  += P_j V_j     tcgen05.mma 128 x D x 128, A = P from TMEM
+//
+// with the running maximum and sum of each row (rows, heads and keys as in
+// cross_attention.cuh).  One CTA per SM computes two 128-row tiles against the
+// same K and V: while one tile's softmax runs on the exponential units the
+// tensor cores work for the other, and a K / V tile read from L2 serves 256
+// rows.  Twelve warps:
+//   warp 0      TMA: the Q tiles, then K and V through rings of their own
+//   warp 1      MMA issue and the TMEM allocation
+//   warp 2      with a mask or lengths: key bits of each tile, and zeros over
+//               V rows of keys that do not count (0 * NaN would reach O)
+//   warps 4-7, 8-11   softmax and epilogue of tile 0 and 1; warp w owns TMEM
+//               lanes 32 (w % 4) .. + 31, a thread a whole row of S
+// TMEM (512 columns): S0 S1 (128 each), O0 O1 (D each), and for D <= 64
+// P0 P1 (64 each), so that S of the next key tile is computed while the
+// softmax of this one runs; for D = 128 P takes the place of its S.
+// O is rescaled lazily, when a row's maximum has grown by more than 2^8.
+// Every mbarrier wait is bounded.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <cstdint>
+#include <cstring>
+
+#include "attention_math.cuh"
+#include "cross_attention.cuh"
+#include "sam3cu_internal.h"
+#include "sm100_ptx.cuh"
+#include "tma_host.cuh"
+
+namespace s3 {
+
+S3_DEV_ERROR_ACCESSOR(dev_error_cross)
+
+namespace {
+
+constexpr int kQ = 128;        // rows of a tile
+constexpr int kKV = 128;       // keys of a tile
+constexpr int kThreads = 384;
+constexpr int kSoftThreads = 256;
+constexpr float kRescaleLog2 = 8.f;
+// f16 P below 2^-14 loses bits: with a maximum of 2^8 (lazy rescaling) there
+// is room for a factor 2^6 under 65504.  It cancels in O / sum.
+constexpr float kF16Shift = 6.f;
+
+template <int kD>
+struct Cfg {
+  static constexpr int kRowBytes = kD == 32 ? 64 : 128;  // a swizzled row (half of one for D = 128)
+  static constexpr int kHalves = kD == 128 ? 2 : 1;
+  static constexpr int kTile = 128 * kD * 2;             // Q, K or V tile
+  static constexpr int kStages = kD == 128 ? 2 : kD == 64 ? 4 : 8;  // of K, and of V
+  static constexpr int kSmem = 2 * kTile + 2 * kStages * kTile;
+  // one CTA per SM: each allocates all of TMEM
+  static_assert(kSmem > 116 * 1024 && kSmem < 226 * 1024, "one CTA per SM");
+  static constexpr bool kOwnP = kD <= 64;                // P beside S
+  static constexpr uint32_t kOCol = 256, kPCol = 256 + 2 * kD;
+  static constexpr int kPitch = kD + 4;                  // floats of a partial row
+  static_assert(2 * kQ * kPitch * 4 <= kSmem, "partial rows fit over the rings");
+};
+
+struct TcParams {
+  CrossParams c;
+  int qpt;        // queries of a tile: 128 / group
+  int items_x;    // row items of a (batch, key head)
+  int tiles;      // 128-row tiles of an item: 1 or 2
+  int splits;     // CTAs of the cluster that share an item's keys
+  int kmul_b, kmul_h, vmul_b, vmul_h, qmul_b;  // 0: that dimension is shared
+};
+
+template <bool kBf16, int kD, bool kMask>
+__global__ void __launch_bounds__(kThreads, 1)
+    cross_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                    const __grid_constant__ CUtensorMap tv, const __grid_constant__ TcParams prm) {
+  using Cf = Cfg<kD>;
+  constexpr int kStages = Cf::kStages, kTile = Cf::kTile;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ uint64_t bars[1 + 2 * 6 + 4 * kStages + 2 * kStages];
+  __shared__ uint32_t bits[kMask ? kStages : 1][4];
+  __shared__ float2 ml[2 * kQ];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag_s;
+  uint64_t* q_full = &bars[0];
+  uint64_t* s_full = &bars[1];    // [2] by tile
+  uint64_t* s_empty = &bars[3];   // [2]
+  uint64_t* p_full = &bars[5];    // [2]
+  uint64_t* p_empty = &bars[7];   // [2]
+  uint64_t* o_full = &bars[9];    // [2]
+  uint64_t* k_full = &bars[13];
+  uint64_t* k_empty = k_full + kStages;
+  uint64_t* v_full = k_empty + kStages;
+  uint64_t* v_empty = v_full + kStages;
+  uint64_t* v_ready = v_empty + kStages;  // kMask: V of the tile is scrubbed
+  uint64_t* w_ready = v_ready + kStages;  // kMask: the tile's key bits are there
+  volatile int* abort_flag = &abort_flag_s;
+
+  const CrossParams& p = prm.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = blockIdx.x % prm.splits, item = blockIdx.x / prm.splits;
+  const int ix = item % prm.items_x, bh = item / prm.items_x;
+  const int kvh = bh % p.kv_heads, b = bh / p.kv_heads;
+  const int q0 = ix * prm.tiles * prm.qpt;  // first query of the item
+  const int tiles = min(prm.tiles, (p.sq - q0 + prm.qpt - 1) / prm.qpt);
+  const int len = cross_len(p, b);
+  const int all_kv = (len + kKV - 1) / kKV;
+  const int j0 = static_cast<int>(static_cast<int64_t>(all_kv) * split / prm.splits);
+  const int n_kv = static_cast<int>(static_cast<int64_t>(all_kv) * (split + 1) / prm.splits) - j0;
+
+  uint8_t* sQ = smem;
+  auto sK = [&](int st) { return smem + 2 * kTile + st * kTile; };
+  auto sV = [&](int st) { return smem + 2 * kTile + (kStages + st) * kTile; };
+  const bool aligned = (smem_u32(smem) & 1023u) == 0;  // the swizzled layouts need it
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&s_empty[t], 4);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&p_empty[t], 1);
+      mbar_init(&o_full[t], 1);
+    }
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_ready[i], 1);
+      mbar_init(&w_ready[i], 1);
+    }
+    abort_flag_s = aligned ? 0 : 1;
+    if (!aligned) atomicCAS(&g_dev_error, 0u, static_cast<unsigned>(kErrTmemAlloc));
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  auto tS = [&](int t) { return tmem + static_cast<uint32_t>(t * 128); };
+  auto tO = [&](int t) { return tmem + Cf::kOCol + static_cast<uint32_t>(t * kD); };
+  auto tP = [&](int t) { return Cf::kOwnP ? tmem + Cf::kPCol + static_cast<uint32_t>(t * 64) : tS(t); };
+  const bool run = aligned && n_kv > 0;
+  auto keys_in = [&](int j) {  // keys of tile j, rounded up to a multiple of 16
+    const int left = len - (j0 + j) * kKV;
+    return left >= kKV ? kKV : ((left + 15) & ~15);
+  };
+
+  if (warp == 0 && run) {
+    // ------------------------------------------------------------ TMA
+    const int kb = b * prm.kmul_b, kh = kvh * prm.kmul_h, vb = b * prm.vmul_b, vh = kvh * prm.vmul_h;
+    if (elect_one()) {
+      tma_prefetch_desc(&tq);
+      tma_prefetch_desc(&tk);
+      tma_prefetch_desc(&tv);
+      mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(tiles * Cf::kHalves * Cf::kRowBytes * p.group * prm.qpt));
+      for (int t = 0; t < tiles; ++t)
+        for (int h = 0; h < Cf::kHalves; ++h)
+          tma_load_4d(sQ + t * kTile + h * (kTile / 2), &tq, q_full, h * 64, kvh * p.group, q0 + t * prm.qpt,
+                      b * prm.qmul_b);
+    }
+    __syncwarp();
+    for (int j = 0; j < n_kv; ++j) {
+      const int st = j % kStages;
+      const uint32_t ph = ((j / kStages) & 1) ^ 1;
+      if (!mbar_wait_warp(&k_empty[st], ph, kErrStageFree, abort_flag)) break;
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&k_full[st], kTile);
+        for (int h = 0; h < Cf::kHalves; ++h)
+          tma_load_4d(sK(st) + h * (kTile / 2), &tk, &k_full[st], h * 64, (j0 + j) * kKV, kh, kb);
+      }
+      __syncwarp();
+      if (!mbar_wait_warp(&v_empty[st], ph, kErrStageFree, abort_flag)) break;
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&v_full[st], kTile);
+        for (int h = 0; h < Cf::kHalves; ++h)
+          tma_load_4d(sV(st) + h * (kTile / 2), &tv, &v_full[st], h * 64, (j0 + j) * kKV, vh, vb);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 1 && run) {
+    // ------------------------------------------------------------ MMA
+    const uint32_t fmt = kBf16 ? 1u : 0u;
+    const uint32_t idesc_pv = make_idesc(fmt, kQ, kD, 1u);
+    auto sdesc_k = [](uint32_t a) { return kD == 32 ? make_sdesc_sw64(a) : make_sdesc_sw128(a); };
+    auto sdesc_mn = [](uint32_t a) { return kD == 32 ? make_sdesc_sw64_mn(a) : make_sdesc_sw128_mn(a); };
+    constexpr uint32_t kHalfStep = kTile / 2 >> 4;            // the second 64 columns of a D = 128 tile
+    constexpr uint32_t kVStep = 16 * Cf::kRowBytes >> 4;      // 16 keys of V
+    const uint64_t qdesc[2] = {sdesc_k(smem_u32(sQ)), sdesc_k(smem_u32(sQ + kTile))};
+    // S_t = Q_t K_j^T, once the softmax has read the S before it
+    auto issue_s = [&](int t, int j) -> bool {
+      const int st = j % kStages;
+      if (Cf::kOwnP && !mbar_wait_warp(&s_empty[t], (j & 1) ^ 1, kErrAccFree, abort_flag)) return false;
+      tc_fence_after();
+      const uint64_t kdesc = sdesc_k(smem_u32(sK(st)));
+      const uint32_t idesc_s = make_idesc(fmt, kQ, keys_in(j));
+#pragma unroll
+      for (int kk = 0; kk < kD / 16; ++kk) {  // 16 elements = 32 bytes along D
+        const uint64_t at = (kk / 4) * kHalfStep + 2 * (kk % 4);
+        umma_ss_warp(tS(t), qdesc[t] + at, kdesc + at, idesc_s, kk ? 1u : 0u);
+      }
+      umma_commit_warp(&s_full[t]);
+      return true;
+    };
+    auto issue_tile_s = [&](int j) -> bool {  // both tiles' S, then K_j is free
+      if (!mbar_wait_warp(&k_full[j % kStages], (j / kStages) & 1, kErrTmaWait, abort_flag)) return false;
+      for (int t = 0; t < tiles; ++t)
+        if (!issue_s(t, j)) return false;
+      umma_commit_warp(&k_empty[j % kStages]);
+      return true;
+    };
+    bool ok = mbar_wait_warp(q_full, 0, kErrTmaWait, abort_flag) && issue_tile_s(0);
+    for (int j = 0; ok && j < n_kv; ++j) {
+      const int st = j % kStages, n = keys_in(j);
+      if (Cf::kOwnP && j + 1 < n_kv && !issue_tile_s(j + 1)) break;  // beside the softmax of tile j
+      if (!mbar_wait_warp(&v_full[st], (j / kStages) & 1, kErrTmaWait, abort_flag)) break;
+      if (kMask && !mbar_wait_warp(&v_ready[st], (j / kStages) & 1, kErrTmaWait, abort_flag)) break;
+      if (!Cf::kOwnP && j + 1 < n_kv &&
+          !mbar_wait_warp(&k_full[(j + 1) % kStages], ((j + 1) / kStages) & 1, kErrTmaWait, abort_flag))
+        break;
+      const uint64_t vdesc = sdesc_mn(smem_u32(sV(st)));
+      for (int t = 0; ok && t < tiles; ++t) {
+        if (!mbar_wait_warp(&p_full[t], j & 1, kErrAccFull, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (n == kKV) {
+#pragma unroll
+          for (int kk = 0; kk < kKV / 16; ++kk)  // A = P from TMEM: 16 keys = 8 columns
+            umma_ts_warp(tO(t), tP(t) + kk * 8, vdesc + kk * kVStep, idesc_pv, (j | kk) ? 1u : 0u);
+        } else {
+          for (int kk = 0; kk < n / 16; ++kk)
+            umma_ts_warp(tO(t), tP(t) + kk * 8, vdesc + kk * kVStep, idesc_pv, (j | kk) ? 1u : 0u);
+        }
+        if (Cf::kOwnP) umma_commit_warp(&p_empty[t]);
+        if (j == n_kv - 1) umma_commit_warp(&o_full[t]);
+        // P has been consumed in issue order: its S columns may be written
+        if (!Cf::kOwnP && j + 1 < n_kv && !issue_s(t, j + 1)) ok = false;
+      }
+      if (!Cf::kOwnP && ok && j + 1 < n_kv) umma_commit_warp(&k_empty[(j + 1) % kStages]);
+      umma_commit_warp(&v_empty[st]);
+    }
+  } else if (kMask && warp == 2 && run) {
+    // ---------------------------------------------- key bits, V scrubbing
+    const uint8_t* mg = p.key_mask ? p.key_mask + b * p.mask_stride : nullptr;
+    for (int j = 0; j < n_kv; ++j) {
+      const int st = j % kStages;
+      // the bits' slot is free with its V stage: both softmaxes are past it
+      if (!mbar_wait_warp(&v_empty[st], ((j / kStages) & 1) ^ 1, kErrStageFree, abort_flag)) break;
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = (j0 + j) * kKV + i * 32 + lane;
+        const bool on = key < len && (!mg || mg[key] != 0);
+        w[i] = __ballot_sync(0xffffffffu, on);
+      }
+      if (lane < 4) bits[kMask ? st : 0][lane] = lane == 0 ? w[0] : lane == 1 ? w[1] : lane == 2 ? w[2] : w[3];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&w_ready[st]);
+      if (!mbar_wait_warp(&v_full[st], (j / kStages) & 1, kErrTmaWait, abort_flag)) break;
+      if ((w[0] & w[1] & w[2] & w[3]) != 0xffffffffu) {
+        const int n = keys_in(j);  // rows past it are not multiplied
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (!(w[i] >> lane & 1) && i * 32 + lane < n) {
+            uint8_t* row = sV(st) + (i * 32 + lane) * Cf::kRowBytes;
+            for (int h = 0; h < Cf::kHalves; ++h)
+#pragma unroll
+              for (int c = 0; c < Cf::kRowBytes; c += 16)
+                *reinterpret_cast<uint4*>(row + h * (kTile / 2) + c) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_ready[st]);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------ softmax + epilogue
+    const int t = (warp - 4) >> 2, quarter = warp & 3;
+    const int r = quarter * 32 + lane;  // row within the tile
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const float sl2 = p.scale_log2;
+    const int query = q0 + t * prm.qpt + r / p.group;
+    const bool row_live = t < tiles && r < prm.qpt * p.group && query < p.sq;
+    // a warp of dead rows only keeps the barriers going
+    const bool live = __any_sync(0xffffffffu, row_live);
+    float m_used = -INFINITY, l = 0.f;
+    bool ok = run && t < tiles;
+    for (int j = 0; ok && j < n_kv; ++j) {
+      const int st = j % kStages;
+      if (!warp_wait(&s_full[t], j & 1, kErrAccFull, abort_flag, lane)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t su[kKV];
+      float* sv = reinterpret_cast<float*>(su);
+      if (live) {
+#pragma unroll
+        for (int c = 0; c < kKV / 32; ++c)
+          tmem_ld_32x32b_x32(tS(t) + lane_off + c * 32, *reinterpret_cast<uint32_t(*)[32]>(su + c * 32));
+        tmem_ld_wait();
+      }
+      if (Cf::kOwnP) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_empty[t]);  // S may be overwritten
+      }
+      if (kMask) {
+        if (!warp_wait(&w_ready[st], (j / kStages) & 1, kErrTmaWait, abort_flag, lane)) { ok = false; break; }
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t w = bits[kMask ? st : 0][i];
+            if (w != 0xffffffffu) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                if (!(w >> c & 1)) sv[i * 32 + c] = -INFINITY;
+            }
+          }
+        }
+      } else if (live && (j0 + j + 1) * kKV > len) {  // the last tile's keys beyond the states
+        const int n = len - (j0 + j) * kKV;
+#pragma unroll
+        for (int c = 0; c < kKV; ++c)
+          if (c >= n) sv[c] = -INFINITY;
+      }
+      const float mt = live ? max128(sv) : -INFINITY;
+      const bool need = (mt - m_used) * sl2 > kRescaleLog2;  // false for -inf - -inf
+      // P (its own columns) is free, and O at rest, after the P.V before it;
+      // with P in S's columns s_full said so already
+      if (Cf::kOwnP && j > 0 && !warp_wait(&p_empty[t], (j & 1) ^ 1, kErrAccFull, abort_flag, lane)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (__any_sync(0xffffffffu, need)) {
+        const float m_new = fmaxf(m_used, mt);
+        const float corr = m_used == -INFINITY ? 0.f : ex2((m_used - m_new) * sl2);
+        l *= corr;
+        m_used = m_new;
+        if (j > 0) {
+#pragma unroll
+          for (int c = 0; c < kD / 8; ++c) {
+            uint32_t u[8];
+            tmem_ld_32x32b_x8(tO(t) + lane_off + c * 8, u);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * corr);
+            tmem_st_32x32b_x8(tO(t) + lane_off + c * 8, u);
+          }
+          tmem_st_wait();
+        }
+      }
+      if (live) {
+        // no key yet: every exponent is -inf against 0
+        const float mb = (m_used == -INFINITY ? 0.f : m_used * sl2) - (kBf16 ? 0.f : kF16Shift);
+        const uint64_t sc2 = f2pack(sl2, sl2), nmb2 = f2pack(-mb, -mb);
+        uint64_t l2[2] = {f2pack(0.f, 0.f), f2pack(0.f, 0.f)};
+#pragma unroll
+        for (int c0 = 0; c0 < kKV; c0 += 16) {  // 16 keys -> 8 P columns
+          uint32_t pk[8];
+#pragma unroll
+          for (int c = c0; c < c0 + 16; c += 2) {
+            float e0, e1;
+            f2unpack(ffma2(f2pack(sv[c], sv[c + 1]), sc2, nmb2), e0, e1);
+            const float p0 = ex2(e0), p1 = ex2(e1);
+            l2[(c >> 1) & 1] = fadd2(l2[(c >> 1) & 1], f2pack(p0, p1));
+            pk[(c - c0) / 2] = pack2(p0, p1, kBf16);
+          }
+          tmem_st_32x32b_x8(tP(t) + lane_off + c0 / 2, *reinterpret_cast<const uint32_t(*)[8]>(pk));
+        }
+        float a0, a1;
+        f2unpack(fadd2(l2[0], l2[1]), a0, a1);
+        l += a0 + a1;
+        tmem_st_wait();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[t]);
+    }
+    bool have_o = false;  // O holds sums (with no key tile it holds nothing)
+    if (ok) {
+      have_o = warp_wait(&o_full[t], 0, kErrAccFull, abort_flag, lane);
+      ok = have_o;
+    }
+    tc_fence_after();
+    if (prm.splits == 1) {
+      if (live && (ok || n_kv == 0)) {
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays NaN
+        uint16_t* orow = p.o + b * p.ob + query * p.os +
+                         static_cast<int64_t>(kvh * p.group + r % p.group) * p.oh;
+#pragma unroll
+        for (int c0 = 0; c0 < kD; c0 += 16) {
+          uint32_t u[16];
+          tmem_ld_32x32b_x16(tO(t) + lane_off + c0, u);
+          tmem_ld_wait();
+          if (row_live) {
+#pragma unroll
+            for (int q8 = 0; q8 < 2; ++q8) {
+              if (c0 + q8 * 8 < p.head_dim) {
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = have_o ? __uint_as_float(u[q8 * 8 + i]) * inv : 0.f;
+                uint4 w;
+                w.x = pack2(f[0], f[1], kBf16);
+                w.y = pack2(f[2], f[3], kBf16);
+                w.z = pack2(f[4], f[5], kBf16);
+                w.w = pack2(f[6], f[7], kBf16);
+                *reinterpret_cast<uint4*>(orow + c0 + q8 * 8) = w;
+              }
+            }
+          }
+        }
+      }
+    } else {
+      // this CTA's share of the keys: (max, sum) and the partial row, over
+      // the rings once neither tile's MMAs read them
+      asm volatile("bar.sync 1, %0;" ::"n"(kSoftThreads) : "memory");
+      ml[t * kQ + r] = make_float2(m_used, l);
+      float* part = reinterpret_cast<float*>(smem) + (t * kQ + r) * Cf::kPitch;
+      if (t < tiles) {
+#pragma unroll
+        for (int c0 = 0; c0 < kD; c0 += 16) {
+          uint32_t u[16];
+          tmem_ld_32x32b_x16(tO(t) + lane_off + c0, u);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<float4*>(part + c0 + i) =
+                have_o ? make_float4(__uint_as_float(u[i]), __uint_as_float(u[i + 1]), __uint_as_float(u[i + 2]),
+                                     __uint_as_float(u[i + 3]))
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (prm.splits == 1) return;
+  // The cluster's CTAs sum a share of the rows each, over all of them in rank
+  // order.
+  cluster_sync();
+  const int chunks = p.head_dim / 8;
+  const uint32_t part_s = smem_u32(smem), ml_s = smem_u32(ml);
+  for (int i = threadIdx.x + kThreads * split; i < tiles * kQ * chunks; i += kThreads * prm.splits) {
+    const int row = i / chunks, c = (i % chunks) * 8;
+    const int t = row / kQ, r = row % kQ, query = q0 + t * prm.qpt + r / p.group;
+    if (r >= prm.qpt * p.group || query >= p.sq) continue;
+    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f, m = -INFINITY;
+    for (int w = 0; w < prm.splits; ++w) m = fmaxf(m, ld_cluster_f2(mapa_shared(ml_s + row * 8, w)).x);
+    const float base = m == -INFINITY ? 0.f : m;
+    for (int w = 0; w < prm.splits; ++w) {
+      const float2 s = ld_cluster_f2(mapa_shared(ml_s + row * 8, w));
+      const float f = ex2((s.x - base) * p.scale_log2);
+      l = fmaf(f, s.y, l);
+      const uint32_t src = mapa_shared(part_s + (row * Cf::kPitch + c) * 4, w);
+      const float4 x = ld_cluster_f4(src), y = ld_cluster_f4(src + 16);
+      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = fmaf(f, v[e], o[e]);
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    uint4 w4;
+    w4.x = pack2(o[0] * inv, o[1] * inv, kBf16);
+    w4.y = pack2(o[2] * inv, o[3] * inv, kBf16);
+    w4.z = pack2(o[4] * inv, o[5] * inv, kBf16);
+    w4.w = pack2(o[6] * inv, o[7] * inv, kBf16);
+    *reinterpret_cast<uint4*>(p.o + b * p.ob + query * p.os +
+                              static_cast<int64_t>(kvh * p.group + r % p.group) * p.oh + c) = w4;
+  }
+  cluster_sync();  // the others may still read this CTA's partial rows
+}
+
+// One tensor as [d2][d1][d0][head_dim] with element strides; a dimension of
+// stride 0 (shared data) or one element becomes one of extent 1 (*mul 0).
+struct Dim {
+  int64_t extent, stride;
+  int* mul;
+};
+bool make_map(CUtensorMap* m, const void* base, int dtype, int head_dim, int box_d, const Dim (&d)[3],
+              const int (&box)[3], CUtensorMapSwizzle swz) {
+  EncodeTiledFn fn = get_encode_tiled();
+  if (!fn) return false;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), 1, 1, 1};
+  cuuint64_t strides[3] = {16, 16, 16};
+  cuuint32_t bx[4] = {static_cast<cuuint32_t>(box_d), 1, 1, 1}, es[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 3; ++i) {
+    bx[i + 1] = static_cast<cuuint32_t>(box[i]);
+    if (d[i].mul) *d[i].mul = d[i].stride != 0;
+    if (d[i].stride == 0) continue;
+    dims[i + 1] = static_cast<cuuint64_t>(d[i].extent);
+    strides[i] = static_cast<cuuint64_t>(d[i].stride) * 2;
+  }
+  return fn(m, dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+            const_cast<void*>(base), dims, strides, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool kBf16, int kD, bool kMask>
+int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TcParams& prm,
+                   int64_t ctas, cudaStream_t st) {
+  const auto kernel = cross_tc_kernel<kBf16, kD, kMask>;
+  static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return kErrCuda;
+  if (dev >= 64 || !(ready.load() >> dev & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<kD>::kSmem) != cudaSuccess)
+      return kErrCuda;
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Cfg<kD>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  if (prm.splits > 1) {
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = prm.splits;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+  }
+  count_launches(1);
+  return cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, prm) == cudaSuccess ? kOk : kErrLaunch;
+}
+
+template <int kD>
+int launch_typed(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TcParams& prm,
+                 int dtype, int64_t ctas, cudaStream_t st) {
+  const bool mask = prm.c.k_lens || prm.c.key_mask;
+  if (dtype == kBF16)
+    return mask ? launch_variant<true, kD, true>(mq, mk, mv, prm, ctas, st)
+                : launch_variant<true, kD, false>(mq, mk, mv, prm, ctas, st);
+  return mask ? launch_variant<false, kD, true>(mq, mk, mv, prm, ctas, st)
+              : launch_variant<false, kD, false>(mq, mk, mv, prm, ctas, st);
+}
+
+}  // namespace
+
+bool cross_tc_takes(const CrossParams& p) {
+  if (p.bias) return false;
+  // a tensor map's stride is below 2^40 bytes, and where it is 0 the
+  // dimension cannot be part of a box
+  const int64_t s[] = {p.qb, p.qs, p.qh, p.kb, p.ks, p.kh, p.vb, p.vs, p.vh};
+  for (int64_t x : s)
+    if (x >= (1ll << 39)) return false;
+  if ((p.sq > 1 && p.qs == 0) || (p.kv_heads * p.group > 1 && p.qh == 0)) return false;
+  return p.sk > 0 && (p.sk == 1 || (p.ks != 0 && p.vs != 0));
+}
+
+int launch_cross_tc(const CrossParams& p, int dtype, cudaStream_t st) {
+  TcParams prm;
+  memset(&prm, 0, sizeof(prm));
+  prm.c = p;
+  prm.qpt = kQ / p.group;
+  const int64_t row_tiles = (static_cast<int64_t>(p.sq) + prm.qpt - 1) / prm.qpt;
+  const int64_t heads = static_cast<int64_t>(p.kv_heads) * p.batch;
+  prm.tiles = 2;
+  prm.splits = 1;
+  prm.items_x = static_cast<int>((row_tiles + prm.tiles - 1) / prm.tiles);
+  const int64_t ctas = heads * prm.items_x * prm.splits;
+  if (ctas > 0x7fffffffLL) return kErrShape;
+  const int box_d = p.head_dim <= 32 ? 32 : 64;
+  const CUtensorMapSwizzle swz = box_d == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+  CUtensorMap mq, mk, mv;
+  const Dim dq[3] = {{static_cast<int64_t>(p.kv_heads) * p.group, p.qh, nullptr}, {p.sq, p.qs, nullptr},
+                     {p.batch, p.qb, &prm.qmul_b}};
+  const Dim dk[3] = {{p.sk, p.ks, nullptr}, {p.kv_heads, p.kh, &prm.kmul_h}, {p.batch, p.kb, &prm.kmul_b}};
+  const Dim dv[3] = {{p.sk, p.vs, nullptr}, {p.kv_heads, p.vh, &prm.vmul_h}, {p.batch, p.vb, &prm.vmul_b}};
+  const int bq[3] = {p.group, prm.qpt, 1}, bk[3] = {kKV, 1, 1};
+  if (!make_map(&mq, p.q, dtype, p.head_dim, box_d, dq, bq, swz) ||
+      !make_map(&mk, p.k, dtype, p.head_dim, box_d, dk, bk, swz) ||
+      !make_map(&mv, p.v, dtype, p.head_dim, box_d, dv, bk, swz))
+    return kErrTma;
+  if (p.head_dim <= 32) return launch_typed<32>(mq, mk, mv, prm, dtype, ctas, st);
+  if (p.head_dim <= 64) return launch_typed<64>(mq, mk, mv, prm, dtype, ctas, st);
+  return launch_typed<128>(mq, mk, mv, prm, dtype, ctas, st);
+}
+
+}  // namespace s3

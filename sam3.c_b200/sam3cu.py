@@ -174,8 +174,11 @@ _TORCH_CODE = None
 
 
 def dtype_code(t) -> int:
-    import torch
-    return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}[t.dtype]
+    global _TORCH_CODE
+    if _TORCH_CODE is None:
+        import torch
+        _TORCH_CODE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    return _TORCH_CODE[t.dtype]
 
 
 # ------------------------------------------------------------------ ops
@@ -310,56 +313,70 @@ class RopeFreqs:
         return self._c.amplitude
 
 
-def _here(device):
-    """The calls launch on the current device, where their tensors must be."""
+def _here(x):
+    """The device index of x, which must be the current device's: the calls
+    launch there, on its current stream."""
     import torch
-    if device.type != "cuda" or device.index != torch.cuda.current_device():
-        raise ValueError(f"tensors must be on the current CUDA device, not on {device}")
+    dev = x.get_device()
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors must be on the current CUDA device, not on {x.device}")
+    return dev
 
 
-def _like(t, x, shape, what):
-    if t.dtype != x.dtype or t.device != x.device or t.shape != shape or (t.stride(-1) != 1 and shape[-1] > 1):
+def _like(t, x, shape, dev, what):
+    if t.dtype != x.dtype or t.get_device() != dev or t.shape != shape or (t.stride(-1) != 1 and shape[-1] > 1):
         raise ValueError(f"{what} must be a {x.dtype} tensor of shape {tuple(shape)} on {x.device} with contiguous "
                          f"last dimension")
-    return t
 
 
-def _head_param(t, x, what):
+def _empty_like(x):
+    import torch
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _raw_stream(dev):
+    """The current stream's handle (the public form makes a Stream object, 3 us a call)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _head_param(t, head_dim, dev, what):
     if t is None:
         return 0
-    if t.shape != x.shape[-1:] or t.device != x.device:
-        raise ValueError(f"{what} must be [head_dim] on {x.device}")
+    if t.shape != (head_dim,) or t.get_device() != dev:
+        raise ValueError(f"{what} must be a [head_dim] tensor on the inputs' device")
     return _f32(t, what)
 
 
-def _head_view(x, out, q, gamma, beta, what):
+def _head_view(x, out, q, dev, gamma, beta, what):
     """x [batch, seq, heads, head_dim] like q, any strides but the last."""
-    import torch
-    if x.dim() != 4 or x.shape[:2] != q.shape[:2] or x.shape[3] != q.shape[3]:
+    shape, like = x.shape, q.shape
+    if len(shape) != 4 or len(like) != 4 or shape[0] != like[0] or shape[1] != like[1] or shape[3] != like[3]:
         raise ValueError("q and k must be [batch, seq, heads, head_dim], alike but in heads")
-    _like(x, q, x.shape, what)
+    _like(x, q, shape, dev, what)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _empty_like(x)
     else:
-        _like(out, q, x.shape, "the output of " + what)
-    xs, ys = x.stride(), out.stride()
-    return out, _HEAD_VIEW.pack(x.data_ptr(), xs[0], xs[1], xs[2], out.data_ptr(), ys[0], ys[1], ys[2], x.shape[2],
-                                _head_param(gamma, x, "gamma"), _head_param(beta, x, "beta"))
+        _like(out, q, shape, dev, "the output of " + what)
+    xb, xs, xh, _ = x.stride()
+    yb, ys, yh, _ = out.stride()
+    return out, _HEAD_VIEW.pack(x.data_ptr(), xb, xs, xh, out.data_ptr(), yb, ys, yh, shape[2],
+                                _head_param(gamma, shape[3], dev, "gamma"), _head_param(beta, shape[3], dev, "beta"))
 
 
-def _positions(positions, x):
+def _positions(positions, batch, seq, dev):
     """Pointer and batch stride of int64 positions [seq], [1, seq] or [batch, seq]."""
     import torch
     if positions is None:
         return None, 0
-    batch, seq = x.shape[:2]
-    if positions.dtype != torch.int64 or positions.device != x.device or positions.dim() not in (1, 2) \
-            or positions.shape[-1] != seq or (positions.stride(-1) != 1 and seq > 1):
-        raise ValueError(f"positions must be int64 [batch, seq] or [seq] on {x.device}, contiguous along seq")
-    if positions.dim() == 1 or positions.shape[0] == 1:
+    shape = positions.shape
+    if positions.dtype != torch.int64 or positions.get_device() != dev or len(shape) not in (1, 2) \
+            or shape[-1] != seq or (seq > 1 and positions.stride(-1) != 1):
+        raise ValueError("positions must be int64 [batch, seq] or [seq] on the inputs' device, contiguous along seq")
+    if len(shape) == 1 or shape[0] == 1:
         return positions.data_ptr(), 0
-    if positions.shape[0] != batch:
-        raise ValueError(f"positions for {positions.shape[0]} sequences, not {batch}")
+    if shape[0] != batch:
+        raise ValueError(f"positions for {shape[0]} sequences, not {batch}")
     return positions.data_ptr(), positions.stride(0)
 
 
@@ -368,14 +385,15 @@ def rope_pos(q, freqs: RopeFreqs, positions=None, start: int = 0, k=None, out=No
     tokens' positions (int64 tensor [batch, seq] or [seq], else start,
     start + 1, ...): sam3cu_rope_pos.  out / k_out may be q / k themselves.
     Returns q's rotation, with k the pair."""
-    _here(q.device)
-    out, qv = _head_view(q, out, q, None, None, "q")
+    dev = _here(q)
+    out, qv = _head_view(q, out, q, dev, None, None, "q")
     kv = None
     if k is not None:
-        k_out, kv = _head_view(k, k_out, q, None, None, "k")
-    pos, stride = _positions(positions, q)
-    check(lib().sam3cu_rope_pos(qv, kv, dtype_code(q), q.shape[0], q.shape[1], q.shape[3], pos, stride, start,
-                                freqs.ptr, _stream()), "sam3cu_rope_pos")
+        k_out, kv = _head_view(k, k_out, q, dev, None, None, "k")
+    batch, seq, _, head_dim = q.shape
+    pos, stride = _positions(positions, batch, seq, dev)
+    check(lib().sam3cu_rope_pos(qv, kv, dtype_code(q), batch, seq, head_dim, pos, stride, start, freqs.ptr,
+                                _raw_stream(dev)), "sam3cu_rope_pos")
     return out if k is None else (out, k_out)
 
 
@@ -385,15 +403,18 @@ def qk_norm_rope(q, k, q_gamma=None, k_gamma=None, q_beta=None, k_beta=None, nor
     be None) over its elements, then rotate as rope_pos does (freqs None: no
     rotation), in one pass: sam3cu_qk_norm_rope.  gamma and beta: float32
     [head_dim] or None."""
-    _here(q.device)
-    out, qv = _head_view(q, out, q, q_gamma, q_beta, "q")
+    dev = _here(q)
+    out, qv = _head_view(q, out, q, dev, q_gamma, q_beta, "q")
     kv = None
     if k is not None:
-        k_out, kv = _head_view(k, k_out, q, k_gamma, k_beta, "k")
-    pos, stride = _positions(positions, q) if freqs is not None else (None, 0)
-    check(lib().sam3cu_qk_norm_rope(qv, kv, dtype_code(q), q.shape[0], q.shape[1], q.shape[3], norm, eps, pos, stride,
-                                    start, freqs.ptr if freqs is not None else None, _stream()),
-          "sam3cu_qk_norm_rope")
+        k_out, kv = _head_view(k, k_out, q, dev, k_gamma, k_beta, "k")
+    batch, seq, _, head_dim = q.shape
+    table, pos, stride = None, None, 0
+    if freqs is not None:
+        table = freqs.ptr
+        pos, stride = _positions(positions, batch, seq, dev)
+    check(lib().sam3cu_qk_norm_rope(qv, kv, dtype_code(q), batch, seq, head_dim, norm, eps, pos, stride, start, table,
+                                    _raw_stream(dev)), "sam3cu_qk_norm_rope")
     return out if k is None else (out, k_out)
 
 
@@ -408,44 +429,50 @@ def cross_attention(q, k, v, k_lens=None, key_mask=None, bias=None, scale: float
     sq, sk] (its last dimension sk); scale 0: 1/sqrt(head_dim).  A query left
     without keys gives zeros."""
     import torch
-    _here(q.device)
-    if q.dim() != 4 or k.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+    dev = _here(q)
+    qshape, kshape = q.shape, k.shape
+    if len(qshape) != 4 or len(kshape) != 4 or kshape[0] != qshape[0] or kshape[3] != qshape[3]:
         raise ValueError("q must be [batch, sq, q_heads, head_dim], k and v [batch, sk, kv_heads, head_dim]")
-    batch, sq, q_heads, head_dim = q.shape
-    sk, kv_heads = k.shape[1], k.shape[2]
-    _like(q, q, q.shape, "q")
-    _like(k, q, k.shape, "k")
-    _like(v, q, k.shape, "v")
+    batch, sq, q_heads, head_dim = qshape
+    _, sk, kv_heads, _ = kshape
+    _like(q, q, qshape, dev, "q")
+    _like(k, q, kshape, dev, "k")
+    _like(v, q, kshape, dev, "v")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = _empty_like(q)
     else:
-        _like(out, q, q.shape, "out")
-    lens = mask = bptr = 0
-    mask_stride, bs = 0, (0, 0, 0)
+        _like(out, q, qshape, dev, "out")
+    lens = mask = bptr = mask_stride = bb = bh = bq = 0
     if k_lens is not None:
-        if k_lens.dtype != torch.int32 or k_lens.shape != (batch,) or k_lens.device != q.device \
+        if k_lens.dtype != torch.int32 or k_lens.shape != (batch,) or k_lens.get_device() != dev \
                 or not k_lens.is_contiguous():
-            raise ValueError(f"k_lens must be a contiguous int32 [batch] tensor on {q.device}")
+            raise ValueError("k_lens must be a contiguous int32 [batch] tensor on the inputs' device")
         lens = k_lens.data_ptr()
     if key_mask is not None:
-        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.dim() != 2 or key_mask.device != q.device \
+        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.dim() != 2 or key_mask.get_device() != dev \
                 or key_mask.shape[0] not in (1, batch) or key_mask.shape[1] != sk \
                 or (key_mask.stride(1) != 1 and sk > 1):
-            raise ValueError(f"key_mask must be a bool or uint8 [batch or 1, sk] tensor on {q.device}, contiguous "
-                             f"along sk")
+            raise ValueError("key_mask must be a bool or uint8 [batch or 1, sk] tensor on the inputs' device, "
+                             "contiguous along sk")
         mask, mask_stride = key_mask.data_ptr(), key_mask.stride(0) if key_mask.shape[0] > 1 else 0
     if bias is not None:
-        if bias.dtype != torch.float32 or bias.device != q.device or bias.dim() > 4 or bias.dim() < 1 \
+        if bias.dtype != torch.float32 or bias.get_device() != dev or bias.dim() > 4 or bias.dim() < 1 \
                 or bias.shape[-1] != sk or (bias.stride(-1) != 1 and sk > 1):
-            raise ValueError(f"bias must be a float32 tensor on {q.device} that broadcasts to [batch, q_heads, sq, "
-                             f"sk], contiguous along sk")
-        bs = bias.expand(batch, q_heads, sq, sk).stride()
+            raise ValueError("bias must be a float32 tensor on the inputs' device that broadcasts to [batch, q_heads, "
+                             "sq, sk], contiguous along sk")
+        try:
+            bb, bh, bq, _ = bias.expand(batch, q_heads, sq, sk).stride()
+        except RuntimeError as e:
+            raise ValueError(f"bias of shape {tuple(bias.shape)} does not broadcast to [batch, q_heads, sq, sk]") from e
         bptr = bias.data_ptr()
-    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
-    args = _CROSS_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qs[0], qs[1], qs[2], ks[0],
-                            ks[1], ks[2], vs[0], vs[1], vs[2], os_[0], os_[1], os_[2], dtype_code(q), batch, sq, sk,
-                            q_heads, kv_heads, head_dim, scale, lens, mask, mask_stride, bptr, bs[0], bs[1], bs[2])
-    check(lib().sam3cu_cross_attention(args, _stream()), "sam3cu_cross_attention")
+    qb, qs, qh, _ = q.stride()
+    kb, ks, kh, _ = k.stride()
+    vb, vs, vh, _ = v.stride()
+    ob, os_, oh, _ = out.stride()
+    args = _CROSS_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qb, qs, qh, kb, ks, kh, vb, vs,
+                            vh, ob, os_, oh, dtype_code(q), batch, sq, sk, q_heads, kv_heads, head_dim, scale, lens,
+                            mask, mask_stride, bptr, bb, bh, bq)
+    check(lib().sam3cu_cross_attention(args, _raw_stream(dev)), "sam3cu_cross_attention")
     return out
 
 
