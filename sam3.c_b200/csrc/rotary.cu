@@ -6,13 +6,11 @@
 //   qk_norm_rope   RMS norm or LayerNorm over each head, then the rotation
 //
 // Both read and write every element once and do a few operations on it, so
-// HBM bounds them; what they must not do is let the angles cost more than
+// HBM bounds them; what they must not do is let anything else cost more than
 // the data.  p f_i is formed and reduced in 64 bits (f_i in revolutions, so
 // the reduction is a subtraction of the nearest integer), cosine and sine in
-// F32 of the remainder, once per token and pair, and reused by all heads of
-// the token: a warp owns one token (or, where there are few tokens, a slice
-// of its heads), computes the token's table into shared memory while its
-// first loads are in flight, then streams the heads.
+// F32 of the remainder: once per token and pair, into a shared-memory table
+// of the CTA's tokens that all their heads then read.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -29,6 +27,8 @@ using namespace s3;
 namespace {
 
 constexpr int kWarps = 8;   // per CTA
+constexpr int kThreads = 32 * kWarps;
+constexpr int kMaxTokens = 32;  // of a CTA (rotary_vec)
 constexpr int kMaxDim = 2 * SAM3CU_ROPE_MAX_PAIRS;
 
 enum : int { kNormNone = 0, kNormRms = SAM3CU_NORM_RMS, kNormLayer = SAM3CU_NORM_LAYER };
@@ -44,8 +44,9 @@ struct View {
 struct Params {
   View v[2];           // q, k
   int q_heads, heads;  // heads of q, of q and k together
-  int slices;          // warps that share a token's heads
-  int per_slice;       // heads of a slice
+  int slices;          // rotary_any: warps that share a token's heads,
+  int per_slice;       //   and the heads of one
+  int block_tokens;    // rotary_vec: tokens of a CTA
   int64_t tokens;      // batch * seq
   int seq, head_dim;
   const int64_t* positions;
@@ -105,23 +106,23 @@ __device__ __forceinline__ void unpack8(const Raw8<T>& r, float* f) {
 template <int T>
 __device__ __forceinline__ void st8(void* p, int64_t i, const float* f) {
   uint4* d = reinterpret_cast<uint4*>(static_cast<char*>(p) + i * (T == kF32 ? 4 : 2));
-  if (T == kF32) {
+  if constexpr (T == kF32) {
     d[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
     d[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
-    return;
-  }
-  uint32_t w[4];
+  } else {
+    uint32_t w[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if (T == kBF16) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
-      w[k] = *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-      const __half2 h = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
-      w[k] = *reinterpret_cast<const uint32_t*>(&h);
+    for (int k = 0; k < 4; ++k) {
+      if (T == kBF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
+        w[k] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
+        w[k] = *reinterpret_cast<const uint32_t*>(&h);
+      }
     }
+    d[0] = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  d[0] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // The warp's place: token and the heads [h0, h1) of q and k together.
@@ -161,72 +162,103 @@ __device__ __forceinline__ double position_of(const Params& p, const Place& at) 
 // bytes.  A lane holds 16 elements of a head: in the interleaved layout 16
 // consecutive ones, in the half layout 8 from either half, so both elements
 // of a pair are always in one lane and a head takes head_dim / 16 lanes (the
-// next power of two, kG, for the reductions).  32 / kG heads go through a
-// warp at a time, kU of those batches with their loads in flight together.
+// next power of two, kG, for the reductions).  The CTA's (token, head) pairs
+// are dealt to its lane groups in order, so no lane idles however many heads
+// there are; a group has two heads' loads in flight.
 template <int T, int kNorm, bool kRot, int kG>
-__global__ void __launch_bounds__(kWarps * 32) rotary_vec(const __grid_constant__ Params p) {
-  constexpr int kHeads = 32 / kG;            // heads of a batch
-  constexpr int kU = T == kF32 ? 1 : 2;      // batches in flight
-  __shared__ float2 table[kWarps][kRot ? kG * 8 : 1];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Place at;
-  if (!place_of(p, warp, at)) return;
-  const int slot = lane % kG, sub = lane / kG;
+__global__ void __launch_bounds__(kThreads, kNorm == kNormLayer ? 2 : 3) rotary_vec(const __grid_constant__ Params p) {
+  constexpr int kGroups = kThreads / kG;
+  constexpr int kES = T == kF32 ? 4 : 2;
+  constexpr int kU = 2;
+  // cos and sin of pairs 8 slot + 2 jj, + 1 at [token][jj][slot]: the lanes
+  // of a head read consecutive words
+  extern __shared__ float4 table[];
+  __shared__ int64_t offs[4][kMaxTokens];  // a token's row in q's x, q's y, k's x, k's y
+  const int tid = threadIdx.x;
+  const int64_t token0 = static_cast<int64_t>(blockIdx.x) * p.block_tokens;
+  const int n_tok = static_cast<int>(min(static_cast<int64_t>(p.block_tokens), p.tokens - token0));
   const int rslots = kRot ? p.f.n_pairs / 8 : 0;  // slots that are rotated
+  const int slot = tid % kG, group = tid / kG;
   const bool turned = kRot && slot < rslots;
   const bool half = kRot && p.f.layout == SAM3CU_ROPE_HALF;
   const int e0 = (half && turned) ? 8 * slot : 16 * slot;
   const int e1 = (half && turned) ? p.f.n_pairs + 8 * slot : 16 * slot + 8;
   const bool have = slot * 16 < p.head_dim;
 
-  float2 cs[kRot ? 8 : 1];
-  bool have_cs = !kRot;
+  for (int i = tid; i < n_tok; i += kThreads) {
+    const int64_t token = token0 + i;
+    const int64_t b = token / p.seq, s = token - b * p.seq;
+    offs[0][i] = b * p.v[0].xb + s * p.v[0].xs;
+    offs[1][i] = b * p.v[0].yb + s * p.v[0].ys;
+    offs[2][i] = b * p.v[1].xb + s * p.v[1].xs;
+    offs[3][i] = b * p.v[1].yb + s * p.v[1].ys;
+  }
+  if constexpr (kRot) {
+    for (int i = tid; i < n_tok * rslots * 4; i += kThreads) {
+      const int per = rslots * 4, tok = i / per, at = i - tok * per;
+      const int jj = at / rslots, sl = at - jj * rslots;
+      const int64_t token = token0 + tok;
+      const int64_t b = token / p.seq, s = token - b * p.seq;
+      const double pos = static_cast<double>(p.positions ? p.positions[b * p.pos_stride + s] : p.start + s);
+      const float2 c0 = turn(p, pos, 8 * sl + 2 * jj), c1 = turn(p, pos, 8 * sl + 2 * jj + 1);
+      table[i] = make_float4(c0.x, c0.y, c1.x, c1.y);
+    }
+  }
+  __syncthreads();
+
 #pragma unroll 1
-  for (int part = 0; part < 2; ++part) {  // the slice's query heads, then its key heads
-    const int lo = part ? max(at.h0, p.q_heads) : at.h0;
-    const int hi = part ? at.h1 : min(at.h1, p.q_heads);
-    if (lo >= hi) continue;
+  for (int part = 0; part < 2; ++part) {
+    const int heads = part ? p.heads - p.q_heads : p.q_heads;
     const View& v = p.v[part];
-    const int64_t first = part ? p.q_heads : 0;
-    const char* x = static_cast<const char*>(v.x) + (at.b * v.xb + at.s * v.xs) * (T == kF32 ? 4 : 2);
-    char* y = static_cast<char*>(v.y) + (at.b * v.yb + at.s * v.ys) * (T == kF32 ? 4 : 2);
     // without a norm, what is not rotated need not move where it already is
-    const bool still = kNorm == kNormNone && v.x == v.y && !turned;
-    const bool mine = have && !still;
-    float g[kNorm ? 16 : 1], bt[kNorm ? 16 : 1];
-    if (kNorm && mine) {
+    const bool mine = have && !(kNorm == kNormNone && v.x == v.y && !turned);
+    const char* x = static_cast<const char*>(v.x);
+    char* y = static_cast<char*>(v.y);
+    float g[kNorm ? 16 : 1], bt[kNorm == kNormLayer ? 16 : 1];
+    if (kNorm && have && heads > 0) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        g[kNorm ? k : 0] = v.gamma ? __ldg(v.gamma + e0 + k) : 1.f;
-        g[kNorm ? 8 + k : 0] = v.gamma ? __ldg(v.gamma + e1 + k) : 1.f;
-        bt[kNorm ? k : 0] = v.beta ? __ldg(v.beta + e0 + k) : 0.f;
-        bt[kNorm ? 8 + k : 0] = v.beta ? __ldg(v.beta + e1 + k) : 0.f;
+      for (int k = 0; k < 16; k += 4) {
+        const int e = k < 8 ? e0 + k : e1 + k - 8;
+        float4 w = v.gamma ? __ldg(reinterpret_cast<const float4*>(v.gamma + e)) : make_float4(1.f, 1.f, 1.f, 1.f);
+        g[kNorm ? k : 0] = w.x;
+        g[kNorm ? k + 1 : 0] = w.y;
+        g[kNorm ? k + 2 : 0] = w.z;
+        g[kNorm ? k + 3 : 0] = w.w;
+        if (kNorm == kNormLayer) {
+          w = v.beta ? __ldg(reinterpret_cast<const float4*>(v.beta + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          bt[kNorm == kNormLayer ? k : 0] = w.x;
+          bt[kNorm == kNormLayer ? k + 1 : 0] = w.y;
+          bt[kNorm == kNormLayer ? k + 2 : 0] = w.z;
+          bt[kNorm == kNormLayer ? k + 3 : 0] = w.w;
+        }
       }
     }
-    for (int h = lo; h < hi; h += kHeads * kU) {
+    const int units = n_tok * heads;
+    int tok = heads ? group / heads : 0, head = heads ? group - tok * heads : 0;
+    const int step_t = heads ? kGroups / heads : 0, step_h = heads ? kGroups - step_t * heads : 0;
+    // (all lanes of a warp stay in the loop while one has a unit: shuffles)
+    for (int w0 = (tid / 32) * (32 / kG); w0 < units; w0 += kU * kGroups) {
       Raw8<T> ra[kU], rb[kU];
+      int tk[kU], hd[kU];
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
-        const int hh = h + u * kHeads + sub;
-        if (mine && hh < hi) {
-          ra[u] = ld8<T>(x, (hh - first) * v.xh + e0);
-          rb[u] = ld8<T>(x, (hh - first) * v.xh + e1);
+        tk[u] = tok;
+        hd[u] = head;
+        if (mine && tok < n_tok) {
+          const char* src = x + (offs[2 * part][tok] + head * v.xh) * kES;
+          ra[u] = ld8<T>(src, e0);
+          rb[u] = ld8<T>(src, e1);
         }
-      }
-      if (!have_cs) {  // once, behind the first loads
-        const double pos = position_of(p, at);
-        for (int i = lane; i < p.f.n_pairs; i += 32) table[warp][i] = turn(p, pos, i);
-        __syncwarp();
-        if (turned) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) cs[kRot ? k : 0] = table[warp][kRot ? 8 * slot + k : 0];
+        tok += step_t;
+        head += step_h;
+        if (head >= heads) {
+          head -= heads;
+          ++tok;
         }
-        have_cs = true;
       }
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
-        const int hh = h + u * kHeads + sub;
-        const bool live = mine && hh < hi;
+        const bool live = mine && tk[u] < n_tok;
         float f[16];
         if (live) {
           unpack8<T>(ra[u], f);
@@ -236,52 +268,59 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_vec(const __grid_constant_
           for (int k = 0; k < 16; ++k) f[k] = 0.f;
         }
         if (kNorm) {
-          const float n = static_cast<float>(p.head_dim);
-          float sum = 0.f, mean = 0.f;
+          const float n = 1.f / static_cast<float>(p.head_dim);
           if (kNorm == kNormLayer) {
+            float sum = 0.f;
 #pragma unroll
             for (int k = 0; k < 16; ++k) sum += f[k];
 #pragma unroll
             for (int o = kG / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            mean = sum / n;
-            if (live) {
+            const float mean = live ? sum * n : 0.f;
 #pragma unroll
-              for (int k = 0; k < 16; ++k) f[k] -= mean;
-            }
+            for (int k = 0; k < 16; ++k) f[k] -= mean;
           }
           float sq = 0.f;
 #pragma unroll
           for (int k = 0; k < 16; ++k) sq = fmaf(f[k], f[k], sq);
 #pragma unroll
           for (int o = kG / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-          const float inv = 1.f / sqrtf(sq / n + p.eps);
+          const float inv = 1.f / sqrtf(fmaf(sq, n, p.eps));
           if (live) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) f[k] = fmaf(f[k] * inv, g[kNorm ? k : 0], bt[kNorm ? k : 0]);
-          }
-        }
-        if (turned) {
-          if (half) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float2 r = cs[kRot ? k : 0];
-              const float a = f[k], b = f[8 + k];
-              f[k] = a * r.x - b * r.y;
-              f[8 + k] = a * r.y + b * r.x;
+            for (int k = 0; k < 16; ++k) {
+              if (kNorm == kNormLayer) f[k] = fmaf(f[k] * inv, g[kNorm ? k : 0], bt[kNorm == kNormLayer ? k : 0]);
+              else f[k] = f[k] * inv * g[kNorm ? k : 0];
             }
-          } else {
+            if (kNorm == kNormRms && v.beta) {  // uncommon: read as it is used
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float2 r = cs[kRot ? k : 0];
-              const float a = f[2 * k], b = f[2 * k + 1];
-              f[2 * k] = a * r.x - b * r.y;
-              f[2 * k + 1] = a * r.y + b * r.x;
+              for (int k = 0; k < 16; ++k) f[k] += __ldg(v.beta + (k < 8 ? e0 + k : e1 + k - 8));
             }
           }
         }
         if (live) {
-          st8<T>(y, (hh - first) * v.yh + e0, f);
-          st8<T>(y, (hh - first) * v.yh + e1, f + 8);
+          if (turned) {
+            const float4* cs = table + tk[u] * rslots * 4 + slot;
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) {
+              const float4 c = cs[jj * rslots];
+              if (half) {
+                const float a0 = f[2 * jj], b0 = f[8 + 2 * jj], a1 = f[2 * jj + 1], b1 = f[9 + 2 * jj];
+                f[2 * jj] = a0 * c.x - b0 * c.y;
+                f[8 + 2 * jj] = a0 * c.y + b0 * c.x;
+                f[2 * jj + 1] = a1 * c.z - b1 * c.w;
+                f[9 + 2 * jj] = a1 * c.w + b1 * c.z;
+              } else {
+                const float a0 = f[4 * jj], b0 = f[4 * jj + 1], a1 = f[4 * jj + 2], b1 = f[4 * jj + 3];
+                f[4 * jj] = a0 * c.x - b0 * c.y;
+                f[4 * jj + 1] = a0 * c.y + b0 * c.x;
+                f[4 * jj + 2] = a1 * c.z - b1 * c.w;
+                f[4 * jj + 3] = a1 * c.w + b1 * c.z;
+              }
+            }
+          }
+          char* dst = y + (offs[2 * part + 1][tk[u]] + hd[u] * v.yh) * kES;
+          st8<T>(dst, e0, f);
+          st8<T>(dst, e1, f + 8);
         }
       }
     }
@@ -387,28 +426,24 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_any(const __grid_constant_
 
 template <int T, int kNorm>
 int launch_typed(Params& p, int rot, bool vec, cudaStream_t st) {
-  // heads that a warp takes at a time; few tokens: more warps to a token, so
-  // that the call fills the SMs with about eight warps each
-  const int lanes = (p.head_dim + 15) / 16;
-  const int g = lanes <= 1 ? 1 : lanes <= 2 ? 2 : lanes <= 4 ? 4 : lanes <= 8 ? 8 : 16;
-  const int step = vec ? 32 / g : 1;
-  const int64_t want = static_cast<int64_t>(num_sms()) * 8;
-  int64_t slices = (want + p.tokens - 1) / p.tokens;
-  const int most = (p.heads + step - 1) / step;
-  if (slices > most) slices = most;
-  if (slices < 1) slices = 1;
-  p.per_slice = (most + static_cast<int>(slices) - 1) / static_cast<int>(slices) * step;
-  p.slices = (p.heads + p.per_slice - 1) / p.per_slice;
-  const int64_t blocks = (p.tokens * p.slices + kWarps - 1) / kWarps;
-  if (blocks > 0x7fffffffLL) return SAM3CU_ESHAPE;
-  const dim3 grid(static_cast<unsigned>(blocks));
   count_launches(1);
-#define S3_ROT(G)                                                                           \
-  case G:                                                                                   \
-    if (rot) rotary_vec<T, kNorm, true, G><<<grid, kWarps * 32, 0, st>>>(p);                \
-    else rotary_vec<T, kNorm, false, G><<<grid, kWarps * 32, 0, st>>>(p);                   \
-    break
   if (vec) {
+    const int lanes = p.head_dim / 16;
+    const int g = lanes <= 1 ? 1 : lanes <= 2 ? 2 : lanes <= 4 ? 4 : lanes <= 8 ? 8 : 16;
+    // Tokens of a CTA: as many as leave two CTAs to an SM, up to 32 (the
+    // table's and the gammas' cost is then spread over the most heads).
+    int bt = kMaxTokens;
+    while (bt > 1 && (p.tokens + bt - 1) / bt < 2 * num_sms()) bt /= 2;
+    p.block_tokens = bt;
+    const int64_t blocks = (p.tokens + bt - 1) / bt;
+    if (blocks > 0x7fffffffLL) return SAM3CU_ESHAPE;
+    const dim3 grid(static_cast<unsigned>(blocks));
+    const size_t smem = static_cast<size_t>(bt) * (rot / 16) * 64;
+#define S3_ROT(G)                                                            \
+  case G:                                                                    \
+    if (rot) rotary_vec<T, kNorm, true, G><<<grid, kThreads, smem, st>>>(p); \
+    else rotary_vec<T, kNorm, false, G><<<grid, kThreads, 0, st>>>(p);       \
+    break
     switch (g) {
       S3_ROT(1);
       S3_ROT(2);
@@ -416,14 +451,22 @@ int launch_typed(Params& p, int rot, bool vec, cudaStream_t st) {
       S3_ROT(8);
       S3_ROT(16);
     }
-  } else if (p.head_dim <= 64) {
-    rotary_any<T, kNorm, 1><<<grid, kWarps * 32, 0, st>>>(p, rot);
-  } else if (p.head_dim <= 128) {
-    rotary_any<T, kNorm, 2><<<grid, kWarps * 32, 0, st>>>(p, rot);
-  } else {
-    rotary_any<T, kNorm, 4><<<grid, kWarps * 32, 0, st>>>(p, rot);
-  }
 #undef S3_ROT
+  } else {
+    // few tokens: more warps to a token, so that the call fills the SMs with
+    // about eight warps each
+    const int64_t want = static_cast<int64_t>(num_sms()) * 8;
+    int64_t slices = (want + p.tokens - 1) / p.tokens;
+    if (slices > p.heads) slices = p.heads;
+    p.per_slice = (p.heads + static_cast<int>(slices) - 1) / static_cast<int>(slices);
+    p.slices = (p.heads + p.per_slice - 1) / p.per_slice;
+    const int64_t blocks = (p.tokens * p.slices + kWarps - 1) / kWarps;
+    if (blocks > 0x7fffffffLL) return SAM3CU_ESHAPE;
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (p.head_dim <= 64) rotary_any<T, kNorm, 1><<<grid, kThreads, 0, st>>>(p, rot);
+    else if (p.head_dim <= 128) rotary_any<T, kNorm, 2><<<grid, kThreads, 0, st>>>(p, rot);
+    else rotary_any<T, kNorm, 4><<<grid, kThreads, 0, st>>>(p, rot);
+  }
   return cudaGetLastError() == cudaSuccess ? SAM3CU_OK : SAM3CU_ELAUNCH;
 }
 
@@ -455,6 +498,7 @@ int take_view(const sam3cu_head_view* h, int dtype, int batch, int seq, View* v,
   const uintptr_t px = reinterpret_cast<uintptr_t>(h->x), py = reinterpret_cast<uintptr_t>(h->y);
   if (px % es || py % es) return SAM3CU_EINVAL;
   if ((px | py) & 15) *vec = false;
+  if ((reinterpret_cast<uintptr_t>(h->gamma) | reinterpret_cast<uintptr_t>(h->beta)) & 15) *vec = false;
   if (h->x == h->y && memcmp(xs, ys, sizeof(xs))) return SAM3CU_EINVAL;
   if ((reinterpret_cast<uintptr_t>(h->gamma) | reinterpret_cast<uintptr_t>(h->beta)) & 3) return SAM3CU_EINVAL;
   *v = View{h->x, h->y, xs[0], xs[1], xs[2], ys[0], ys[1], ys[2], h->gamma, h->beta};
