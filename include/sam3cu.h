@@ -651,7 +651,7 @@ struct sam3cu_head_view {
  * for every sequence; negative positions turn backwards), or start + s where
  * positions is NULL.  The angle is formed in 64 bits, the rotation in F32.
  * dtype SAM3CU_F32, _F16 or _BF16; head_dim 2 .. 256, >= 2*n_pairs.  Heads
- * whose head_dim and rot_dim are multiples of 16 and whose rows start on 16
+ * whose head_dim is a multiple of 16 and whose rows start on 16
  * bytes take 16-byte accesses.
  */
 SAM3CU_API int sam3cu_rope_pos(const struct sam3cu_head_view *q, const struct sam3cu_head_view *k,

@@ -9,8 +9,7 @@
 // HBM bounds them; what they must not do is let anything else cost more than
 // the data.  p f_i is formed and reduced in 64 bits (f_i in revolutions, so
 // the reduction is a subtraction of the nearest integer), cosine and sine in
-// F32 of the remainder: once per token and pair, into a shared-memory table
-// of the CTA's tokens that all their heads then read.
+// F32 of the remainder: once per token and pair, for all of its heads.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -20,6 +19,7 @@
 #include <cstring>
 
 #include "../../include/sam3cu.h"
+#include "attention_math.cuh"
 #include "sam3cu_internal.h"
 
 using namespace s3;
@@ -28,7 +28,12 @@ namespace {
 
 constexpr int kWarps = 8;   // per CTA
 constexpr int kThreads = 32 * kWarps;
-constexpr int kMaxTokens = 32;  // of a CTA (rotary_vec)
+// rotary_vec: CTAs per SM it is compiled for, and heads of a lane under way.
+// Measured (us: 8 x 5184 tokens x 32 heads of 64 bf16 / LayerNorm, 16 x 5184 x
+// 20 heads / f16, 6185 tokens x 24 heads of 128): 3 CTAs, 4 heads 60.1 / 78.7 /
+// 16.0; 4, 4: 65.1 / 80.3 / 15.5; 5, 4: 75.0 / 115 / 17.7; 3 CTAs with one head
+// ahead in registers 81.1 / 98.0 / 21.5.
+constexpr int kVecCtas = 3, kAhead = 4;
 constexpr int kMaxDim = 2 * SAM3CU_ROPE_MAX_PAIRS;
 
 enum : int { kNormNone = 0, kNormRms = SAM3CU_NORM_RMS, kNormLayer = SAM3CU_NORM_LAYER };
@@ -44,9 +49,8 @@ struct View {
 struct Params {
   View v[2];           // q, k
   int q_heads, heads;  // heads of q, of q and k together
-  int slices;          // rotary_any: warps that share a token's heads,
+  int slices;          // warps or lane groups that share a token's heads,
   int per_slice;       //   and the heads of one
-  int block_tokens;    // rotary_vec: tokens of a CTA
   int64_t tokens;      // batch * seq
   int seq, head_dim;
   const int64_t* positions;
@@ -68,60 +72,62 @@ __device__ __forceinline__ void st1(void* p, int64_t i, float v) {
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
-// Eight elements as loaded: one 16-byte word, or two for F32.
+// The 16 elements of a lane as loaded: 16-byte pieces of kP elements.
 template <int T>
-struct Raw8 {
-  uint4 w[T == kF32 ? 2 : 1];
+struct Raw {
+  static constexpr int kP = T == kF32 ? 4 : 8;
+  static constexpr int kN = 16 / kP;
+  uint4 w[kN];
 };
+// Elements 2k, 2k + 1 of a lane as a packed operand.
 template <int T>
-__device__ __forceinline__ Raw8<T> ld8(const void* p, int64_t i) {
-  Raw8<T> r;
-  const uint4* s = reinterpret_cast<const uint4*>(static_cast<const char*>(p) + i * (T == kF32 ? 4 : 2));
-  r.w[0] = s[0];
-  if constexpr (T == kF32) r.w[1] = s[1];
-  return r;
-}
-template <int T>
-__device__ __forceinline__ void unpack8(const Raw8<T>& r, float* f) {
+__device__ __forceinline__ uint64_t pair_of(const Raw<T>& r, int k) {
+  const uint4& q = r.w[2 * k / Raw<T>::kP];
   if constexpr (T == kF32) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      f[4 * k] = __uint_as_float(r.w[k].x);
-      f[4 * k + 1] = __uint_as_float(r.w[k].y);
-      f[4 * k + 2] = __uint_as_float(r.w[k].z);
-      f[4 * k + 3] = __uint_as_float(r.w[k].w);
-    }
+    return k & 1 ? f2pack(__uint_as_float(q.z), __uint_as_float(q.w))
+                 : f2pack(__uint_as_float(q.x), __uint_as_float(q.y));
   } else {
-    const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float2 v;
-      if (T == kBF16) v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
-      else v = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-      f[2 * k] = v.x;
-      f[2 * k + 1] = v.y;
-    }
+    const uint32_t w = (k & 3) == 0 ? q.x : (k & 3) == 1 ? q.y : (k & 3) == 2 ? q.z : q.w;
+    float2 v;
+    if (T == kBF16) v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+    else v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return f2pack(v.x, v.y);
   }
 }
 template <int T>
-__device__ __forceinline__ void st8(void* p, int64_t i, const float* f) {
-  uint4* d = reinterpret_cast<uint4*>(static_cast<char*>(p) + i * (T == kF32 ? 4 : 2));
-  if constexpr (T == kF32) {
-    d[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-    d[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
-  } else {
-    uint32_t w[4];
+__device__ __forceinline__ void st_piece(void* p, int64_t i, const uint64_t* h) {
+  float f[8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (T == kBF16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
-        w[k] = *reinterpret_cast<const uint32_t*>(&h);
-      } else {
-        const __half2 h = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
-        w[k] = *reinterpret_cast<const uint32_t*>(&h);
-      }
-    }
-    d[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  for (int k = 0; k < Raw<T>::kP / 2; ++k) f2unpack(h[k], f[2 * k], f[2 * k + 1]);
+  uint4 w;
+  if constexpr (T == kF32) {
+    w = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  } else {
+    w = make_uint4(pack2(f[0], f[1], T == kBF16), pack2(f[2], f[3], T == kBF16), pack2(f[4], f[5], T == kBF16),
+                   pack2(f[6], f[7], T == kBF16));
+  }
+  *reinterpret_cast<uint4*>(static_cast<char*>(p) + i * (T == kF32 ? 4 : 2)) = w;
+}
+
+// Heads of a lane under way: 32 bytes each, 64 for F32.
+template <int T, int kRot>
+constexpr int ring_depth() {
+  return (T == kF32 ? kAhead / 2 : kAhead) / (kRot == 2 ? 2 : 1);  // the exchange takes shared memory too
+}
+template <int T, int kRot>
+constexpr size_t ring_bytes() {
+  return static_cast<size_t>(ring_depth<T, kRot>()) * Raw<T>::kN * 16 * kThreads;
+}
+
+// token = b * seq + s
+__device__ __forceinline__ void split_token(const Params& p, int64_t token, int64_t& b, int64_t& s) {
+  if (p.tokens <= 0x7fffffff) {  // the 64-bit division is several times dearer
+    const uint32_t t = static_cast<uint32_t>(token), n = static_cast<uint32_t>(p.seq);
+    b = t / n;
+    s = t - static_cast<uint32_t>(b) * n;
+  } else {
+    b = token / p.seq;
+    s = token - b * p.seq;
   }
 }
 
@@ -138,8 +144,10 @@ __device__ __forceinline__ bool place_of(const Params& p, int warp, Place& at) {
     token = item / p.slices;
     slice = static_cast<int>(item - token * p.slices);
   }
-  at.b = static_cast<int>(token / p.seq);
-  at.s = static_cast<int>(token - static_cast<int64_t>(at.b) * p.seq);
+  int64_t b, s;
+  split_token(p, token, b, s);
+  at.b = static_cast<int>(b);
+  at.s = static_cast<int>(s);
   at.h0 = slice * p.per_slice;
   at.h1 = min(p.heads, at.h0 + p.per_slice);
   return true;
@@ -159,175 +167,241 @@ __device__ __forceinline__ double position_of(const Params& p, const Place& at) 
 }
 
 // Heads whose dimensions are multiples of 16 and whose rows start on 16
-// bytes.  A lane holds 16 elements of a head: in the interleaved layout 16
-// consecutive ones, in the half layout 8 from either half, so both elements
-// of a pair are always in one lane and a head takes head_dim / 16 lanes (the
-// next power of two, kG, for the reductions).  The CTA's (token, head) pairs
-// are dealt to its lane groups in order, so no lane idles however many heads
-// there are; a group has two heads' loads in flight.
-template <int T, int kNorm, bool kRot, int kG>
-__global__ void __launch_bounds__(kThreads, kNorm == kNormLayer ? 2 : 3) rotary_vec(const __grid_constant__ Params p) {
-  constexpr int kGroups = kThreads / kG;
+// bytes.  A lane holds 16 elements of a head in 16-byte pieces, chosen so that
+// both elements of a pair are in one lane and the lanes of a head access
+// consecutive pieces (whole 32-byte sectors): half of its pieces from either
+// half of the rotated part in the half layout, pieces spread over the head in
+// the interleaved one.  head_dim / 16 lanes (kG, the next power of two) are a
+// group; a group takes the heads of one token (or, where there are few
+// tokens, a slice of them) one after the other, with the cosines and sines of
+// its lanes' pairs in registers and the next heads' copies under way (cp.async
+// into places of the lane's own, which costs no registers).
+//
+// kRot 2: the half layout with halves that are not multiples of 8 elements.  A
+// pair's elements are then in different lanes, which exchange the (normalised)
+// head through shared memory; the pieces lie as in the interleaved layout.
+template <int T, int kNorm, int kRot, int kG>
+__global__ void __launch_bounds__(kThreads, kRot == 2 ? 2 : kVecCtas) rotary_vec(const __grid_constant__ Params p) {
+  using R = Raw<T>;
   constexpr int kES = T == kF32 ? 4 : 2;
-  constexpr int kU = 2;
-  // cos and sin of pairs 8 slot + 2 jj, + 1 at [token][jj][slot]: the lanes
-  // of a head read consecutive words
-  extern __shared__ float4 table[];
-  __shared__ int64_t offs[4][kMaxTokens];  // a token's row in q's x, q's y, k's x, k's y
+  constexpr int kDepth = ring_depth<T, kRot>();
+  __shared__ __align__(16) float affine[kNorm ? 2 : 1][2][kNorm ? 16 * kG : 1];  // gamma, beta of q and k
   const int tid = threadIdx.x;
-  const int64_t token0 = static_cast<int64_t>(blockIdx.x) * p.block_tokens;
-  const int n_tok = static_cast<int>(min(static_cast<int64_t>(p.block_tokens), p.tokens - token0));
-  const int rslots = kRot ? p.f.n_pairs / 8 : 0;  // slots that are rotated
-  const int slot = tid % kG, group = tid / kG;
-  const bool turned = kRot && slot < rslots;
-  const bool half = kRot && p.f.layout == SAM3CU_ROPE_HALF;
-  const int e0 = (half && turned) ? 8 * slot : 16 * slot;
-  const int e1 = (half && turned) ? p.f.n_pairs + 8 * slot : 16 * slot + 8;
-  const bool have = slot * 16 < p.head_dim;
-
-  for (int i = tid; i < n_tok; i += kThreads) {
-    const int64_t token = token0 + i;
-    const int64_t b = token / p.seq, s = token - b * p.seq;
-    offs[0][i] = b * p.v[0].xb + s * p.v[0].xs;
-    offs[1][i] = b * p.v[0].yb + s * p.v[0].ys;
-    offs[2][i] = b * p.v[1].xb + s * p.v[1].xs;
-    offs[3][i] = b * p.v[1].yb + s * p.v[1].ys;
+  const int slot = tid % kG;
+  const int slots = p.head_dim / 16;              // lanes of a head
+  const int rslots = kRot ? p.f.n_pairs / 8 : 0;  // half layout: those that rotate
+  const bool half = kRot == 1 && p.f.layout == SAM3CU_ROPE_HALF;
+  int off[R::kN];  // elements of the head that the lane's pieces start at
+  bool turned = false;
+#pragma unroll
+  for (int i = 0; i < R::kN; ++i) {
+    if (half && slot < rslots) {
+      off[i] = R::kP * slot + (i % (R::kN / 2)) * R::kP * rslots + (i >= R::kN / 2 ? p.f.n_pairs : 0);
+    } else if (half) {  // behind the rotated part
+      off[i] = 16 * rslots + R::kP * (slot - rslots) + i * R::kP * (slots - rslots);
+    } else {
+      off[i] = R::kP * slot + i * R::kP * slots;
+    }
+    turned = turned || (kRot && off[i] < 2 * p.f.n_pairs);
   }
-  if constexpr (kRot) {
-    for (int i = tid; i < n_tok * rslots * 4; i += kThreads) {
-      const int per = rslots * 4, tok = i / per, at = i - tok * per;
-      const int jj = at / rslots, sl = at - jj * rslots;
-      const int64_t token = token0 + tok;
-      const int64_t b = token / p.seq, s = token - b * p.seq;
-      const double pos = static_cast<double>(p.positions ? p.positions[b * p.pos_stride + s] : p.start + s);
-      const float2 c0 = turn(p, pos, 8 * sl + 2 * jj), c1 = turn(p, pos, 8 * sl + 2 * jj + 1);
-      table[i] = make_float4(c0.x, c0.y, c1.x, c1.y);
+
+  // the group's token and heads
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / kG) + tid / kG;
+  const int64_t token = p.slices > 1 ? item / p.slices : item;
+  const int slice = p.slices > 1 ? static_cast<int>(item - token * p.slices) : 0;
+  const bool have = slot < slots && token < p.tokens;
+  const int h0 = slice * p.per_slice;
+  const int h1 = min(p.heads, h0 + p.per_slice);
+  int64_t b, s;
+  split_token(p, have ? token : 0, b, s);
+  const char* xq = static_cast<const char*>(p.v[0].x) + (b * p.v[0].xb + s * p.v[0].xs) * kES;
+  const char* xk = static_cast<const char*>(p.v[1].x) + (b * p.v[1].xb + s * p.v[1].xs - p.q_heads * p.v[1].xh) * kES;
+  char* yq = static_cast<char*>(p.v[0].y) + (b * p.v[0].yb + s * p.v[0].ys) * kES;
+  char* yk = static_cast<char*>(p.v[1].y) + (b * p.v[1].yb + s * p.v[1].ys - p.q_heads * p.v[1].yh) * kES;
+  // without a norm, what is not rotated need not move where it already is
+  const bool mq = have && (kNorm != kNormNone || p.v[0].x != p.v[0].y || turned);
+  const bool mk = have && (kNorm != kNormNone || p.v[1].x != p.v[1].y || turned);
+
+  // The lane's pieces of a head (zeros where it has none) into its places of
+  // the ring; nobody else reads them, so no barrier is needed.
+  extern __shared__ uint4 ring[];  // [kDepth][pieces][kThreads]
+  const uint32_t mine_s = smem_u32(ring) + tid * 16;
+  auto issue = [&](int i) {
+    const int h = h0 + i;
+    const bool k = h >= p.q_heads;
+    const bool on = h < h1 && (k ? mk : mq);
+    const char* x = on ? (k ? xk : xq) + h * (k ? p.v[1].xh : p.v[0].xh) * kES : static_cast<const char*>(p.v[0].x);
+    const uint32_t dst = mine_s + static_cast<uint32_t>(i % kDepth) * (R::kN * kThreads * 16);
+#pragma unroll
+    for (int n = 0; n < R::kN; ++n)
+      cp_async16(dst + n * (kThreads * 16), x + (on ? off[n] * kES : 0), on);
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kDepth - 1; ++i) issue(i);
+
+  if constexpr (kNorm != kNormNone) {
+    for (int i = tid; i < 4 * 16 * kG; i += kThreads) {
+      const int e = i % (16 * kG), which = i / (16 * kG);
+      const View& v = p.v[which >> 1];
+      const float* src = which & 1 ? v.beta : v.gamma;
+      affine[which >> 1][which & 1][e] = src && e < p.head_dim ? src[e] : (which & 1 ? 0.f : 1.f);
+    }
+    __syncthreads();
+  }
+  // kRot 1: (cos, cos) and (sin, sin) of the lane's pairs 2 jj, 2 jj + 1.
+  // kRot 2: cos, and the factor of the partner, of its elements 2 jj, 2 jj + 1.
+  constexpr int kCs = kRot == 2 ? 8 : 4;
+  uint64_t cc[kRot ? kCs : 1], ss[kRot ? kCs : 1];
+  // a pair or element of the lane that turns (in the half layout: all or none)
+  uint32_t turns = 0;
+  if constexpr (kRot != 0) {
+    if (have && turned) {
+      const double pos =
+          static_cast<double>(p.positions ? p.positions[b * p.pos_stride + s] : p.start + s);
+#pragma unroll
+      for (int jj = 0; jj < kCs; ++jj) {
+        // element of the lane: of its low pieces, or of all
+        const int e = (half || kRot == 2) ? 2 * jj : 4 * jj;
+        const int at = off[e / R::kP] + e % R::kP;
+        float2 c[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          c[i] = make_float2(1.f, 0.f);
+          const int el = kRot == 2 ? at + i : 0;
+          const int pair = kRot == 2 ? (el >= p.f.n_pairs ? el - p.f.n_pairs : el) : (half ? at : at / 2) + i;
+          if (pair < p.f.n_pairs) {
+            c[i] = turn(p, pos, pair);
+            if (kRot == 2 && el < p.f.n_pairs) c[i].y = -c[i].y;
+            turns |= 1u << (2 * jj + i);
+          }
+        }
+        cc[jj] = f2pack(c[0].x, c[1].x);
+        ss[jj] = f2pack(c[0].y, c[1].y);
+      }
     }
   }
-  __syncthreads();
 
+  auto process = [&](const Raw<T>& raw, int h) {
+    const bool k = h >= p.q_heads;
+    uint64_t h2[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h2[i] = pair_of<T>(raw, i);
+    if constexpr (kNorm != kNormNone) {
+      const float n = 1.f / static_cast<float>(p.head_dim);
+      if constexpr (kNorm == kNormLayer) {
+        float a, c;
+        f2unpack(fadd2(fadd2(fadd2(h2[0], h2[1]), fadd2(h2[2], h2[3])),
+                       fadd2(fadd2(h2[4], h2[5]), fadd2(h2[6], h2[7]))),
+                 a, c);
+        float sum = a + c;
+#pragma unroll
+        for (int o = kG / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float mean = slot < slots ? -sum * n : 0.f;
+        const uint64_t m2 = f2pack(mean, mean);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h2[i] = fadd2(h2[i], m2);
+      }
+      uint64_t q2[2] = {f2pack(0.f, 0.f), f2pack(0.f, 0.f)};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q2[i & 1] = ffma2(h2[i], h2[i], q2[i & 1]);
+      float a, c;
+      f2unpack(fadd2(q2[0], q2[1]), a, c);
+      float sq = a + c;
+#pragma unroll
+      for (int o = kG / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+      const float inv = rsqrtf(fmaf(sq, n, p.eps));
+      const uint64_t i2 = f2pack(inv, inv);
+      if (slot < slots) {
+        const float(&af)[2][kNorm ? 16 * kG : 1] = affine[kNorm && k ? 1 : 0];
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const int e = kNorm ? off[2 * i / R::kP] + 2 * i % R::kP : 0;
+          const float4 g = *reinterpret_cast<const float4*>(&af[0][e]);
+          const float4 t = *reinterpret_cast<const float4*>(&af[1][e]);
+          h2[i] = ffma2(fmul2(h2[i], i2), f2pack(g.x, g.y), f2pack(t.x, t.y));
+          h2[i + 1] = ffma2(fmul2(h2[i + 1], i2), f2pack(g.z, g.w), f2pack(t.z, t.w));
+        }
+      }
+    }
+    if constexpr (kRot == 2) {
+      // one word of padding after eight, so that lanes and groups spread over
+      // the banks
+      constexpr int kPitch = kG * 18 + 1;
+      __shared__ float heads[kThreads / kG][kPitch];
+      float* mine_h = heads[tid / kG];
+      float f[16];
+      __syncwarp();  // the last head has been read
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        f2unpack(h2[i], f[2 * i], f[2 * i + 1]);
+        const int e = off[2 * i / R::kP] + 2 * i % R::kP;
+        mine_h[e + (e >> 3)] = f[2 * i];
+        mine_h[e + 1 + (e >> 3)] = f[2 * i + 1];
+      }
+      __syncwarp();
+      if (turns) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float c[2], sn[2];
+          f2unpack(cc[i], c[0], c[1]);
+          f2unpack(ss[i], sn[0], sn[1]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            if (turns >> (2 * i + j) & 1) {
+              const int e = off[2 * i / R::kP] + 2 * i % R::kP + j;
+              const int o = e < p.f.n_pairs ? e + p.f.n_pairs : e - p.f.n_pairs;
+              f[2 * i + j] = f[2 * i + j] * c[j] + mine_h[o + (o >> 3)] * sn[j];
+            }
+          }
+          h2[i] = f2pack(f[2 * i], f[2 * i + 1]);
+        }
+      }
+    } else if constexpr (kRot == 1) {
+      if (half) {
+        if (turned) {
+#pragma unroll
+          for (int jj = 0; jj < 4; ++jj) {
+            const uint64_t a2 = h2[jj], b2 = h2[4 + jj];
+            h2[jj] = ffma2(b2, fneg2(ss[jj]), fmul2(a2, cc[jj]));
+            h2[4 + jj] = ffma2(a2, ss[jj], fmul2(b2, cc[jj]));
+          }
+        }
+      } else if (turns) {
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+          float co[2], si[2];
+          f2unpack(cc[jj], co[0], co[1]);
+          f2unpack(ss[jj], si[0], si[1]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float a, c;
+            f2unpack(h2[2 * jj + i], a, c);
+            const uint64_t r = f2pack(a * co[i] - c * si[i], a * si[i] + c * co[i]);
+            if (turns >> (2 * jj + i) & 1) h2[2 * jj + i] = r;
+          }
+        }
+      }
+    }
+    if (h < h1 && (k ? mk : mq)) {
+      char* y = (k ? yk : yq) + h * (k ? p.v[1].yh : p.v[0].yh) * kES;
+#pragma unroll
+      for (int i = 0; i < R::kN; ++i) st_piece<T>(y, off[i], h2 + i * R::kP / 2);
+    }
+  };
+  // (every lane of a warp makes the same number of turns: shuffles)
 #pragma unroll 1
-  for (int part = 0; part < 2; ++part) {
-    const int heads = part ? p.heads - p.q_heads : p.q_heads;
-    const View& v = p.v[part];
-    // without a norm, what is not rotated need not move where it already is
-    const bool mine = have && !(kNorm == kNormNone && v.x == v.y && !turned);
-    const char* x = static_cast<const char*>(v.x);
-    char* y = static_cast<char*>(v.y);
-    float g[kNorm ? 16 : 1], bt[kNorm == kNormLayer ? 16 : 1];
-    if (kNorm && have && heads > 0) {
+  for (int i = 0; i < p.per_slice; ++i) {
+    issue(i + kDepth - 1);  // into the place read last
+    cp_async_wait<kDepth - 1>();
+    Raw<T> raw;
 #pragma unroll
-      for (int k = 0; k < 16; k += 4) {
-        const int e = k < 8 ? e0 + k : e1 + k - 8;
-        float4 w = v.gamma ? __ldg(reinterpret_cast<const float4*>(v.gamma + e)) : make_float4(1.f, 1.f, 1.f, 1.f);
-        g[kNorm ? k : 0] = w.x;
-        g[kNorm ? k + 1 : 0] = w.y;
-        g[kNorm ? k + 2 : 0] = w.z;
-        g[kNorm ? k + 3 : 0] = w.w;
-        if (kNorm == kNormLayer) {
-          w = v.beta ? __ldg(reinterpret_cast<const float4*>(v.beta + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
-          bt[kNorm == kNormLayer ? k : 0] = w.x;
-          bt[kNorm == kNormLayer ? k + 1 : 0] = w.y;
-          bt[kNorm == kNormLayer ? k + 2 : 0] = w.z;
-          bt[kNorm == kNormLayer ? k + 3 : 0] = w.w;
-        }
-      }
-    }
-    const int units = n_tok * heads;
-    int tok = heads ? group / heads : 0, head = heads ? group - tok * heads : 0;
-    const int step_t = heads ? kGroups / heads : 0, step_h = heads ? kGroups - step_t * heads : 0;
-    // (all lanes of a warp stay in the loop while one has a unit: shuffles)
-    for (int w0 = (tid / 32) * (32 / kG); w0 < units; w0 += kU * kGroups) {
-      Raw8<T> ra[kU], rb[kU];
-      int tk[kU], hd[kU];
-#pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        tk[u] = tok;
-        hd[u] = head;
-        if (mine && tok < n_tok) {
-          const char* src = x + (offs[2 * part][tok] + head * v.xh) * kES;
-          ra[u] = ld8<T>(src, e0);
-          rb[u] = ld8<T>(src, e1);
-        }
-        tok += step_t;
-        head += step_h;
-        if (head >= heads) {
-          head -= heads;
-          ++tok;
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        const bool live = mine && tk[u] < n_tok;
-        float f[16];
-        if (live) {
-          unpack8<T>(ra[u], f);
-          unpack8<T>(rb[u], f + 8);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 16; ++k) f[k] = 0.f;
-        }
-        if (kNorm) {
-          const float n = 1.f / static_cast<float>(p.head_dim);
-          if (kNorm == kNormLayer) {
-            float sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) sum += f[k];
-#pragma unroll
-            for (int o = kG / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            const float mean = live ? sum * n : 0.f;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) f[k] -= mean;
-          }
-          float sq = 0.f;
-#pragma unroll
-          for (int k = 0; k < 16; ++k) sq = fmaf(f[k], f[k], sq);
-#pragma unroll
-          for (int o = kG / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-          const float inv = 1.f / sqrtf(fmaf(sq, n, p.eps));
-          if (live) {
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              if (kNorm == kNormLayer) f[k] = fmaf(f[k] * inv, g[kNorm ? k : 0], bt[kNorm == kNormLayer ? k : 0]);
-              else f[k] = f[k] * inv * g[kNorm ? k : 0];
-            }
-            if (kNorm == kNormRms && v.beta) {  // uncommon: read as it is used
-#pragma unroll
-              for (int k = 0; k < 16; ++k) f[k] += __ldg(v.beta + (k < 8 ? e0 + k : e1 + k - 8));
-            }
-          }
-        }
-        if (live) {
-          if (turned) {
-            const float4* cs = table + tk[u] * rslots * 4 + slot;
-#pragma unroll
-            for (int jj = 0; jj < 4; ++jj) {
-              const float4 c = cs[jj * rslots];
-              if (half) {
-                const float a0 = f[2 * jj], b0 = f[8 + 2 * jj], a1 = f[2 * jj + 1], b1 = f[9 + 2 * jj];
-                f[2 * jj] = a0 * c.x - b0 * c.y;
-                f[8 + 2 * jj] = a0 * c.y + b0 * c.x;
-                f[2 * jj + 1] = a1 * c.z - b1 * c.w;
-                f[9 + 2 * jj] = a1 * c.w + b1 * c.z;
-              } else {
-                const float a0 = f[4 * jj], b0 = f[4 * jj + 1], a1 = f[4 * jj + 2], b1 = f[4 * jj + 3];
-                f[4 * jj] = a0 * c.x - b0 * c.y;
-                f[4 * jj + 1] = a0 * c.y + b0 * c.x;
-                f[4 * jj + 2] = a1 * c.z - b1 * c.w;
-                f[4 * jj + 3] = a1 * c.w + b1 * c.z;
-              }
-            }
-          }
-          char* dst = y + (offs[2 * part + 1][tk[u]] + hd[u] * v.yh) * kES;
-          st8<T>(dst, e0, f);
-          st8<T>(dst, e1, f + 8);
-        }
-      }
-    }
+    for (int n = 0; n < R::kN; ++n) raw.w[n] = ring[(i % kDepth * R::kN + n) * kThreads + tid];
+    process(raw, h0 + i);
   }
 }
 
-// Any head_dim, rotated part, alignment and stride: a lane holds the pairs
+// Any head_dim, alignment and stride: a lane holds the pairs
 // lane, lane + 32, ... of a head (kP of them at most) and, behind them, the
 // elements that are not rotated.
 template <int T, int kNorm, int kP>
@@ -392,7 +466,7 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_any(const __grid_constant_
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-      const float inv = 1.f / sqrtf(sq / n + p.eps);
+      const float inv = rsqrtf(sq / n + p.eps);
       auto scaled = [&](float f, int e) {
         return fmaf(f * inv, v.gamma ? __ldg(v.gamma + e) : 1.f, v.beta ? __ldg(v.beta + e) : 0.f);
       };
@@ -424,25 +498,37 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_any(const __grid_constant_
   }
 }
 
+// At most `slices` (>= 1) slices of a token's heads.
+void set_slices(Params& p, int64_t slices) {
+  if (slices > p.heads) slices = p.heads;
+  p.per_slice = (p.heads + static_cast<int>(slices) - 1) / static_cast<int>(slices);
+  p.slices = (p.heads + p.per_slice - 1) / p.per_slice;
+}
+
 template <int T, int kNorm>
 int launch_typed(Params& p, int rot, bool vec, cudaStream_t st) {
   count_launches(1);
   if (vec) {
     const int lanes = p.head_dim / 16;
     const int g = lanes <= 1 ? 1 : lanes <= 2 ? 2 : lanes <= 4 ? 4 : lanes <= 8 ? 8 : 16;
-    // Tokens of a CTA: as many as leave two CTAs to an SM, up to 32 (the
-    // table's and the gammas' cost is then spread over the most heads).
-    int bt = kMaxTokens;
-    while (bt > 1 && (p.tokens + bt - 1) / bt < 2 * num_sms()) bt /= 2;
-    p.block_tokens = bt;
-    const int64_t blocks = (p.tokens + bt - 1) / bt;
+    // Lane groups that share a token's heads (they repeat its cosines): as
+    // many as one wave of CTAs has room for.  Beyond a wave one, but two where
+    // a second wave would be mostly empty and 16 heads are left to each
+    // (41472 tokens x 32 heads of 64, 1.5 waves: 60.6 -> 56.6 us; 82944 x 20
+    // with LayerNorm, 2.9 waves: 79.2 with one, 89.6 with two).
+    const bool exchange = rot % 16 && p.f.layout == SAM3CU_ROPE_HALF;
+    const int per_block = kThreads / g;
+    const int64_t alone = (p.tokens + per_block - 1) / per_block;
+    const int64_t wave = static_cast<int64_t>(exchange ? 4 : kVecCtas) * num_sms();  // (two waves of the exchange)
+    set_slices(p, alone <= wave ? wave / alone : (alone < 2 * wave && p.heads >= 32 ? 2 : 1));
+    const int64_t blocks = (p.tokens * p.slices + per_block - 1) / per_block;
     if (blocks > 0x7fffffffLL) return SAM3CU_ESHAPE;
     const dim3 grid(static_cast<unsigned>(blocks));
-    const size_t smem = static_cast<size_t>(bt) * (rot / 16) * 64;
-#define S3_ROT(G)                                                            \
-  case G:                                                                    \
-    if (rot) rotary_vec<T, kNorm, true, G><<<grid, kThreads, smem, st>>>(p); \
-    else rotary_vec<T, kNorm, false, G><<<grid, kThreads, 0, st>>>(p);       \
+#define S3_ROT(G)                                                                               \
+  case G:                                                                                       \
+    if (!rot) rotary_vec<T, kNorm, 0, G><<<grid, kThreads, ring_bytes<T, 0>(), st>>>(p);           \
+    else if (!exchange) rotary_vec<T, kNorm, 1, G><<<grid, kThreads, ring_bytes<T, 1>(), st>>>(p); \
+    else rotary_vec<T, kNorm, 2, G><<<grid, kThreads, ring_bytes<T, 2>(), st>>>(p);                \
     break
     switch (g) {
       S3_ROT(1);
@@ -456,10 +542,7 @@ int launch_typed(Params& p, int rot, bool vec, cudaStream_t st) {
     // few tokens: more warps to a token, so that the call fills the SMs with
     // about eight warps each
     const int64_t want = static_cast<int64_t>(num_sms()) * 8;
-    int64_t slices = (want + p.tokens - 1) / p.tokens;
-    if (slices > p.heads) slices = p.heads;
-    p.per_slice = (p.heads + static_cast<int>(slices) - 1) / static_cast<int>(slices);
-    p.slices = (p.heads + p.per_slice - 1) / p.per_slice;
+    set_slices(p, (want + p.tokens - 1) / p.tokens);
     const int64_t blocks = (p.tokens * p.slices + kWarps - 1) / kWarps;
     if (blocks > 0x7fffffffLL) return SAM3CU_ESHAPE;
     const dim3 grid(static_cast<unsigned>(blocks));
@@ -498,7 +581,6 @@ int take_view(const sam3cu_head_view* h, int dtype, int batch, int seq, View* v,
   const uintptr_t px = reinterpret_cast<uintptr_t>(h->x), py = reinterpret_cast<uintptr_t>(h->y);
   if (px % es || py % es) return SAM3CU_EINVAL;
   if ((px | py) & 15) *vec = false;
-  if ((reinterpret_cast<uintptr_t>(h->gamma) | reinterpret_cast<uintptr_t>(h->beta)) & 15) *vec = false;
   if (h->x == h->y && memcmp(xs, ys, sizeof(xs))) return SAM3CU_EINVAL;
   if ((reinterpret_cast<uintptr_t>(h->gamma) | reinterpret_cast<uintptr_t>(h->beta)) & 3) return SAM3CU_EINVAL;
   *v = View{h->x, h->y, xs[0], xs[1], xs[2], ys[0], ys[1], ys[2], h->gamma, h->beta};
@@ -521,7 +603,7 @@ int rotary_common(const sam3cu_head_view* q, const sam3cu_head_view* k, int dtyp
     if (reinterpret_cast<uintptr_t>(positions) & 7) return SAM3CU_EINVAL;
   }
   Params p;
-  bool vec = head_dim % 16 == 0 && rot % 16 == 0;
+  bool vec = head_dim % 16 == 0;
   int rc = take_view(q, dtype, batch, seq, &p.v[0], &vec);
   if (!rc) rc = take_view(k, dtype, batch, seq, &p.v[1], &vec);
   if (rc) return rc;

@@ -102,7 +102,8 @@ def _check(shape, kh, dt, rot, half, norm=0, far=1000, seed=0, order="bshd", aff
 @pytest.mark.parametrize("half", [False, True])
 @pytest.mark.parametrize("hd,rot", [(64, 64), (64, 32), (128, 128), (128, 64), (32, 32), (16, 16), (80, 48), (96, 96),
                                     (256, 256), (240, 16), (64, 2), (64, 50), (72, 72), (40, 8), (2, 2), (7, 4),
-                                    (130, 66), (255, 254)])
+                                    (130, 66), (255, 254), (96, 70), (128, 18), (256, 250),
+                                    (48, 34), (80, 20)])
 def test_rope(cuda, dt, half, hd, rot):
     _check((3, 5, 6, hd), 2, dt, rot, half, seed=hd + rot)
 
@@ -111,7 +112,8 @@ def test_rope(cuda, dt, half, hd, rot):
 @pytest.mark.parametrize("norm", [1, 2])
 @pytest.mark.parametrize("hd,rot,half", [(64, 64, True), (64, 64, False), (128, 64, True), (80, 48, False), (32, 0, True),
                                          (256, 128, True), (72, 40, True), (7, 2, False), (1, 0, True), (250, 0, True),
-                                         (16, 16, True)])
+                                         (16, 16, True), (96, 70, True), (96, 70, False), (256, 250, True),
+                                         (48, 2, True), (16, 6, True), (128, 36, False)])
 def test_norm(cuda, dt, norm, hd, rot, half):
     _check((2, 7, 5, hd), 3, dt, rot, half, norm=norm, seed=hd + rot)
 
@@ -125,7 +127,7 @@ def test_sizes(cuda, order, norm, shape, kh):
 
 
 @pytest.mark.parametrize("norm", [0, 1])
-@pytest.mark.parametrize("hd,rot", [(64, 64), (128, 32), (72, 20)])
+@pytest.mark.parametrize("hd,rot", [(64, 64), (128, 32), (72, 20), (96, 70), (256, 4)])
 @pytest.mark.parametrize("order", ["bshd", "bhsd"])
 def test_in_place(cuda, norm, hd, rot, order):
     _check((2, 9, 4, hd), 2, "f16", rot, True, norm=norm, inplace=True, order=order)
