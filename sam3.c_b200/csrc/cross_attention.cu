@@ -23,12 +23,14 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <cstring>
 
 #include "../../include/sam3cu.h"
+#include "attention_math.cuh"
 #include "cross_attention.cuh"
 #include "sam3cu_internal.h"
 #include "sm100_ptx.cuh"
@@ -37,8 +39,15 @@ namespace s3 {
 
 namespace {
 
+#ifndef S3_KEEP
+#define S3_KEEP 256
+#endif
+#ifndef S3_TCK
+#define S3_TCK 256
+#endif
 constexpr int kThreads = 128;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxKeep = 2048;  // keys that cross_keep_kernel may hold
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -76,11 +85,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&h);
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // kD: head_dim rounded up to 32, 64 or 128 (the copies fill the rest with
 // zeros).  kWM: row warps of the CTA (4 / kWM warps split the keys of a tile).
 template <int kD, int kWM>
@@ -108,6 +112,52 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c) {
   const int key = kChunks == 4 ? (r >> 1) & 3 : r & 7;
   return static_cast<uint32_t>((at ^ key) << 4);
 }
+
+// A warp's 16 rows (a lane: rows lane / 4 and + 8): running maximum, sum (this
+// lane's share) and O.
+template <int kD>
+struct RowState {
+  float acc[kD / 8][4];
+  float m[2], l[2];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < kD / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+  }
+  // Scores to P, against the maximum with them in it; sum and O rescaled.
+  // f16 P are times 2^14, which cancels in O / sum: below 2^-14 the type has
+  // no full precision left.
+  template <int kKeys>
+  __device__ __forceinline__ void softmax(float (&s)[kKeys / 8][4], float to_log2, bool bf) {
+    const float shift = bf ? 0.f : 14.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kKeys / 8; ++j) mx = max3(mx, s[j][2 * h], s[j][2 * h + 1]);
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float m_new = fmaxf(m[h], mx);
+      const float base = m_new == -INFINITY ? 0.f : m_new;  // nothing counted yet: every p is 0
+      const float corr = ex2((m[h] - base) * to_log2);
+      m[h] = m_new;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < kKeys / 8; ++j) {
+        s[j][2 * h] = ex2(fmaf(s[j][2 * h] - base, to_log2, shift));
+        s[j][2 * h + 1] = ex2(fmaf(s[j][2 * h + 1] - base, to_log2, shift));
+        sum += s[j][2 * h] + s[j][2 * h + 1];
+      }
+      l[h] = fmaf(l[h], corr, sum);
+#pragma unroll
+      for (int j = 0; j < kD / 8; ++j) {
+        acc[j][2 * h] *= corr;
+        acc[j][2 * h + 1] *= corr;
+      }
+    }
+  }
+};
 
 template <bool kBf16, int kD, int kWM, bool kBias>
 __global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_constant__ CrossParams p, int row_tiles,
@@ -168,10 +218,8 @@ __global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_consta
     cp_async_commit();
   }
 
-  float acc[kD / 8][4];
-#pragma unroll
-  for (int j = 0; j < kD / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+  RowState<kD> st;
+  st.clear();
   uint32_t qf[kD / 16][4];
   // with a bias the scores are in natural units (its lowest finite values
   // would overflow in base 2), without one they stay unscaled dot products
@@ -244,32 +292,7 @@ __global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_consta
         }
       }
     }
-    // online softmax: rows lane/4 and lane/4 + 8 of the warp's 16
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < kKW / 8; ++j) mx = fmaxf(mx, fmaxf(s[j][2 * h], s[j][2 * h + 1]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float m_new = fmaxf(m_run[h], mx);
-      const float base = m_new == -INFINITY ? 0.f : m_new;  // nothing counted yet: every p is 0
-      const float corr = ex2((m_run[h] - base) * to_log2);
-      m_run[h] = m_new;
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < kKW / 8; ++j) {
-        s[j][2 * h] = ex2((s[j][2 * h] - base) * to_log2);
-        s[j][2 * h + 1] = ex2((s[j][2 * h + 1] - base) * to_log2);
-        sum += s[j][2 * h] + s[j][2 * h + 1];
-      }
-      l_run[h] = l_run[h] * corr + sum;
-#pragma unroll
-      for (int j = 0; j < kD / 8; ++j) {
-        acc[j][2 * h] *= corr;
-        acc[j][2 * h + 1] *= corr;
-      }
-    }
+    st.template softmax<kKW>(s, to_log2, kBf16);
     // O += P V, P rounded to the operands' type
 #pragma unroll
     for (int kk = 0; kk < kKW / 16; ++kk) {
@@ -283,8 +306,8 @@ __global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_consta
         const int r = wk * kKW + kk * 16 + (lane & 15);
         uint32_t b0, b1, b2, b3;
         ldsm_x4_t(sv + tile_at<kCh>(r, jp * 2 + (lane >> 4)), b0, b1, b2, b3);
-        mma16816<kBf16>(acc[2 * jp], pa, b0, b1);
-        mma16816<kBf16>(acc[2 * jp + 1], pa, b2, b3);
+        mma16816<kBf16>(st.acc[2 * jp], pa, b0, b1);
+        mma16816<kBf16>(st.acc[2 * jp + 1], pa, b2, b3);
       }
     }
   }
@@ -297,14 +320,14 @@ __global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_consta
   const int r_lo = wm * 16 + (lane >> 2);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    float l = l_run[h];
+    float l = st.l[h];
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if ((lane & 3) == 0) ml[wk][r_lo + 8 * h] = make_float2(m_run[h], l);
+    if ((lane & 3) == 0) ml[wk][r_lo + 8 * h] = make_float2(st.m[h], l);
     float* dst = part + (wk * Cf::kRows + r_lo + 8 * h) * Cf::kOPitch + (lane & 3) * 2;
 #pragma unroll
     for (int j = 0; j < kD / 8; ++j)
-      *reinterpret_cast<float2*>(dst + j * 8) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+      *reinterpret_cast<float2*>(dst + j * 8) = make_float2(st.acc[j][2 * h], st.acc[j][2 * h + 1]);
   }
   __syncthreads();
   // The weight of each key warp's partial row against the row's maximum over
@@ -394,6 +417,182 @@ __global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_consta
   if (splits > 1) cluster_sync();  // the others may still read this CTA's partial rows
 }
 
+// Few keys, many rows: the CTA keeps K and V of its key head in shared memory
+// and its warps walk 16-row tiles on their own: the next tile's queries are
+// copied while this one is computed, and no barrier is met in the loop.  Q is
+// read and O written once, which is what bounds it.
+template <int kD>
+struct KeepCfg {
+  static constexpr int kChunks = kD / 8;
+  static constexpr int kQBytes = 16 * kD * 2;  // a warp's tile, two of them
+  static int smem(int keys) { return (keys + 15) / 16 * 16 * kD * 2 * 2 + (kThreads / 32) * 2 * kQBytes; }
+};
+
+template <bool kBf16, int kD, bool kBias>
+__global__ void __launch_bounds__(kThreads) cross_keep_kernel(const __grid_constant__ CrossParams p, int chunks) {
+  using Cf = KeepCfg<kD>;
+  constexpr int kCh = Cf::kChunks, kKW = 64, kWarps = kThreads / 32;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint32_t on[kMaxKeep / 32];  // bit per key that counts
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kp = (p.sk + 15) & ~15;
+  const int chunk = blockIdx.x % chunks, bh = blockIdx.x / chunks;
+  const int kvh = bh % p.kv_heads, b = bh / p.kv_heads;
+  const int len = cross_len(p, b);
+  const uint32_t sk = smem_u32(smem), sv = sk + kp * kD * 2;
+  const uint32_t sq = sv + kp * kD * 2 + warp * 2 * Cf::kQBytes;
+  const uint16_t* kg = p.k + b * p.kb + kvh * p.kh;
+  const uint16_t* vg = p.v + b * p.vb + kvh * p.vh;
+  const uint8_t* mg = p.key_mask ? p.key_mask + b * p.mask_stride : nullptr;
+
+  // this CTA's 16-row tiles, dealt to its warps
+  const int tiles = (p.rows + 15) / 16;
+  const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * chunk / chunks);
+  const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (chunk + 1) / chunks);
+  auto load_q = [&](int t, int buf) {
+    if (t < t1) {
+#pragma unroll
+      for (int i = 0; i < 16 * kCh / 32; ++i) {
+        const int r = (lane + i * 32) / kCh, c = (lane + i * 32) % kCh, row = t * 16 + r;
+        const bool ok = row < p.rows && c * 8 < p.head_dim;
+        const int q = ok ? row / p.group : 0, h = ok ? row - q * p.group : 0;
+        const uint16_t* src = p.q + b * p.qb + q * p.qs + (kvh * p.group + h) * p.qh + (ok ? c * 8 : 0);
+        cp_async16(sq + buf * Cf::kQBytes + tile_at<kCh>(r, c), src, ok);
+      }
+    }
+    cp_async_commit();
+  };
+  for (int i = tid; i < kp * kCh; i += kThreads) {
+    const int r = i / kCh, c = i % kCh;
+    bool ok = r < len && c * 8 < p.head_dim;
+    if (mg && ok) ok = mg[r] != 0;
+    const int64_t at = ok ? r : 0;
+    const int cc = ok ? c * 8 : 0;
+    cp_async16(sk + tile_at<kCh>(r, c), kg + at * p.ks + cc, ok);
+    cp_async16(sv + tile_at<kCh>(r, c), vg + at * p.vs + cc, ok);
+  }
+  load_q(t0 + warp, 0);
+  for (int w = warp; w < (kp + 31) / 32; w += kWarps) {
+    const int key = w * 32 + lane;
+    const uint32_t bits = __ballot_sync(0xffffffffu, key < len && (!mg || mg[key] != 0));
+    if (lane == 0) on[w] = bits;
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+
+  const float to_log2 = kBias ? kLog2e : p.scale_log2;
+  int buf = 0;
+  for (int t = t0 + warp; t < t1; t += kWarps, buf ^= 1) {
+    load_q(t + kWarps, buf ^ 1);
+    cp_async_wait<1>();
+    __syncwarp();
+    const uint32_t mine = sq + buf * Cf::kQBytes;
+    uint32_t qf[kD / 16][4];
+#pragma unroll
+    for (int kk = 0; kk < kD / 16; ++kk)
+      ldsm_x4(mine + tile_at<kCh>(lane & 15, kk * 2 + (lane >> 4)), qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3]);
+    const float* brow[2] = {nullptr, nullptr};
+    if (kBias) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = min(t * 16 + (lane >> 2) + 8 * h, p.rows - 1);
+        brow[h] = p.bias + b * p.bb + (kvh * p.group + r % p.group) * p.bh + (r / p.group) * p.bs;
+      }
+    }
+    RowState<kD> st;
+    st.clear();
+    for (int k0 = 0; k0 < len; k0 += kKW) {
+      const int n = min(kKW, (len - k0 + 15) & ~15);  // keys of the chunk, a multiple of 16
+      float s[kKW / 8][4];
+#pragma unroll
+      for (int jp = 0; jp < kKW / 16; ++jp) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[2 * jp][e] = s[2 * jp + 1][e] = 0.f;
+        if (jp * 16 < n) {
+#pragma unroll
+          for (int kk = 0; kk < kD / 16; ++kk) {
+            const int r = k0 + jp * 16 + (lane & 7) + (lane >> 4) * 8;
+            uint32_t b0, b1, b2, b3;
+            ldsm_x4(sk + tile_at<kCh>(r, kk * 2 + ((lane >> 3) & 1)), b0, b1, b2, b3);
+            mma16816<kBf16>(s[2 * jp], qf[kk], b0, b1);
+            mma16816<kBf16>(s[2 * jp + 1], qf[kk], b2, b3);
+          }
+        }
+      }
+      const uint64_t bits = static_cast<uint64_t>(on[k0 / 32]) |
+                            (k0 + 32 < kp ? static_cast<uint64_t>(on[k0 / 32 + 1]) << 32 : 0ull);
+#pragma unroll
+      for (int j = 0; j < kKW / 8; ++j) {
+        if (kBias && j * 8 < n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = k0 + j * 8 + (lane & 3) * 2 + (e & 1);
+            s[j][e] = fmaf(s[j][e], p.scale, key < len ? __ldg(brow[e >> 1] + key) : 0.f);
+          }
+        }
+      }
+      if (bits != ~0ull) {
+        const uint64_t mine_on = bits >> ((lane & 3) * 2);
+#pragma unroll
+        for (int j = 0; j < kKW / 8; ++j) {
+          if (!(mine_on >> (j * 8) & 1)) s[j][0] = s[j][2] = -INFINITY;
+          if (!(mine_on >> (j * 8 + 1) & 1)) s[j][1] = s[j][3] = -INFINITY;
+        }
+      }
+      st.template softmax<kKW>(s, to_log2, kBf16);
+      // O += P V, P rounded to the operands' type
+#pragma unroll
+      for (int kk = 0; kk < kKW / 16; ++kk) {
+        if (kk * 16 < n) {
+          uint32_t pa[4];
+          pa[0] = pack2<kBf16>(s[2 * kk][0], s[2 * kk][1]);
+          pa[1] = pack2<kBf16>(s[2 * kk][2], s[2 * kk][3]);
+          pa[2] = pack2<kBf16>(s[2 * kk + 1][0], s[2 * kk + 1][1]);
+          pa[3] = pack2<kBf16>(s[2 * kk + 1][2], s[2 * kk + 1][3]);
+#pragma unroll
+          for (int jp = 0; jp < kD / 16; ++jp) {
+            const int r = k0 + kk * 16 + (lane & 15);
+            uint32_t b0, b1, b2, b3;
+            ldsm_x4_t(sv + tile_at<kCh>(r, jp * 2 + (lane >> 4)), b0, b1, b2, b3);
+            mma16816<kBf16>(st.acc[2 * jp], pa, b0, b1);
+            mma16816<kBf16>(st.acc[2 * jp + 1], pa, b2, b3);
+          }
+        }
+      }
+    }
+    // O over the tile's queries in shared memory, then rows in 16-byte pieces
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float l = st.l[h];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays NaN
+      const int r = (lane >> 2) + 8 * h;
+#pragma unroll
+      for (int j = 0; j < kD / 8; ++j) {
+        const uint32_t w = pack2<kBf16>(st.acc[j][2 * h] * inv, st.acc[j][2 * h + 1] * inv);
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(mine + tile_at<kCh>(r, j) + (lane & 3) * 4), "r"(w) : "memory");
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16 * kCh / 32; ++i) {
+      const int r = (lane + i * 32) / kCh, c = (lane + i * 32) % kCh, row = t * 16 + r;
+      if (row < p.rows && c * 8 < p.head_dim) {
+        uint4 w;
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                     : "r"(mine + tile_at<kCh>(r, c))
+                     : "memory");
+        const int q = row / p.group, h = row - q * p.group;
+        *reinterpret_cast<uint4*>(p.o + b * p.ob + q * p.os + (kvh * p.group + h) * p.oh + c * 8) = w;
+      }
+    }
+    __syncwarp();  // the buffer's next queries may come
+  }
+}
+
 template <bool kBf16, int kD, int kWM, bool kBias>
 int launch_variant(const CrossParams& p, cudaStream_t st) {
   using Cf = Cfg<kD, kWM>;
@@ -430,8 +629,35 @@ int launch_variant(const CrossParams& p, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, kernel, p, static_cast<int>(row_tiles), splits) == cudaSuccess ? kOk : kErrLaunch;
 }
 
+template <bool kBf16, int kD, bool kBias>
+int launch_keep(const CrossParams& p, cudaStream_t st) {
+  const auto kernel = cross_keep_kernel<kBf16, kD, kBias>;
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return kErrCuda;
+  if (dev >= 64 || !(ready.load() >> dev & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess)
+      return kErrCuda;
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  const int smem = KeepCfg<kD>::smem(p.sk);
+  // as many CTAs as the SMs hold at once (about 200 registers a thread for
+  // D = 128, and the shared memory), each with a share of the rows
+  const int64_t bh = static_cast<int64_t>(p.kv_heads) * p.batch;
+  const int per_sm = std::min(kD == 128 ? 2 : kD == 64 ? 4 : 6, 200 * 1024 / smem);
+  const int tiles = (p.rows + 15) / 16;
+  int64_t chunks = std::max<int64_t>(1, static_cast<int64_t>(per_sm) * num_sms() / bh);
+  chunks = std::min<int64_t>(chunks, (tiles + kThreads / 32 - 1) / (kThreads / 32));
+  if (bh * chunks > 0x7fffffffLL) return kErrShape;
+  count_launches(1);
+  kernel<<<static_cast<unsigned>(bh * chunks), kThreads, smem, st>>>(p, static_cast<int>(chunks));
+  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+}
+
 template <bool kBf16, int kD>
 int launch_rows(const CrossParams& p, cudaStream_t st) {
+  if (p.rows > 64 && p.sk <= S3_KEEP && KeepCfg<kD>::smem(p.sk) <= 100 * 1024)
+    return p.bias ? launch_keep<kBf16, kD, true>(p, st) : launch_keep<kBf16, kD, false>(p, st);
   if (p.rows <= 16)
     return p.bias ? launch_variant<kBf16, kD, 1, true>(p, st) : launch_variant<kBf16, kD, 1, false>(p, st);
   return p.bias ? launch_variant<kBf16, kD, 4, true>(p, st) : launch_variant<kBf16, kD, 4, false>(p, st);
@@ -511,6 +737,6 @@ extern "C" int sam3cu_cross_attention(const struct sam3cu_cross_attention_args* 
     p.bs = a->bias_strides[2];
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (cross_tc_takes(p) && p.rows > 64 && p.sk > 256) return launch_cross_tc(p, a->dtype, st);
+  if (cross_tc_takes(p) && p.rows > 64 && p.sk > S3_TCK) return launch_cross_tc(p, a->dtype, st);
   return launch_cross_mma(p, a->dtype, st);
 }
