@@ -11,7 +11,9 @@
 // tensor cores work for the other, and a K / V tile read from L2 serves 256
 // rows.  Twelve warps:
 //   warp 0      TMA: the Q tiles, then K and V through rings of their own
-//   warp 1      MMA issue and the TMEM allocation
+//   warps 1, 3  MMA issue, one for each query tile: with one for both, the tiles
+//               ran in step, both on the exponential units and then both not
+//               (warp 1 also allocates TMEM)
 //   warp 2      with a mask or lengths: key bits of each tile, and zeros over
 //               V rows of keys that do not count (0 * NaN would reach O)
 //   warps 4-7, 8-11   softmax and epilogue of tile 0 and 1; warp w owns TMEM
@@ -24,8 +26,10 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdint>
+#include <cstdlib>
 #include <cstring>
 
 #include "attention_math.cuh"
@@ -43,7 +47,6 @@ namespace {
 constexpr int kQ = 128;        // rows of a tile
 constexpr int kKV = 128;       // keys of a tile
 constexpr int kThreads = 384;
-constexpr int kSoftThreads = 256;
 constexpr float kRescaleLog2 = 8.f;
 // f16 P below 2^-14 loses bits: with a maximum of 2^8 (lazy rescaling) there
 // is room for a factor 2^6 under 65504.  It cancels in O / sum.
@@ -64,13 +67,82 @@ struct Cfg {
   static_assert(2 * kQ * kPitch * 4 <= kSmem, "partial rows fit over the rings");
 };
 
+// A value that the compiler may not compute ahead of its place.
+__device__ __forceinline__ uint64_t here(uint64_t v) {
+  asm volatile("" : "+l"(v));
+  return v;
+}
+__device__ __forceinline__ uint32_t here(uint32_t v) {
+  asm volatile("" : "+r"(v));
+  return v;
+}
+
 struct TcParams {
   CrossParams c;
   int qpt;        // queries of a tile: 128 / group
   int items_x;    // row items of a (batch, key head)
+  int n_items;    // items_x * kv_heads * batch
   int tiles;      // 128-row tiles of an item: 1 or 2
-  int splits;     // CTAs of the cluster that share an item's keys
+  int splits;     // CTAs of the cluster that share an item's keys (then one item a CTA)
   int kmul_b, kmul_h, vmul_b, vmul_h, qmul_b;  // 0: that dimension is shared
+};
+
+// One work item: up to two query tiles of a (batch, key head) and the key
+// tiles [j0, j0 + n_kv) that this CTA takes.
+struct Item {
+  int b, kvh, q0, tiles, len, j0, n_kv;
+};
+__device__ __forceinline__ Item item_of(const TcParams& prm, int idx, int split) {
+  Item it;
+  const int bh = idx / prm.items_x;
+  it.q0 = (idx - bh * prm.items_x) * prm.tiles * prm.qpt;
+  it.tiles = it.q0 + prm.qpt < prm.c.sq ? prm.tiles : 1;  // the second may lie past the last query
+  it.b = bh / prm.c.kv_heads;
+  it.kvh = bh - it.b * prm.c.kv_heads;
+  it.len = cross_len(prm.c, it.b);
+  const int all = (it.len + kKV - 1) / kKV;
+  it.j0 = static_cast<int>(static_cast<int64_t>(all) * split / prm.splits);
+  it.n_kv = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / prm.splits) - it.j0;
+  return it;
+}
+
+// Walks the (item, key tile) pairs of a CTA; items without keys are passed over.
+struct Cursor {
+  int idx, j;      // item, key tile of it
+  int kt;          // key tiles before it: place in the rings
+  int nth, nth_b;  // items before it, and those with a second query tile,
+  int kt_b;        //   and their key tiles: phases of the query tiles' barriers
+  Item it;
+  __device__ __forceinline__ bool more(const TcParams& prm) const { return idx < prm.n_items; }
+  __device__ __forceinline__ void find(const TcParams& prm, int step, int split) {
+    for (; idx < prm.n_items; idx += step) {
+      it = item_of(prm, idx, split);
+      if (it.n_kv > 0) break;
+    }
+  }
+  __device__ __forceinline__ void start(const TcParams& prm, int first, int step, int split) {
+    idx = first;
+    j = kt = nth = nth_b = kt_b = 0;
+    find(prm, step, split);
+  }
+  __device__ __forceinline__ void next(const TcParams& prm, int step, int split) {
+    ++kt;
+    kt_b += it.tiles > 1;
+    if (++j == it.n_kv) {
+      j = 0;
+      ++nth;
+      nth_b += it.tiles > 1;
+      idx += step;
+      find(prm, step, split);
+    }
+  }
+  __device__ __forceinline__ int items(int t) const { return t ? nth_b : nth; }
+  __device__ __forceinline__ int turns(int t) const { return t ? kt_b : kt; }
+  // keys of the tile, rounded up to a multiple of 16
+  __device__ __forceinline__ int keys() const {
+    const int left = it.len - (it.j0 + j) * kKV;
+    return left >= kKV ? kKV : ((left + 15) & ~15);
+  }
 };
 
 template <bool kBf16, int kD, bool kMask>
@@ -80,18 +152,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   using Cf = Cfg<kD>;
   constexpr int kStages = Cf::kStages, kTile = Cf::kTile;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ uint64_t bars[1 + 2 * 6 + 4 * kStages + 2 * kStages];
+  __shared__ uint64_t bars[16 + 6 * kStages];
   __shared__ uint32_t bits[kMask ? kStages : 1][4];
   __shared__ float2 ml[2 * kQ];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag_s;
+  // [2] by tile; phases: per item (q, o) or per key tile (s, p)
   uint64_t* q_full = &bars[0];
-  uint64_t* s_full = &bars[1];    // [2] by tile
-  uint64_t* s_empty = &bars[3];   // [2]
-  uint64_t* p_full = &bars[5];    // [2]
-  uint64_t* p_empty = &bars[7];   // [2]
-  uint64_t* o_full = &bars[9];    // [2]
-  uint64_t* k_full = &bars[13];
+  uint64_t* q_empty = &bars[2];
+  uint64_t* o_full = &bars[4];
+  uint64_t* o_empty = &bars[6];
+  uint64_t* s_full = &bars[8];
+  uint64_t* s_empty = &bars[10];
+  uint64_t* p_full = &bars[12];
+  uint64_t* p_empty = &bars[14];
+  // [kStages]
+  uint64_t* k_full = &bars[16];
   uint64_t* k_empty = k_full + kStages;
   uint64_t* v_full = k_empty + kStages;
   uint64_t* v_empty = v_full + kStages;
@@ -101,15 +177,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const CrossParams& p = prm.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = blockIdx.x % prm.splits, item = blockIdx.x / prm.splits;
-  const int ix = item % prm.items_x, bh = item / prm.items_x;
-  const int kvh = bh % p.kv_heads, b = bh / p.kv_heads;
-  const int q0 = ix * prm.tiles * prm.qpt;  // first query of the item
-  const int tiles = min(prm.tiles, (p.sq - q0 + prm.qpt - 1) / prm.qpt);
-  const int len = cross_len(p, b);
-  const int all_kv = (len + kKV - 1) / kKV;
-  const int j0 = static_cast<int>(static_cast<int64_t>(all_kv) * split / prm.splits);
-  const int n_kv = static_cast<int>(static_cast<int64_t>(all_kv) * (split + 1) / prm.splits) - j0;
+  const int split = blockIdx.x % prm.splits;
+  const int first = blockIdx.x / prm.splits, step = gridDim.x / prm.splits;
 
   uint8_t* sQ = smem;
   auto sK = [&](int st) { return smem + 2 * kTile + st * kTile; };
@@ -117,19 +186,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool aligned = (smem_u32(smem) & 1023u) == 0;  // the swizzled layouts need it
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
     for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 1);
+      mbar_init(&q_empty[t], 1);
+      mbar_init(&o_full[t], 1);
+      mbar_init(&o_empty[t], 4);
       mbar_init(&s_full[t], 1);
       mbar_init(&s_empty[t], 4);
       mbar_init(&p_full[t], 4);
       mbar_init(&p_empty[t], 1);
-      mbar_init(&o_full[t], 1);
     }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], prm.tiles);
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], prm.tiles);
       mbar_init(&v_ready[i], 1);
       mbar_init(&w_ready[i], 1);
     }
@@ -148,135 +219,158 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto tS = [&](int t) { return tmem + static_cast<uint32_t>(t * 128); };
   auto tO = [&](int t) { return tmem + Cf::kOCol + static_cast<uint32_t>(t * kD); };
   auto tP = [&](int t) { return Cf::kOwnP ? tmem + Cf::kPCol + static_cast<uint32_t>(t * 64) : tS(t); };
-  const bool run = aligned && n_kv > 0;
-  auto keys_in = [&](int j) {  // keys of tile j, rounded up to a multiple of 16
-    const int left = len - (j0 + j) * kKV;
-    return left >= kKV ? kKV : ((left + 15) & ~15);
-  };
 
-  if (warp == 0 && run) {
+  if (warp == 0 && aligned) {
     // ------------------------------------------------------------ TMA
-    const int kb = b * prm.kmul_b, kh = kvh * prm.kmul_h, vb = b * prm.vmul_b, vh = kvh * prm.vmul_h;
     if (elect_one()) {
       tma_prefetch_desc(&tq);
       tma_prefetch_desc(&tk);
       tma_prefetch_desc(&tv);
-      mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(tiles * Cf::kHalves * Cf::kRowBytes * p.group * prm.qpt));
-      for (int t = 0; t < tiles; ++t)
-        for (int h = 0; h < Cf::kHalves; ++h)
-          tma_load_4d(sQ + t * kTile + h * (kTile / 2), &tq, q_full, h * 64, kvh * p.group, q0 + t * prm.qpt,
-                      b * prm.qmul_b);
     }
     __syncwarp();
-    for (int j = 0; j < n_kv; ++j) {
-      const int st = j % kStages;
-      const uint32_t ph = ((j / kStages) & 1) ^ 1;
+    Cursor c;
+    c.start(prm, first, step, split);
+    for (; c.more(prm); c.next(prm, step, split)) {
+      const Item& it = c.it;
+      const int st = c.kt % kStages;
+      const uint32_t ph = ((c.kt / kStages) & 1) ^ 1;
+      const int row = (it.j0 + c.j) * kKV;
       if (!mbar_wait_warp(&k_empty[st], ph, kErrStageFree, abort_flag)) break;
       if (elect_one()) {
         mbar_arrive_expect_tx(&k_full[st], kTile);
         for (int h = 0; h < Cf::kHalves; ++h)
-          tma_load_4d(sK(st) + h * (kTile / 2), &tk, &k_full[st], h * 64, (j0 + j) * kKV, kh, kb);
+          tma_load_4d(sK(st) + h * (kTile / 2), &tk, &k_full[st], h * 64, row, it.kvh * prm.kmul_h,
+                      it.b * prm.kmul_b);
       }
       __syncwarp();
+      if (c.j == 0) {
+        bool ok = true;
+        for (int t = 0; ok && t < it.tiles; ++t) {
+          // the item before has made its last S from this tile's queries
+          ok = mbar_wait_warp(&q_empty[t], (c.items(t) & 1) ^ 1, kErrStageFree, abort_flag);
+          if (ok && elect_one()) {
+            mbar_arrive_expect_tx(&q_full[t],
+                                  static_cast<uint32_t>(Cf::kHalves * Cf::kRowBytes * p.group * prm.qpt));
+            for (int h = 0; h < Cf::kHalves; ++h)
+              tma_load_4d(sQ + t * kTile + h * (kTile / 2), &tq, &q_full[t], h * 64, it.kvh * p.group,
+                          it.q0 + t * prm.qpt, it.b * prm.qmul_b);
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+      }
       if (!mbar_wait_warp(&v_empty[st], ph, kErrStageFree, abort_flag)) break;
       if (elect_one()) {
         mbar_arrive_expect_tx(&v_full[st], kTile);
         for (int h = 0; h < Cf::kHalves; ++h)
-          tma_load_4d(sV(st) + h * (kTile / 2), &tv, &v_full[st], h * 64, (j0 + j) * kKV, vh, vb);
+          tma_load_4d(sV(st) + h * (kTile / 2), &tv, &v_full[st], h * 64, row, it.kvh * prm.vmul_h,
+                      it.b * prm.vmul_b);
       }
       __syncwarp();
     }
-  } else if (warp == 1 && run) {
+  } else if ((warp == 1 || warp == 3) && warp / 2 < prm.tiles && aligned) {
     // ------------------------------------------------------------ MMA
+    const int t = warp / 2;
     const uint32_t fmt = kBf16 ? 1u : 0u;
     const uint32_t idesc_pv = make_idesc(fmt, kQ, kD, 1u);
     auto sdesc_k = [](uint32_t a) { return kD == 32 ? make_sdesc_sw64(a) : make_sdesc_sw128(a); };
     auto sdesc_mn = [](uint32_t a) { return kD == 32 ? make_sdesc_sw64_mn(a) : make_sdesc_sw128_mn(a); };
     constexpr uint32_t kHalfStep = kTile / 2 >> 4;            // the second 64 columns of a D = 128 tile
     constexpr uint32_t kVStep = 16 * Cf::kRowBytes >> 4;      // 16 keys of V
-    const uint64_t qdesc[2] = {sdesc_k(smem_u32(sQ)), sdesc_k(smem_u32(sQ + kTile))};
-    // S_t = Q_t K_j^T, once the softmax has read the S before it
-    auto issue_s = [&](int t, int j) -> bool {
-      const int st = j % kStages;
-      if (Cf::kOwnP && !mbar_wait_warp(&s_empty[t], (j & 1) ^ 1, kErrAccFree, abort_flag)) return false;
-      tc_fence_after();
-      const uint64_t kdesc = sdesc_k(smem_u32(sK(st)));
-      const uint32_t idesc_s = make_idesc(fmt, kQ, keys_in(j));
-#pragma unroll
-      for (int kk = 0; kk < kD / 16; ++kk) {  // 16 elements = 32 bytes along D
-        const uint64_t at = (kk / 4) * kHalfStep + 2 * (kk % 4);
-        umma_ss_warp(tS(t), qdesc[t] + at, kdesc + at, idesc_s, kk ? 1u : 0u);
-      }
-      umma_commit_warp(&s_full[t]);
-      return true;
-    };
-    auto issue_tile_s = [&](int j) -> bool {  // both tiles' S, then K_j is free
-      if (!mbar_wait_warp(&k_full[j % kStages], (j / kStages) & 1, kErrTmaWait, abort_flag)) return false;
-      for (int t = 0; t < tiles; ++t)
-        if (!issue_s(t, j)) return false;
-      umma_commit_warp(&k_empty[j % kStages]);
-      return true;
-    };
-    bool ok = mbar_wait_warp(q_full, 0, kErrTmaWait, abort_flag) && issue_tile_s(0);
-    for (int j = 0; ok && j < n_kv; ++j) {
-      const int st = j % kStages, n = keys_in(j);
-      if (Cf::kOwnP && j + 1 < n_kv && !issue_tile_s(j + 1)) break;  // beside the softmax of tile j
-      if (!mbar_wait_warp(&v_full[st], (j / kStages) & 1, kErrTmaWait, abort_flag)) break;
-      if (kMask && !mbar_wait_warp(&v_ready[st], (j / kStages) & 1, kErrTmaWait, abort_flag)) break;
-      if (!Cf::kOwnP && j + 1 < n_kv &&
-          !mbar_wait_warp(&k_full[(j + 1) % kStages], ((j + 1) / kStages) & 1, kErrTmaWait, abort_flag))
-        break;
-      const uint64_t vdesc = sdesc_mn(smem_u32(sV(st)));
-      for (int t = 0; ok && t < tiles; ++t) {
-        if (!mbar_wait_warp(&p_full[t], j & 1, kErrAccFull, abort_flag)) {
-          ok = false;
-          break;
-        }
+    const uint64_t qdesc = sdesc_k(smem_u32(sQ + t * kTile));
+    // S = Q K_j^T, once the softmax has read the S before it
+    auto issue_s = [&](const Cursor& c) -> bool {
+      const int st = c.kt % kStages;
+      if (!mbar_wait_warp(&k_full[st], (c.kt / kStages) & 1, kErrTmaWait, abort_flag)) return false;
+      if (t < c.it.tiles) {
+        if (c.j == 0 && !mbar_wait_warp(&q_full[t], c.items(t) & 1, kErrTmaWait, abort_flag)) return false;
+        if (Cf::kOwnP && !mbar_wait_warp(&s_empty[t], (c.turns(t) & 1) ^ 1, kErrAccFree, abort_flag)) return false;
         tc_fence_after();
+        const uint64_t kdesc = sdesc_k(smem_u32(sK(st)));
+        const uint32_t idesc_s = make_idesc(fmt, kQ, c.keys());
+#pragma unroll
+        for (int kk = 0; kk < kD / 16; ++kk) {  // 16 elements = 32 bytes along D
+          const uint64_t at = (kk / 4) * kHalfStep + 2 * (kk % 4);
+          umma_ss_warp(tS(t), qdesc + at, kdesc + at, idesc_s, kk ? 1u : 0u);
+        }
+        umma_commit_warp(&s_full[t]);
+        if (c.j == c.it.n_kv - 1) umma_commit_warp(&q_empty[t]);
+      }
+      umma_commit_warp(&k_empty[st]);  // (an item without this query tile: nothing to wait for)
+      return true;
+    };
+    Cursor s, c;  // of the next S, and of P.V behind it
+    s.start(prm, first, step, split);
+    c = s;
+    bool ok = true;
+    if (s.more(prm)) {
+      ok = issue_s(s);
+      s.next(prm, step, split);
+    }
+    for (; ok && c.more(prm); c.next(prm, step, split)) {
+      const int st = c.kt % kStages, n = c.keys();
+      if (Cf::kOwnP && s.more(prm)) {  // the next S, beside this tile's softmax
+        ok = issue_s(s);
+        if (!ok) break;
+        s.next(prm, step, split);
+      }
+      if (!mbar_wait_warp(&v_full[st], (c.kt / kStages) & 1, kErrTmaWait, abort_flag)) break;
+      if (kMask && !mbar_wait_warp(&v_ready[st], (c.kt / kStages) & 1, kErrTmaWait, abort_flag)) break;
+      if (t < c.it.tiles) {
+        // the epilogue of the item before has read O
+        if (c.j == 0 && c.items(t) > 0 &&
+            !mbar_wait_warp(&o_empty[t], (c.items(t) - 1) & 1, kErrAccFree, abort_flag))
+          break;
+        if (!mbar_wait_warp(&p_full[t], c.turns(t) & 1, kErrAccFull, abort_flag)) break;
+        tc_fence_after();
+        const uint64_t vdesc = sdesc_mn(smem_u32(sV(st)));
         if (n == kKV) {
 #pragma unroll
           for (int kk = 0; kk < kKV / 16; ++kk)  // A = P from TMEM: 16 keys = 8 columns
-            umma_ts_warp(tO(t), tP(t) + kk * 8, vdesc + kk * kVStep, idesc_pv, (j | kk) ? 1u : 0u);
+            umma_ts_warp(tO(t), tP(t) + kk * 8, vdesc + kk * kVStep, idesc_pv, (c.j | kk) ? 1u : 0u);
         } else {
+#pragma unroll 1
           for (int kk = 0; kk < n / 16; ++kk)
-            umma_ts_warp(tO(t), tP(t) + kk * 8, vdesc + kk * kVStep, idesc_pv, (j | kk) ? 1u : 0u);
+            umma_ts_warp(tO(t), tP(t) + kk * 8, vdesc + kk * kVStep, idesc_pv, (c.j | kk) ? 1u : 0u);
         }
         if (Cf::kOwnP) umma_commit_warp(&p_empty[t]);
-        if (j == n_kv - 1) umma_commit_warp(&o_full[t]);
-        // P has been consumed in issue order: its S columns may be written
-        if (!Cf::kOwnP && j + 1 < n_kv && !issue_s(t, j + 1)) ok = false;
+        if (c.j == c.it.n_kv - 1) umma_commit_warp(&o_full[t]);
       }
-      if (!Cf::kOwnP && ok && j + 1 < n_kv) umma_commit_warp(&k_empty[(j + 1) % kStages]);
       umma_commit_warp(&v_empty[st]);
+      // P has been consumed in issue order: its S columns may be written
+      if (!Cf::kOwnP && s.more(prm)) {
+        ok = issue_s(s);
+        s.next(prm, step, split);
+      }
     }
-  } else if (kMask && warp == 2 && run) {
+  } else if (kMask && warp == 2 && aligned) {
     // ---------------------------------------------- key bits, V scrubbing
-    const uint8_t* mg = p.key_mask ? p.key_mask + b * p.mask_stride : nullptr;
-    for (int j = 0; j < n_kv; ++j) {
-      const int st = j % kStages;
+    Cursor c;
+    c.start(prm, first, step, split);
+    for (; c.more(prm); c.next(prm, step, split)) {
+      const uint8_t* mg = p.key_mask ? p.key_mask + c.it.b * p.mask_stride : nullptr;
+      const int st = c.kt % kStages, n = c.keys();
       // the bits' slot is free with its V stage: both softmaxes are past it
-      if (!mbar_wait_warp(&v_empty[st], ((j / kStages) & 1) ^ 1, kErrStageFree, abort_flag)) break;
+      if (!mbar_wait_warp(&v_empty[st], ((c.kt / kStages) & 1) ^ 1, kErrStageFree, abort_flag)) break;
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int key = (j0 + j) * kKV + i * 32 + lane;
-        const bool on = key < len && (!mg || mg[key] != 0);
-        w[i] = __ballot_sync(0xffffffffu, on);
+        const int key = (c.it.j0 + c.j) * kKV + i * 32 + lane;
+        w[i] = __ballot_sync(0xffffffffu, key < c.it.len && (!mg || mg[key] != 0));
       }
       if (lane < 4) bits[kMask ? st : 0][lane] = lane == 0 ? w[0] : lane == 1 ? w[1] : lane == 2 ? w[2] : w[3];
       __syncwarp();
       if (lane == 0) mbar_arrive(&w_ready[st]);
-      if (!mbar_wait_warp(&v_full[st], (j / kStages) & 1, kErrTmaWait, abort_flag)) break;
+      if (!mbar_wait_warp(&v_full[st], (c.kt / kStages) & 1, kErrTmaWait, abort_flag)) break;
       if ((w[0] & w[1] & w[2] & w[3]) != 0xffffffffu) {
-        const int n = keys_in(j);  // rows past it are not multiplied
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (!(w[i] >> lane & 1) && i * 32 + lane < n) {
+          if (!(w[i] >> lane & 1) && i * 32 + lane < n) {  // (rows past n are not multiplied)
             uint8_t* row = sV(st) + (i * 32 + lane) * Cf::kRowBytes;
             for (int h = 0; h < Cf::kHalves; ++h)
 #pragma unroll
-              for (int c = 0; c < Cf::kRowBytes; c += 16)
-                *reinterpret_cast<uint4*>(row + h * (kTile / 2) + c) = make_uint4(0, 0, 0, 0);
+              for (int k = 0; k < Cf::kRowBytes; k += 16)
+                *reinterpret_cast<uint4*>(row + h * (kTile / 2) + k) = make_uint4(0, 0, 0, 0);
           }
         }
         fence_proxy_async_smem();
@@ -290,125 +384,159 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int r = quarter * 32 + lane;  // row within the tile
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const float sl2 = p.scale_log2;
-    const int query = q0 + t * prm.qpt + r / p.group;
-    const bool row_live = t < tiles && r < prm.qpt * p.group && query < p.sq;
-    // a warp of dead rows only keeps the barriers going
-    const bool live = __any_sync(0xffffffffu, row_live);
-    float m_used = -INFINITY, l = 0.f;
-    bool ok = run && t < tiles;
-    for (int j = 0; ok && j < n_kv; ++j) {
-      const int st = j % kStages;
-      if (!warp_wait(&s_full[t], j & 1, kErrAccFull, abort_flag, lane)) { ok = false; break; }
-      tc_fence_after();
-      uint32_t su[kKV];
-      float* sv = reinterpret_cast<float*>(su);
-      if (live) {
-#pragma unroll
-        for (int c = 0; c < kKV / 32; ++c)
-          tmem_ld_32x32b_x32(tS(t) + lane_off + c * 32, *reinterpret_cast<uint32_t(*)[32]>(su + c * 32));
-        tmem_ld_wait();
+    bool ok = aligned && t < prm.tiles;
+    int kt = 0, turn = 0, nth = 0;  // key tiles in the rings, of this query tile, its items
+    for (int idx = first; ok && idx < prm.n_items; idx += step) {
+      // What the key loop needs of the item; the epilogue works the rest out
+      // again, so that the loop has no registers to spill (S takes 128).
+      int n_kv, n;  // key tiles, keys left
+      {
+        const Item it = item_of(prm, idx, split);
+        n_kv = it.n_kv;
+        n = it.len - it.j0 * kKV;
+        if (t >= it.tiles) {
+          kt += n_kv;
+          if (prm.splits == 1) continue;
+          n_kv = 0;  // (a cluster's CTA still meets its barriers)
+        }
       }
-      if (Cf::kOwnP) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_empty[t]);  // S may be overwritten
-      }
-      if (kMask) {
-        if (!warp_wait(&w_ready[st], (j / kStages) & 1, kErrTmaWait, abort_flag, lane)) { ok = false; break; }
-        if (live) {
+      float m_used = -INFINITY, l = 0.f;
+#pragma unroll 1
+      for (int j = 0; j < n_kv; ++j, ++kt, ++turn, n -= kKV) {
+        const int st = kt % kStages;
+        if (!warp_wait(&s_full[t], turn & 1, kErrAccFull, abort_flag, lane)) { ok = false; break; }
+        tc_fence_after();
+        if (kMask && !warp_wait(&w_ready[st], (kt / kStages) & 1, kErrTmaWait, abort_flag, lane)) { ok = false; break; }
+        // S is read twice, 64 columns at a time: for the maximum, then for the
+        // exponentials.  (Held in registers for both, its 128 values leave too
+        // few: spilled, a load's registers are stored before its data arrives.)
+        auto load_s = [&](int h, float (&sv)[64]) {
+          tmem_ld_wait_32x32b_64(tS(t) + lane_off + h * 64, sv);
+          if (kMask) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t w = bits[kMask ? st : 0][i];
-            if (w != 0xffffffffu) {
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t w = bits[kMask ? st : 0][2 * h + i];
+              if (w != 0xffffffffu) {
 #pragma unroll
-              for (int c = 0; c < 32; ++c)
-                if (!(w >> c & 1)) sv[i * 32 + c] = -INFINITY;
+                for (int c = 0; c < 32; ++c)
+                  if (!(w >> c & 1)) sv[i * 32 + c] = -INFINITY;
+              }
             }
+          } else if (n < (h + 1) * 64) {  // the last tile's keys beyond the states
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+              if (h * 64 + c >= n) sv[c] = -INFINITY;
+          }
+        };
+        float mt;
+        {
+          float sv[64];
+          load_s(0, sv);
+          mt = max64(sv);
+          if (n > 64) {
+            load_s(1, sv);
+            mt = fmaxf(mt, max64(sv));
           }
         }
-      } else if (live && (j0 + j + 1) * kKV > len) {  // the last tile's keys beyond the states
-        const int n = len - (j0 + j) * kKV;
-#pragma unroll
-        for (int c = 0; c < kKV; ++c)
-          if (c >= n) sv[c] = -INFINITY;
-      }
-      const float mt = live ? max128(sv) : -INFINITY;
-      const bool need = (mt - m_used) * sl2 > kRescaleLog2;  // false for -inf - -inf
-      // P (its own columns) is free, and O at rest, after the P.V before it;
-      // with P in S's columns s_full said so already
-      if (Cf::kOwnP && j > 0 && !warp_wait(&p_empty[t], (j & 1) ^ 1, kErrAccFull, abort_flag, lane)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      if (__any_sync(0xffffffffu, need)) {
-        const float m_new = fmaxf(m_used, mt);
-        const float corr = m_used == -INFINITY ? 0.f : ex2((m_used - m_new) * sl2);
-        l *= corr;
-        m_used = m_new;
-        if (j > 0) {
-#pragma unroll
-          for (int c = 0; c < kD / 8; ++c) {
-            uint32_t u[8];
-            tmem_ld_32x32b_x8(tO(t) + lane_off + c * 8, u);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * corr);
-            tmem_st_32x32b_x8(tO(t) + lane_off + c * 8, u);
-          }
-          tmem_st_wait();
+        const bool need = (mt - m_used) * sl2 > kRescaleLog2;  // false for -inf - -inf
+        // P (its own columns) is free, and O at rest, after the P.V before it;
+        // with P in S's columns s_full said so already
+        if (Cf::kOwnP && turn > 0 && !warp_wait(&p_empty[t], (turn & 1) ^ 1, kErrAccFull, abort_flag, lane)) {
+          ok = false;
+          break;
         }
-      }
-      if (live) {
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, need)) {
+          const float m_new = fmaxf(m_used, mt);
+          const float corr = m_used == -INFINITY ? 0.f : ex2((m_used - m_new) * sl2);
+          l *= corr;
+          m_used = m_new;
+          if (j > 0) {
+#pragma unroll
+            for (int c = 0; c < kD / 8; ++c) {
+              uint32_t u[8];
+              tmem_ld_wait_32x32b_x8(tO(t) + lane_off + c * 8, u);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * corr);
+              tmem_st_32x32b_x8(tO(t) + lane_off + c * 8, u);
+            }
+            tmem_st_wait();
+          }
+        }
         // no key yet: every exponent is -inf against 0
         const float mb = (m_used == -INFINITY ? 0.f : m_used * sl2) - (kBf16 ? 0.f : kF16Shift);
         const uint64_t sc2 = f2pack(sl2, sl2), nmb2 = f2pack(-mb, -mb);
         uint64_t l2[2] = {f2pack(0.f, 0.f), f2pack(0.f, 0.f)};
 #pragma unroll
-        for (int c0 = 0; c0 < kKV; c0 += 16) {  // 16 keys -> 8 P columns
-          uint32_t pk[8];
+        for (int h = 0; h < 2; ++h) {
+          if (h * 64 < n) {  // (P of keys past the last 16 is not multiplied)
+            float sv[64];
+            load_s(h, sv);
+            if (Cf::kOwnP && (h == 1 || n <= 64)) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&s_empty[t]);  // S may be overwritten
+            }
 #pragma unroll
-          for (int c = c0; c < c0 + 16; c += 2) {
-            float e0, e1;
-            f2unpack(ffma2(f2pack(sv[c], sv[c + 1]), sc2, nmb2), e0, e1);
-            const float p0 = ex2(e0), p1 = ex2(e1);
-            l2[(c >> 1) & 1] = fadd2(l2[(c >> 1) & 1], f2pack(p0, p1));
-            pk[(c - c0) / 2] = pack2(p0, p1, kBf16);
+            for (int c0 = 0; c0 < 64; c0 += 16) {  // 16 keys -> 8 P columns
+              uint32_t pk[8];
+#pragma unroll
+              for (int c = c0; c < c0 + 16; c += 2) {
+                float e0, e1;
+                f2unpack(ffma2(f2pack(sv[c], sv[c + 1]), sc2, nmb2), e0, e1);
+                const float p0 = ex2(e0), p1 = ex2(e1);
+                l2[(c >> 1) & 1] = fadd2(l2[(c >> 1) & 1], f2pack(p0, p1));
+                pk[(c - c0) / 2] = pack2(p0, p1, kBf16);
+              }
+              tmem_st_32x32b_x8(tP(t) + lane_off + h * 32 + c0 / 2, *reinterpret_cast<const uint32_t(*)[8]>(pk));
+            }
           }
-          tmem_st_32x32b_x8(tP(t) + lane_off + c0 / 2, *reinterpret_cast<const uint32_t(*)[8]>(pk));
         }
         float a0, a1;
         f2unpack(fadd2(l2[0], l2[1]), a0, a1);
         l += a0 + a1;
         tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[t]);
-    }
-    bool have_o = false;  // O holds sums (with no key tile it holds nothing)
-    if (ok) {
-      have_o = warp_wait(&o_full[t], 0, kErrAccFull, abort_flag, lane);
-      ok = have_o;
-    }
-    tc_fence_after();
-    if (prm.splits == 1) {
-      if (live && (ok || n_kv == 0)) {
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays NaN
-        uint16_t* orow = p.o + b * p.ob + query * p.os +
-                         static_cast<int64_t>(kvh * p.group + r % p.group) * p.oh;
+      if (ok && n_kv > 0) ok = warp_wait(&o_full[t], nth & 1, kErrAccFull, abort_flag, lane);
+      if (!ok && prm.splits == 1) break;  // (a cluster's CTA still meets its barriers)
+      tc_fence_after();
+      const Item it = item_of(prm, static_cast<int>(here(static_cast<uint32_t>(idx))), split);
+      const int rq = r / p.group, rh = r - rq * p.group, query = it.q0 + t * prm.qpt + rq;
+      const bool row_live = r < prm.qpt * p.group && query < p.sq;
+      if (prm.splits > 1) {
+        // this CTA's share of the keys: (max, sum) and the partial row, over
+        // the rings once neither tile's MMAs read them
+        asm volatile("bar.sync 1, %0;" ::"r"(prm.tiles * kQ) : "memory");
+        ml[t * kQ + r] = make_float2(m_used, l);
+        float* part = reinterpret_cast<float*>(smem) + (t * kQ + r) * Cf::kPitch;
 #pragma unroll
         for (int c0 = 0; c0 < kD; c0 += 16) {
           uint32_t u[16];
-          tmem_ld_32x32b_x16(tO(t) + lane_off + c0, u);
-          tmem_ld_wait();
+          tmem_ld_wait_32x32b_x16(tO(t) + lane_off + c0, u);
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)  // (without a key tile O holds nothing)
+            *reinterpret_cast<float4*>(part + c0 + i) =
+                n_kv ? make_float4(__uint_as_float(u[i]), __uint_as_float(u[i + 1]), __uint_as_float(u[i + 2]),
+                                      __uint_as_float(u[i + 3]))
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      } else {
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays NaN
+        uint16_t* orow = p.o + it.b * p.ob + query * p.os + static_cast<int64_t>(it.kvh * p.group + rh) * p.oh;
+#pragma unroll
+        for (int c0 = 0; c0 < kD; c0 += 16) {
+          uint32_t u[16];
+          tmem_ld_wait_32x32b_x16(tO(t) + lane_off + c0, u);
           if (row_live) {
 #pragma unroll
             for (int q8 = 0; q8 < 2; ++q8) {
               if (c0 + q8 * 8 < p.head_dim) {
                 float f[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = have_o ? __uint_as_float(u[q8 * 8 + i]) * inv : 0.f;
+                for (int i = 0; i < 8; ++i) f[i] = n_kv ? __uint_as_float(u[q8 * 8 + i]) * inv : 0.f;
                 uint4 w;
                 w.x = pack2(f[0], f[1], kBf16);
                 w.y = pack2(f[2], f[3], kBf16);
@@ -420,25 +548,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-    } else {
-      // this CTA's share of the keys: (max, sum) and the partial row, over
-      // the rings once neither tile's MMAs read them
-      asm volatile("bar.sync 1, %0;" ::"n"(kSoftThreads) : "memory");
-      ml[t * kQ + r] = make_float2(m_used, l);
-      float* part = reinterpret_cast<float*>(smem) + (t * kQ + r) * Cf::kPitch;
-      if (t < tiles) {
-#pragma unroll
-        for (int c0 = 0; c0 < kD; c0 += 16) {
-          uint32_t u[16];
-          tmem_ld_32x32b_x16(tO(t) + lane_off + c0, u);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<float4*>(part + c0 + i) =
-                have_o ? make_float4(__uint_as_float(u[i]), __uint_as_float(u[i + 1]), __uint_as_float(u[i + 2]),
-                                     __uint_as_float(u[i + 3]))
-                       : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+      if (n_kv > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_empty[t]);  // the next item's P.V may overwrite O
+        ++nth;
       }
     }
   }
@@ -449,14 +563,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_dealloc(tmem, 512);
   }
   if (prm.splits == 1) return;
-  // The cluster's CTAs sum a share of the rows each, over all of them in rank
-  // order.
+  // The cluster's CTAs sum a share of the item's rows each, over all of them
+  // in rank order.
   cluster_sync();
+  const Item it = item_of(prm, first, split);
   const int chunks = p.head_dim / 8;
   const uint32_t part_s = smem_u32(smem), ml_s = smem_u32(ml);
-  for (int i = threadIdx.x + kThreads * split; i < tiles * kQ * chunks; i += kThreads * prm.splits) {
+  for (int i = threadIdx.x + kThreads * split; i < it.tiles * kQ * chunks; i += kThreads * prm.splits) {
     const int row = i / chunks, c = (i % chunks) * 8;
-    const int t = row / kQ, r = row % kQ, query = q0 + t * prm.qpt + r / p.group;
+    const int t = row / kQ, r = row % kQ, rq = r / p.group, query = it.q0 + t * prm.qpt + rq;
     if (r >= prm.qpt * p.group || query >= p.sq) continue;
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f, m = -INFINITY;
     for (int w = 0; w < prm.splits; ++w) m = fmaxf(m, ld_cluster_f2(mapa_shared(ml_s + row * 8, w)).x);
@@ -477,8 +592,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     w4.y = pack2(o[2] * inv, o[3] * inv, kBf16);
     w4.z = pack2(o[4] * inv, o[5] * inv, kBf16);
     w4.w = pack2(o[6] * inv, o[7] * inv, kBf16);
-    *reinterpret_cast<uint4*>(p.o + b * p.ob + query * p.os +
-                              static_cast<int64_t>(kvh * p.group + r % p.group) * p.oh + c) = w4;
+    *reinterpret_cast<uint4*>(p.o + it.b * p.ob + query * p.os +
+                              static_cast<int64_t>(it.kvh * p.group + r - rq * p.group) * p.oh + c) = w4;
   }
   cluster_sync();  // the others may still read this CTA's partial rows
 }
@@ -572,8 +687,12 @@ int launch_cross_tc(const CrossParams& p, int dtype, cudaStream_t st) {
   prm.tiles = 2;
   prm.splits = 1;
   prm.items_x = static_cast<int>((row_tiles + prm.tiles - 1) / prm.tiles);
-  const int64_t ctas = heads * prm.items_x * prm.splits;
-  if (ctas > 0x7fffffffLL) return kErrShape;
+  if (heads * prm.items_x > 0x3fffffffLL) return kErrShape;
+  prm.n_items = static_cast<int>(heads * prm.items_x);
+  const int key_tiles = (p.sk + kKV - 1) / kKV;
+  static const int persist_tiles = getenv("S3P") ? atoi(getenv("S3P")) : 8;
+  int64_t ctas = static_cast<int64_t>(prm.n_items) * prm.splits;
+  if (prm.splits == 1 && key_tiles <= persist_tiles) ctas = std::min<int64_t>(ctas, num_sms());
   const int box_d = p.head_dim <= 32 ? 32 : 64;
   const CUtensorMapSwizzle swz = box_d == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
   CUtensorMap mq, mk, mv;
