@@ -58,6 +58,17 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// Maximum of 32 values.
+__device__ __forceinline__ float max32(const float* v) {
+  float m[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+  for (int c = 4; c < 28; c += 8) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m[k] = max3(m[k], v[c + 2 * k], v[c + 2 * k + 1]);
+  }
+  return fmaxf(max3(max3(m[0], m[1], m[2]), m[3], v[28]), max3(v[29], v[30], v[31]));
+}
+
 // Maximum of 64 values: four chains of three-input max.
 __device__ __forceinline__ float max64(const float* v) {
   float m[4] = {v[0], v[1], v[2], v[3]};

@@ -14,8 +14,6 @@
 //   warps 1, 3  MMA issue, one for each query tile: with one for both, the tiles
 //               ran in step, both on the exponential units and then both not
 //               (warp 1 also allocates TMEM)
-//   warp 2      with a mask or lengths: key bits of each tile, and zeros over
-//               V rows of keys that do not count (0 * NaN would reach O)
 //   warps 4-7, 8-11   softmax and epilogue of tile 0 and 1; warp w owns TMEM
 //               lanes 32 (w % 4) .. + 31, a thread a whole row of S
 // TMEM (512 columns): S0 S1 (128 each), O0 O1 (D each), and for D <= 64
@@ -62,6 +60,7 @@ struct Cfg {
   // one CTA per SM: each allocates all of TMEM
   static_assert(kSmem > 116 * 1024 && kSmem < 226 * 1024, "one CTA per SM");
   static constexpr bool kOwnP = kD <= 64;                // P beside S
+  static constexpr int kIssuers = kD <= 64 ? 2 : 1;      // MMA warps
   static constexpr uint32_t kOCol = 256, kPCol = 256 + 2 * kD;
   static constexpr int kPitch = kD + 4;                  // floats of a partial row
   static_assert(2 * kQ * kPitch * 4 <= kSmem, "partial rows fit over the rings");
@@ -145,6 +144,26 @@ struct Cursor {
   }
 };
 
+// P = exp2(S sl2 - mb) of kN keys as 16-bit pairs to TMEM from column tp on,
+// added up into l2.
+template <bool kBf16, int kN>
+__device__ __forceinline__ void exp_store(const float (&sv)[kN], float sl2, float mb, uint32_t tp, uint64_t (&l2)[2]) {
+  const uint64_t sc2 = f2pack(sl2, sl2), nmb2 = f2pack(-mb, -mb);
+#pragma unroll
+  for (int c0 = 0; c0 < kN; c0 += 16) {  // 16 keys -> 8 P columns
+    uint32_t pk[8];
+#pragma unroll
+    for (int c = c0; c < c0 + 16; c += 2) {
+      float e0, e1;
+      f2unpack(ffma2(f2pack(sv[c], sv[c + 1]), sc2, nmb2), e0, e1);
+      const float p0 = ex2(e0), p1 = ex2(e1);
+      l2[(c >> 1) & 1] = fadd2(l2[(c >> 1) & 1], f2pack(p0, p1));
+      pk[(c - c0) / 2] = pack2(p0, p1, kBf16);
+    }
+    tmem_st_32x32b_x8(tp + c0 / 2, *reinterpret_cast<const uint32_t(*)[8]>(pk));
+  }
+}
+
 template <bool kBf16, int kD, bool kMask>
 __global__ void __launch_bounds__(kThreads, 1)
     cross_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -152,8 +171,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using Cf = Cfg<kD>;
   constexpr int kStages = Cf::kStages, kTile = Cf::kTile;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ uint64_t bars[16 + 6 * kStages];
-  __shared__ uint32_t bits[kMask ? kStages : 1][4];
+  __shared__ uint64_t bars[16 + 4 * kStages];
   __shared__ float2 ml[2 * kQ];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag_s;
@@ -171,8 +189,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* k_empty = k_full + kStages;
   uint64_t* v_full = k_empty + kStages;
   uint64_t* v_empty = v_full + kStages;
-  uint64_t* v_ready = v_empty + kStages;  // kMask: V of the tile is scrubbed
-  uint64_t* w_ready = v_ready + kStages;  // kMask: the tile's key bits are there
   volatile int* abort_flag = &abort_flag_s;
 
   const CrossParams& p = prm.c;
@@ -196,13 +212,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&p_full[t], 4);
       mbar_init(&p_empty[t], 1);
     }
+    const int users = Cf::kIssuers == 2 ? prm.tiles : 1;  // warps that release K and V
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], prm.tiles);
+      mbar_init(&k_empty[i], users);
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], prm.tiles);
-      mbar_init(&v_ready[i], 1);
-      mbar_init(&w_ready[i], 1);
+      mbar_init(&v_empty[i], users);
     }
     abort_flag_s = aligned ? 0 : 1;
     if (!aligned) atomicCAS(&g_dev_error, 0u, static_cast<unsigned>(kErrTmemAlloc));
@@ -268,35 +283,41 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     }
-  } else if ((warp == 1 || warp == 3) && warp / 2 < prm.tiles && aligned) {
+  } else if (warp >= 1 && warp <= Cf::kIssuers && warp <= prm.tiles && aligned) {
     // ------------------------------------------------------------ MMA
-    const int t = warp / 2;
+    const int t0 = Cf::kIssuers == 2 ? warp - 1 : 0, t1 = Cf::kIssuers == 2 ? warp : 2;  // its query tiles
     const uint32_t fmt = kBf16 ? 1u : 0u;
     const uint32_t idesc_pv = make_idesc(fmt, kQ, kD, 1u);
     auto sdesc_k = [](uint32_t a) { return kD == 32 ? make_sdesc_sw64(a) : make_sdesc_sw128(a); };
     auto sdesc_mn = [](uint32_t a) { return kD == 32 ? make_sdesc_sw64_mn(a) : make_sdesc_sw128_mn(a); };
     constexpr uint32_t kHalfStep = kTile / 2 >> 4;            // the second 64 columns of a D = 128 tile
     constexpr uint32_t kVStep = 16 * Cf::kRowBytes >> 4;      // 16 keys of V
-    const uint64_t qdesc = sdesc_k(smem_u32(sQ + t * kTile));
-    // S = Q K_j^T, once the softmax has read the S before it
-    auto issue_s = [&](const Cursor& c) -> bool {
+    // S_t = Q_t K_j^T, once the softmax has read the S before it
+    auto issue_s = [&](int t, const Cursor& c) -> bool {
       const int st = c.kt % kStages;
-      if (!mbar_wait_warp(&k_full[st], (c.kt / kStages) & 1, kErrTmaWait, abort_flag)) return false;
-      if (t < c.it.tiles) {
-        if (c.j == 0 && !mbar_wait_warp(&q_full[t], c.items(t) & 1, kErrTmaWait, abort_flag)) return false;
-        if (Cf::kOwnP && !mbar_wait_warp(&s_empty[t], (c.turns(t) & 1) ^ 1, kErrAccFree, abort_flag)) return false;
-        tc_fence_after();
-        const uint64_t kdesc = sdesc_k(smem_u32(sK(st)));
-        const uint32_t idesc_s = make_idesc(fmt, kQ, c.keys());
+      if (c.j == 0 && !mbar_wait_warp(&q_full[t], c.items(t) & 1, kErrTmaWait, abort_flag)) return false;
+      if (Cf::kOwnP && !mbar_wait_warp(&s_empty[t], (c.turns(t) & 1) ^ 1, kErrAccFree, abort_flag)) return false;
+      tc_fence_after();
+      const uint64_t qdesc = sdesc_k(smem_u32(sQ + t * kTile)), kdesc = sdesc_k(smem_u32(sK(st)));
+      const uint32_t idesc_s = make_idesc(fmt, kQ, c.keys());
 #pragma unroll
-        for (int kk = 0; kk < kD / 16; ++kk) {  // 16 elements = 32 bytes along D
-          const uint64_t at = (kk / 4) * kHalfStep + 2 * (kk % 4);
-          umma_ss_warp(tS(t), qdesc + at, kdesc + at, idesc_s, kk ? 1u : 0u);
-        }
-        umma_commit_warp(&s_full[t]);
-        if (c.j == c.it.n_kv - 1) umma_commit_warp(&q_empty[t]);
+      for (int kk = 0; kk < kD / 16; ++kk) {  // 16 elements = 32 bytes along D
+        const uint64_t at = (kk / 4) * kHalfStep + 2 * (kk % 4);
+        umma_ss_warp(tS(t), qdesc + at, kdesc + at, idesc_s, kk ? 1u : 0u);
       }
-      umma_commit_warp(&k_empty[st]);  // (an item without this query tile: nothing to wait for)
+      umma_commit_warp(&s_full[t]);
+      if (c.j == c.it.n_kv - 1) umma_commit_warp(&q_empty[t]);
+      return true;
+    };
+    auto wait_k = [&](const Cursor& c) {
+      return mbar_wait_warp(&k_full[c.kt % kStages], (c.kt / kStages) & 1, kErrTmaWait, abort_flag);
+    };
+    // S of all of its query tiles, and K released by it
+    auto issue_all_s = [&](const Cursor& c) -> bool {
+      if (!wait_k(c)) return false;
+      for (int t = t0; t < t1 && t < c.it.tiles; ++t)
+        if (!issue_s(t, c)) return false;
+      umma_commit_warp(&k_empty[c.kt % kStages]);
       return true;
     };
     Cursor s, c;  // of the next S, and of P.V behind it
@@ -304,79 +325,46 @@ __global__ void __launch_bounds__(kThreads, 1)
     c = s;
     bool ok = true;
     if (s.more(prm)) {
-      ok = issue_s(s);
+      ok = issue_all_s(s);
       s.next(prm, step, split);
     }
     for (; ok && c.more(prm); c.next(prm, step, split)) {
       const int st = c.kt % kStages, n = c.keys();
-      if (Cf::kOwnP && s.more(prm)) {  // the next S, beside this tile's softmax
-        ok = issue_s(s);
+      const bool ahead = s.more(prm);
+      if (Cf::kOwnP && ahead) {  // the next S, beside this tile's softmax
+        ok = issue_all_s(s);
         if (!ok) break;
-        s.next(prm, step, split);
       }
       if (!mbar_wait_warp(&v_full[st], (c.kt / kStages) & 1, kErrTmaWait, abort_flag)) break;
-      if (kMask && !mbar_wait_warp(&v_ready[st], (c.kt / kStages) & 1, kErrTmaWait, abort_flag)) break;
-      if (t < c.it.tiles) {
-        // the epilogue of the item before has read O
-        if (c.j == 0 && c.items(t) > 0 &&
-            !mbar_wait_warp(&o_empty[t], (c.items(t) - 1) & 1, kErrAccFree, abort_flag))
-          break;
-        if (!mbar_wait_warp(&p_full[t], c.turns(t) & 1, kErrAccFull, abort_flag)) break;
-        tc_fence_after();
-        const uint64_t vdesc = sdesc_mn(smem_u32(sV(st)));
-        if (n == kKV) {
+      if (!Cf::kOwnP && ahead && !wait_k(s)) break;
+      const uint64_t vdesc = sdesc_mn(smem_u32(sV(st)));
+      for (int t = t0; ok && t < t1; ++t) {
+        if (t < c.it.tiles) {
+          // the epilogue of the item before has read O
+          ok = c.j > 0 || c.items(t) == 0 ||
+               mbar_wait_warp(&o_empty[t], (c.items(t) - 1) & 1, kErrAccFree, abort_flag);
+          ok = ok && mbar_wait_warp(&p_full[t], c.turns(t) & 1, kErrAccFull, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          if (n == kKV) {
 #pragma unroll
-          for (int kk = 0; kk < kKV / 16; ++kk)  // A = P from TMEM: 16 keys = 8 columns
-            umma_ts_warp(tO(t), tP(t) + kk * 8, vdesc + kk * kVStep, idesc_pv, (c.j | kk) ? 1u : 0u);
-        } else {
+            for (int kk = 0; kk < kKV / 16; ++kk)  // A = P from TMEM: 16 keys = 8 columns
+              umma_ts_warp(tO(t), tP(t) + kk * 8, vdesc + kk * kVStep, idesc_pv, (c.j | kk) ? 1u : 0u);
+          } else {
 #pragma unroll 1
-          for (int kk = 0; kk < n / 16; ++kk)
-            umma_ts_warp(tO(t), tP(t) + kk * 8, vdesc + kk * kVStep, idesc_pv, (c.j | kk) ? 1u : 0u);
-        }
-        if (Cf::kOwnP) umma_commit_warp(&p_empty[t]);
-        if (c.j == c.it.n_kv - 1) umma_commit_warp(&o_full[t]);
-      }
-      umma_commit_warp(&v_empty[st]);
-      // P has been consumed in issue order: its S columns may be written
-      if (!Cf::kOwnP && s.more(prm)) {
-        ok = issue_s(s);
-        s.next(prm, step, split);
-      }
-    }
-  } else if (kMask && warp == 2 && aligned) {
-    // ---------------------------------------------- key bits, V scrubbing
-    Cursor c;
-    c.start(prm, first, step, split);
-    for (; c.more(prm); c.next(prm, step, split)) {
-      const uint8_t* mg = p.key_mask ? p.key_mask + c.it.b * p.mask_stride : nullptr;
-      const int st = c.kt % kStages, n = c.keys();
-      // the bits' slot is free with its V stage: both softmaxes are past it
-      if (!mbar_wait_warp(&v_empty[st], ((c.kt / kStages) & 1) ^ 1, kErrStageFree, abort_flag)) break;
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = (c.it.j0 + c.j) * kKV + i * 32 + lane;
-        w[i] = __ballot_sync(0xffffffffu, key < c.it.len && (!mg || mg[key] != 0));
-      }
-      if (lane < 4) bits[kMask ? st : 0][lane] = lane == 0 ? w[0] : lane == 1 ? w[1] : lane == 2 ? w[2] : w[3];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&w_ready[st]);
-      if (!mbar_wait_warp(&v_full[st], (c.kt / kStages) & 1, kErrTmaWait, abort_flag)) break;
-      if ((w[0] & w[1] & w[2] & w[3]) != 0xffffffffu) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (!(w[i] >> lane & 1) && i * 32 + lane < n) {  // (rows past n are not multiplied)
-            uint8_t* row = sV(st) + (i * 32 + lane) * Cf::kRowBytes;
-            for (int h = 0; h < Cf::kHalves; ++h)
-#pragma unroll
-              for (int k = 0; k < Cf::kRowBytes; k += 16)
-                *reinterpret_cast<uint4*>(row + h * (kTile / 2) + k) = make_uint4(0, 0, 0, 0);
+            for (int kk = 0; kk < n / 16; ++kk)
+              umma_ts_warp(tO(t), tP(t) + kk * 8, vdesc + kk * kVStep, idesc_pv, (c.j | kk) ? 1u : 0u);
           }
+          if (Cf::kOwnP) umma_commit_warp(&p_empty[t]);
+          if (c.j == c.it.n_kv - 1) umma_commit_warp(&o_full[t]);
         }
-        fence_proxy_async_smem();
+        // P has been consumed in issue order: its S columns may be written
+        if (!Cf::kOwnP && ahead && t < s.it.tiles) ok = issue_s(t, s);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_ready[st]);
+      if (!ok) break;
+      umma_commit_warp(&v_empty[st]);  // (a warp whose query tile the item has not has nothing to wait for)
+      if (!Cf::kOwnP && ahead) umma_commit_warp(&k_empty[s.kt % kStages]);
+      if (ahead) s.next(prm, step, split);
     }
   } else if (warp >= 4) {
     // ------------------------------------------------ softmax + epilogue
@@ -390,10 +378,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       // What the key loop needs of the item; the epilogue works the rest out
       // again, so that the loop has no registers to spill (S takes 128).
       int n_kv, n;  // key tiles, keys left
+      const uint8_t* mask = nullptr;
       {
         const Item it = item_of(prm, idx, split);
         n_kv = it.n_kv;
         n = it.len - it.j0 * kKV;
+        if (kMask) mask = p.key_mask + it.b * p.mask_stride + it.j0 * kKV;
         if (t >= it.tiles) {
           kt += n_kv;
           if (prm.splits == 1) continue;
@@ -404,44 +394,52 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int j = 0; j < n_kv; ++j, ++kt, ++turn, n -= kKV) {
         const int st = kt % kStages;
-        if (!warp_wait(&s_full[t], turn & 1, kErrAccFull, abort_flag, lane)) { ok = false; break; }
-        tc_fence_after();
-        if (kMask && !warp_wait(&w_ready[st], (kt / kStages) & 1, kErrTmaWait, abort_flag, lane)) { ok = false; break; }
-        // S is read twice, 64 columns at a time: for the maximum, then for the
-        // exponentials.  (Held in registers for both, its 128 values leave too
-        // few: spilled, a load's registers are stored before its data arrives.)
-        auto load_s = [&](int h, float (&sv)[64]) {
-          tmem_ld_wait_32x32b_64(tS(t) + lane_off + h * 64, sv);
-          if (kMask) {
+        // the tile's key bits, by 32 keys
+        uint32_t w[4] = {~0u, ~0u, ~0u, ~0u};
+        if (kMask) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t w = bits[kMask ? st : 0][2 * h + i];
-              if (w != 0xffffffffu) {
-#pragma unroll
-                for (int c = 0; c < 32; ++c)
-                  if (!(w >> c & 1)) sv[i * 32 + c] = -INFINITY;
-              }
-            }
-          } else if (n < (h + 1) * 64) {  // the last tile's keys beyond the states
-#pragma unroll
-            for (int c = 0; c < 64; ++c)
-              if (h * 64 + c >= n) sv[c] = -INFINITY;
-          }
-        };
-        float mt;
-        {
-          float sv[64];
-          load_s(0, sv);
-          mt = max64(sv);
-          if (n > 64) {
-            load_s(1, sv);
-            mt = fmaxf(mt, max64(sv));
+          for (int i = 0; i < 4; ++i) {
+            const int key = i * 32 + lane;
+            w[i] = __ballot_sync(0xffffffffu, key < n && mask[j * kKV + key] != 0);
           }
         }
+        const bool some_off = (w[0] & w[1] & w[2] & w[3]) != ~0u;
+        if (!mbar_wait_warp(&s_full[t], turn & 1, kErrAccFull, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        // Columns c0 .. of S, with -inf where a key does not count.
+        auto masked = [&](float* sv, int c0, int cols) {
+          if (kMask) {
+#pragma unroll
+            for (int i = 0; i < cols / 32; ++i) {
+              if (w[c0 / 32 + i] != 0xffffffffu) {
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                  if (!(w[c0 / 32 + i] >> c & 1)) sv[i * 32 + c] = -INFINITY;
+              }
+            }
+          } else if (n < c0 + cols) {
+#pragma unroll
+            for (int c = 0; c < cols; ++c)
+              if (c0 + c >= n) sv[c] = -INFINITY;
+          }
+        };
+        // A thread keeps 96 of its 128 values from here to the exponentials and
+        // loads the other 32 again for them.  (With all 128 the registers do not
+        // do, and a spilled register of a TMEM load gave wrong values.)
+        float sv[96], mt;
+        {
+          float last[32];
+          tmem_ld_wait_32x32b_32(tS(t) + lane_off + 96, last);
+          masked(last, 96, 32);
+          mt = max32(last);
+        }
+        tmem_ld_wait_32x32b_96(tS(t) + lane_off, sv);
+        masked(sv, 0, 96);
+        mt = fmaxf(mt, fmaxf(max64(sv), max32(sv + 64)));
         const bool need = (mt - m_used) * sl2 > kRescaleLog2;  // false for -inf - -inf
         // P (its own columns) is free, and O at rest, after the P.V before it;
         // with P in S's columns s_full said so already
-        if (Cf::kOwnP && turn > 0 && !warp_wait(&p_empty[t], (turn & 1) ^ 1, kErrAccFull, abort_flag, lane)) {
+        if (Cf::kOwnP && turn > 0 && !mbar_wait_warp(&p_empty[t], (turn & 1) ^ 1, kErrAccFull, abort_flag)) {
           ok = false;
           break;
         }
@@ -465,42 +463,42 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // no key yet: every exponent is -inf against 0
         const float mb = (m_used == -INFINITY ? 0.f : m_used * sl2) - (kBf16 ? 0.f : kF16Shift);
-        const uint64_t sc2 = f2pack(sl2, sl2), nmb2 = f2pack(-mb, -mb);
         uint64_t l2[2] = {f2pack(0.f, 0.f), f2pack(0.f, 0.f)};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (h * 64 < n) {  // (P of keys past the last 16 is not multiplied)
-            float sv[64];
-            load_s(h, sv);
-            if (Cf::kOwnP && (h == 1 || n <= 64)) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&s_empty[t]);  // S may be overwritten
-            }
-#pragma unroll
-            for (int c0 = 0; c0 < 64; c0 += 16) {  // 16 keys -> 8 P columns
-              uint32_t pk[8];
-#pragma unroll
-              for (int c = c0; c < c0 + 16; c += 2) {
-                float e0, e1;
-                f2unpack(ffma2(f2pack(sv[c], sv[c + 1]), sc2, nmb2), e0, e1);
-                const float p0 = ex2(e0), p1 = ex2(e1);
-                l2[(c >> 1) & 1] = fadd2(l2[(c >> 1) & 1], f2pack(p0, p1));
-                pk[(c - c0) / 2] = pack2(p0, p1, kBf16);
-              }
-              tmem_st_32x32b_x8(tP(t) + lane_off + h * 32 + c0 / 2, *reinterpret_cast<const uint32_t(*)[8]>(pk));
-            }
-          }
+        exp_store<kBf16, 96>(sv, sl2, mb, tP(t) + lane_off, l2);
+        if (n > 96) {  // (P of keys past the last 16 is not multiplied)
+          float last[32];
+          tmem_ld_wait_32x32b_32(tS(t) + lane_off + 96, last);
+          masked(last, 96, 32);
+          exp_store<kBf16, 32>(last, sl2, mb, tP(t) + lane_off + 48, l2);
+        }
+        if (Cf::kOwnP) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_empty[t]);  // S may be overwritten
         }
         float a0, a1;
         f2unpack(fadd2(l2[0], l2[1]), a0, a1);
         l += a0 + a1;
         tmem_st_wait();
+        // V rows that P.V reads and that do not count: 0 * NaN would reach O.
+        // (Both query tiles' warps write the same zeros.)
+        const int n16 = min((n + 15) & ~15, kKV);
+        if (kMask ? some_off : n < n16 && p.k_lens != nullptr) {
+          if (!mbar_wait_warp(&v_full[st], (kt / kStages) & 1, kErrTmaWait, abort_flag)) { ok = false; break; }
+          const int v = quarter * 32 + lane;
+          if (v < n16 && (v >= n || (kMask && mask[j * kKV + v] == 0))) {
+            for (int h = 0; h < Cf::kHalves; ++h)
+#pragma unroll
+              for (int k = 0; k < Cf::kRowBytes; k += 16)
+                *reinterpret_cast<uint4*>(sV(st) + h * (kTile / 2) + v * Cf::kRowBytes + k) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
       }
-      if (ok && n_kv > 0) ok = warp_wait(&o_full[t], nth & 1, kErrAccFull, abort_flag, lane);
+      if (ok && n_kv > 0) ok = mbar_wait_warp(&o_full[t], nth & 1, kErrAccFull, abort_flag);
       if (!ok && prm.splits == 1) break;  // (a cluster's CTA still meets its barriers)
       tc_fence_after();
       const Item it = item_of(prm, static_cast<int>(here(static_cast<uint32_t>(idx))), split);
@@ -656,7 +654,7 @@ int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
 template <int kD>
 int launch_typed(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TcParams& prm,
                  int dtype, int64_t ctas, cudaStream_t st) {
-  const bool mask = prm.c.k_lens || prm.c.key_mask;
+  const bool mask = prm.c.key_mask != nullptr;  // (lengths alone need none of it)
   if (dtype == kBF16)
     return mask ? launch_variant<true, kD, true>(mq, mk, mv, prm, ctas, st)
                 : launch_variant<true, kD, false>(mq, mk, mv, prm, ctas, st);
