@@ -7,27 +7,35 @@
 //
 // with the running maximum and sum of each row (rows, heads and keys as in
 // cross_attention.cuh).  One CTA per SM computes two 128-row tiles against the
-// same K and V: while one tile's softmax runs on the exponential units the
-// tensor cores work for the other, and a K / V tile read from L2 serves 256
-// rows.  Twelve warps:
+// same K and V: a K / V tile read from L2 serves 256 rows, and while one tile's
+// softmax runs the tensor cores work for the other.  Twelve warps:
 //   warp 0      TMA: the Q tiles, then K and V through rings of their own
-//   warps 1, 3  MMA issue, one for each query tile: with one for both, the tiles
-//               ran in step, both on the exponential units and then both not
-//               (warp 1 also allocates TMEM)
+//   warp 1      MMA issue, in the order P0.V S0 P1.V S1, which sets the two
+//               tiles half a turn apart (an issuing warp for each tile let them
+//               fall into step: 184 -> 235 us on the case below); allocates TMEM
 //   warps 4-7, 8-11   softmax and epilogue of tile 0 and 1; warp w owns TMEM
 //               lanes 32 (w % 4) .. + 31, a thread a whole row of S
-// TMEM (512 columns): S0 S1 (128 each), O0 O1 (D each), and for D <= 64
-// P0 P1 (64 each), so that S of the next key tile is computed while the
-// softmax of this one runs; for D = 128 P takes the place of its S.
-// O is rescaled lazily, when a row's maximum has grown by more than 2^8.
-// Every mbarrier wait is bounded.
+// TMEM (512 columns): S0 S1 (128 each; P takes the place of its S), O0 O1 (D
+// each).  O is rescaled lazily, when a row's maximum has grown by more than
+// 2^8.  Every mbarrier wait is bounded.
+//
+// What bounds it: a 128 x 128 tile takes 1024 clocks of the exponential units
+// (16 results per clock and SM) and 16 D clocks of the tensor cores, so both at
+// D = 128 and the exponentials below.  Measured: 20/4 heads of 128, 2 x 1729
+// queries, 6001 keys with lengths 184 us, 1008 TFLOP/s (0.61 of the measured
+// GEMM rate); 2 x 16 heads of 64, 5184 queries, 20736 keys 1.47 - 1.57 ms, 560
+// - 597 TFLOP/s, the exponential units 0.53 busy: what is missing is the way
+// from S to P and back (waits, two TMEM loads, the maximum), which two warps on
+// a scheduler do not hide.  Tried without gain: S read twice in 64-column
+// halves, no maximum before the exponentials (made again where a row's P would
+// overflow): 1.59 ms; P beside S with S of the next tile made early: 1.84 ms;
+// one or two of eight exponentials by polynomial: within 4%.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
-#include <cstdlib>
 #include <cstring>
 
 #include "attention_math.cuh"
@@ -46,8 +54,8 @@ constexpr int kQ = 128;        // rows of a tile
 constexpr int kKV = 128;       // keys of a tile
 constexpr int kThreads = 384;
 constexpr float kRescaleLog2 = 8.f;
-// f16 P below 2^-14 loses bits: with a maximum of 2^8 (lazy rescaling) there
-// is room for a factor 2^6 under 65504.  It cancels in O / sum.
+// f16 P below 2^-14 loses bits: with a maximum of 2^9 there is room for a
+// factor 2^6 under 65504.  It cancels in O / sum.
 constexpr float kF16Shift = 6.f;
 
 template <int kD>
@@ -59,22 +67,10 @@ struct Cfg {
   static constexpr int kSmem = 2 * kTile + 2 * kStages * kTile;
   // one CTA per SM: each allocates all of TMEM
   static_assert(kSmem > 116 * 1024 && kSmem < 226 * 1024, "one CTA per SM");
-  static constexpr bool kOwnP = kD <= 64;                // P beside S
-  static constexpr int kIssuers = kD <= 64 ? 2 : 1;      // MMA warps
-  static constexpr uint32_t kOCol = 256, kPCol = 256 + 2 * kD;
+  static constexpr uint32_t kOCol = 256;
   static constexpr int kPitch = kD + 4;                  // floats of a partial row
   static_assert(2 * kQ * kPitch * 4 <= kSmem, "partial rows fit over the rings");
 };
-
-// A value that the compiler may not compute ahead of its place.
-__device__ __forceinline__ uint64_t here(uint64_t v) {
-  asm volatile("" : "+l"(v));
-  return v;
-}
-__device__ __forceinline__ uint32_t here(uint32_t v) {
-  asm volatile("" : "+r"(v));
-  return v;
-}
 
 struct TcParams {
   CrossParams c;
@@ -171,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using Cf = Cfg<kD>;
   constexpr int kStages = Cf::kStages, kTile = Cf::kTile;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ uint64_t bars[16 + 4 * kStages];
+  __shared__ uint64_t bars[12 + 4 * kStages];
   __shared__ float2 ml[2 * kQ];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag_s;
@@ -181,11 +177,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* o_full = &bars[4];
   uint64_t* o_empty = &bars[6];
   uint64_t* s_full = &bars[8];
-  uint64_t* s_empty = &bars[10];
-  uint64_t* p_full = &bars[12];
-  uint64_t* p_empty = &bars[14];
+  uint64_t* p_full = &bars[10];
   // [kStages]
-  uint64_t* k_full = &bars[16];
+  uint64_t* k_full = &bars[12];
   uint64_t* k_empty = k_full + kStages;
   uint64_t* v_full = k_empty + kStages;
   uint64_t* v_empty = v_full + kStages;
@@ -208,16 +202,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&o_full[t], 1);
       mbar_init(&o_empty[t], 4);
       mbar_init(&s_full[t], 1);
-      mbar_init(&s_empty[t], 4);
       mbar_init(&p_full[t], 4);
-      mbar_init(&p_empty[t], 1);
     }
-    const int users = Cf::kIssuers == 2 ? prm.tiles : 1;  // warps that release K and V
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], users);
+      mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], users);
+      mbar_init(&v_empty[i], 1);
     }
     abort_flag_s = aligned ? 0 : 1;
     if (!aligned) atomicCAS(&g_dev_error, 0u, static_cast<unsigned>(kErrTmemAlloc));
@@ -233,7 +224,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tmem_slot;
   auto tS = [&](int t) { return tmem + static_cast<uint32_t>(t * 128); };
   auto tO = [&](int t) { return tmem + Cf::kOCol + static_cast<uint32_t>(t * kD); };
-  auto tP = [&](int t) { return Cf::kOwnP ? tmem + Cf::kPCol + static_cast<uint32_t>(t * 64) : tS(t); };
 
   if (warp == 0 && aligned) {
     // ------------------------------------------------------------ TMA
@@ -283,20 +273,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     }
-  } else if (warp >= 1 && warp <= Cf::kIssuers && warp <= prm.tiles && aligned) {
+  } else if (warp == 1 && aligned) {
     // ------------------------------------------------------------ MMA
-    const int t0 = Cf::kIssuers == 2 ? warp - 1 : 0, t1 = Cf::kIssuers == 2 ? warp : 2;  // its query tiles
     const uint32_t fmt = kBf16 ? 1u : 0u;
     const uint32_t idesc_pv = make_idesc(fmt, kQ, kD, 1u);
     auto sdesc_k = [](uint32_t a) { return kD == 32 ? make_sdesc_sw64(a) : make_sdesc_sw128(a); };
     auto sdesc_mn = [](uint32_t a) { return kD == 32 ? make_sdesc_sw64_mn(a) : make_sdesc_sw128_mn(a); };
     constexpr uint32_t kHalfStep = kTile / 2 >> 4;            // the second 64 columns of a D = 128 tile
     constexpr uint32_t kVStep = 16 * Cf::kRowBytes >> 4;      // 16 keys of V
-    // S_t = Q_t K_j^T, once the softmax has read the S before it
+    // S_t = Q_t K_j^T, over the P (and S) that the MMAs issued before have read
     auto issue_s = [&](int t, const Cursor& c) -> bool {
       const int st = c.kt % kStages;
+      if (t == 0 && !mbar_wait_warp(&k_full[st], (c.kt / kStages) & 1, kErrTmaWait, abort_flag)) return false;
       if (c.j == 0 && !mbar_wait_warp(&q_full[t], c.items(t) & 1, kErrTmaWait, abort_flag)) return false;
-      if (Cf::kOwnP && !mbar_wait_warp(&s_empty[t], (c.turns(t) & 1) ^ 1, kErrAccFree, abort_flag)) return false;
       tc_fence_after();
       const uint64_t qdesc = sdesc_k(smem_u32(sQ + t * kTile)), kdesc = sdesc_k(smem_u32(sK(st)));
       const uint32_t idesc_s = make_idesc(fmt, kQ, c.keys());
@@ -307,17 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       umma_commit_warp(&s_full[t]);
       if (c.j == c.it.n_kv - 1) umma_commit_warp(&q_empty[t]);
-      return true;
-    };
-    auto wait_k = [&](const Cursor& c) {
-      return mbar_wait_warp(&k_full[c.kt % kStages], (c.kt / kStages) & 1, kErrTmaWait, abort_flag);
-    };
-    // S of all of its query tiles, and K released by it
-    auto issue_all_s = [&](const Cursor& c) -> bool {
-      if (!wait_k(c)) return false;
-      for (int t = t0; t < t1 && t < c.it.tiles; ++t)
-        if (!issue_s(t, c)) return false;
-      umma_commit_warp(&k_empty[c.kt % kStages]);
+      if (t == c.it.tiles - 1) umma_commit_warp(&k_empty[st]);
       return true;
     };
     Cursor s, c;  // of the next S, and of P.V behind it
@@ -325,20 +304,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     c = s;
     bool ok = true;
     if (s.more(prm)) {
-      ok = issue_all_s(s);
+      for (int t = 0; ok && t < s.it.tiles; ++t) ok = issue_s(t, s);
       s.next(prm, step, split);
     }
     for (; ok && c.more(prm); c.next(prm, step, split)) {
       const int st = c.kt % kStages, n = c.keys();
       const bool ahead = s.more(prm);
-      if (Cf::kOwnP && ahead) {  // the next S, beside this tile's softmax
-        ok = issue_all_s(s);
-        if (!ok) break;
-      }
       if (!mbar_wait_warp(&v_full[st], (c.kt / kStages) & 1, kErrTmaWait, abort_flag)) break;
-      if (!Cf::kOwnP && ahead && !wait_k(s)) break;
       const uint64_t vdesc = sdesc_mn(smem_u32(sV(st)));
-      for (int t = t0; ok && t < t1; ++t) {
+      for (int t = 0; ok && t < 2; ++t) {
         if (t < c.it.tiles) {
           // the epilogue of the item before has read O
           ok = c.j > 0 || c.items(t) == 0 ||
@@ -349,21 +323,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (n == kKV) {
 #pragma unroll
             for (int kk = 0; kk < kKV / 16; ++kk)  // A = P from TMEM: 16 keys = 8 columns
-              umma_ts_warp(tO(t), tP(t) + kk * 8, vdesc + kk * kVStep, idesc_pv, (c.j | kk) ? 1u : 0u);
+              umma_ts_warp(tO(t), tS(t) + kk * 8, vdesc + kk * kVStep, idesc_pv, (c.j | kk) ? 1u : 0u);
           } else {
 #pragma unroll 1
             for (int kk = 0; kk < n / 16; ++kk)
-              umma_ts_warp(tO(t), tP(t) + kk * 8, vdesc + kk * kVStep, idesc_pv, (c.j | kk) ? 1u : 0u);
+              umma_ts_warp(tO(t), tS(t) + kk * 8, vdesc + kk * kVStep, idesc_pv, (c.j | kk) ? 1u : 0u);
           }
-          if (Cf::kOwnP) umma_commit_warp(&p_empty[t]);
+          if (t == c.it.tiles - 1) umma_commit_warp(&v_empty[st]);
           if (c.j == c.it.n_kv - 1) umma_commit_warp(&o_full[t]);
         }
-        // P has been consumed in issue order: its S columns may be written
-        if (!Cf::kOwnP && ahead && t < s.it.tiles) ok = issue_s(t, s);
+        if (ahead && t < s.it.tiles) ok = issue_s(t, s);
       }
-      if (!ok) break;
-      umma_commit_warp(&v_empty[st]);  // (a warp whose query tile the item has not has nothing to wait for)
-      if (!Cf::kOwnP && ahead) umma_commit_warp(&k_empty[s.kt % kStages]);
       if (ahead) s.next(prm, step, split);
     }
   } else if (warp >= 4) {
@@ -375,8 +345,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = aligned && t < prm.tiles;
     int kt = 0, turn = 0, nth = 0;  // key tiles in the rings, of this query tile, its items
     for (int idx = first; ok && idx < prm.n_items; idx += step) {
-      // What the key loop needs of the item; the epilogue works the rest out
-      // again, so that the loop has no registers to spill (S takes 128).
       int n_kv, n;  // key tiles, keys left
       const uint8_t* mask = nullptr;
       {
@@ -423,9 +391,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (c0 + c >= n) sv[c] = -INFINITY;
           }
         };
-        // A thread keeps 96 of its 128 values from here to the exponentials and
-        // loads the other 32 again for them.  (With all 128 the registers do not
-        // do, and a spilled register of a TMEM load gave wrong values.)
+        // A thread keeps 96 of its 128 values from the maximum to the
+        // exponentials and loads the other 32 again: with all of them the
+        // registers do not do, and spilled ones gave wrong values (they are
+        // targets of asynchronous loads).
         float sv[96], mt;
         {
           float last[32];
@@ -437,19 +406,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         masked(sv, 0, 96);
         mt = fmaxf(mt, fmaxf(max64(sv), max32(sv + 64)));
         const bool need = (mt - m_used) * sl2 > kRescaleLog2;  // false for -inf - -inf
-        // P (its own columns) is free, and O at rest, after the P.V before it;
-        // with P in S's columns s_full said so already
-        if (Cf::kOwnP && turn > 0 && !mbar_wait_warp(&p_empty[t], (turn & 1) ^ 1, kErrAccFull, abort_flag)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
         if (__any_sync(0xffffffffu, need)) {
           const float m_new = fmaxf(m_used, mt);
           const float corr = m_used == -INFINITY ? 0.f : ex2((m_used - m_new) * sl2);
           l *= corr;
           m_used = m_new;
-          if (j > 0) {
+          if (j > 0) {  // (O is at rest: s_full counts the P.V issued before this S)
 #pragma unroll
             for (int c = 0; c < kD / 8; ++c) {
               uint32_t u[8];
@@ -464,17 +426,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         // no key yet: every exponent is -inf against 0
         const float mb = (m_used == -INFINITY ? 0.f : m_used * sl2) - (kBf16 ? 0.f : kF16Shift);
         uint64_t l2[2] = {f2pack(0.f, 0.f), f2pack(0.f, 0.f)};
-        exp_store<kBf16, 96>(sv, sl2, mb, tP(t) + lane_off, l2);
+        exp_store<kBf16, 96>(sv, sl2, mb, tS(t) + lane_off, l2);  // P takes the place of S
         if (n > 96) {  // (P of keys past the last 16 is not multiplied)
           float last[32];
           tmem_ld_wait_32x32b_32(tS(t) + lane_off + 96, last);
           masked(last, 96, 32);
-          exp_store<kBf16, 32>(last, sl2, mb, tP(t) + lane_off + 48, l2);
-        }
-        if (Cf::kOwnP) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_empty[t]);  // S may be overwritten
+          exp_store<kBf16, 32>(last, sl2, mb, tS(t) + lane_off + 48, l2);
         }
         float a0, a1;
         f2unpack(fadd2(l2[0], l2[1]), a0, a1);
@@ -501,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && n_kv > 0) ok = mbar_wait_warp(&o_full[t], nth & 1, kErrAccFull, abort_flag);
       if (!ok && prm.splits == 1) break;  // (a cluster's CTA still meets its barriers)
       tc_fence_after();
-      const Item it = item_of(prm, static_cast<int>(here(static_cast<uint32_t>(idx))), split);
+      const Item it = item_of(prm, idx, split);
       const int rq = r / p.group, rh = r - rq * p.group, query = it.q0 + t * prm.qpt + rq;
       const bool row_live = r < prm.qpt * p.group && query < p.sq;
       if (prm.splits > 1) {
@@ -688,9 +645,12 @@ int launch_cross_tc(const CrossParams& p, int dtype, cudaStream_t st) {
   if (heads * prm.items_x > 0x3fffffffLL) return kErrShape;
   prm.n_items = static_cast<int>(heads * prm.items_x);
   const int key_tiles = (p.sk + kKV - 1) / kKV;
-  static const int persist_tiles = getenv("S3P") ? atoi(getenv("S3P")) : 8;
   int64_t ctas = static_cast<int64_t>(prm.n_items) * prm.splits;
-  if (prm.splits == 1 && key_tiles <= persist_tiles) ctas = std::min<int64_t>(ctas, num_sms());
+  // Short items: one CTA per SM that walks them, so that an item's first loads
+  // and S overlap the epilogue before it (4 x 8 heads x 5184 queries, 77 / 512 /
+  // 2048 keys, D = 64: 29 / 63 / 203 us against 37 / 71 / 208 with a CTA each).
+  // Long ones have a CTA each, dealt out as SMs come free (lengths differ).
+  if (prm.splits == 1 && key_tiles <= 16) ctas = std::min<int64_t>(ctas, num_sms());
   const int box_d = p.head_dim <= 32 ? 32 : 64;
   const CUtensorMapSwizzle swz = box_d == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
   CUtensorMap mq, mk, mv;
