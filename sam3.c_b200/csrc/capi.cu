@@ -157,8 +157,8 @@ const char* sam3cu_strerror(int s) {
 unsigned int sam3cu_last_device_error(void) {
   cudaDeviceSynchronize();
   unsigned int a = dev_error_gemm(), b = dev_error_attn(), c = dev_error_misc(), d = dev_error_attn_tc(),
-               e = dev_error_gemm2(), f = dev_error_cross();
-  return a ? a : (b ? b : (c ? c : (d ? d : (e ? e : f))));
+               e = dev_error_gemm2(), f = dev_error_cross(), g = dev_error_cross_few();
+  return a ? a : (b ? b : (c ? c : (d ? d : (e ? e : (f ? f : g)))));
 }
 
 uint64_t sam3cu_launch_count(int reset) {

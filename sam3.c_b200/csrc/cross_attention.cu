@@ -19,6 +19,7 @@
 // A key that does not count is not read at all: its K and V rows are
 // zero-filled by the copy (so what they hold cannot reach the sums as 0 * NaN)
 // and its score is -inf.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -34,8 +35,11 @@
 #include "cross_attention.cuh"
 #include "sam3cu_internal.h"
 #include "sm100_ptx.cuh"
+#include "tma_host.cuh"
 
 namespace s3 {
+
+S3_DEV_ERROR_ACCESSOR(dev_error_cross_few)
 
 namespace {
 
@@ -86,21 +90,34 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 // kD: head_dim rounded up to 32, 64 or 128 (the copies fill the rest with
-// zeros).  kWM: row warps of the CTA (4 / kWM warps split the keys of a tile).
-template <int kD, int kWM>
-struct Cfg {
-  static constexpr int kRows = 16 * kWM;               // query rows of a CTA
-  static constexpr int kWK = 4 / kWM;                  // key warps
-  static constexpr int kKW = kWM == 4 ? 64 : 32;       // keys of a warp's tile
-  static constexpr int kKT = kKW * kWK;                // keys of the CTA's tile
+// zeros).
+template <int kD>
+struct RowsCfg {
+  static constexpr int kRows = 64;                     // query rows of a CTA, 16 to a warp
+  static constexpr int kKT = 64;                       // keys of a tile
   static constexpr int kChunks = kD / 8;               // 16-byte pieces of a row
   static constexpr int kTileBytes = kKT * kD * 2;      // K or V
   static constexpr int kStages = kD == 32 ? 4 : kD == 64 ? 3 : 2;
   static constexpr int kQBytes = kRows * kD * 2;
-  static constexpr int kOPitch = kD + 4;               // floats of a partial row
-  static constexpr int kPartBytes = kWK * kRows * kOPitch * 4;  // partial O of each key warp (over the ring)
+  static constexpr int kPitch = kD + 4;                // floats of a partial row
+  static constexpr int kPartBytes = kRows * kPitch * 4;  // over the ring
   static constexpr int kRing = 2 * kStages * kTileBytes;
   static constexpr int kSmem = kQBytes + (kRing > kPartBytes ? kRing : kPartBytes);
+};
+template <int kD>
+struct FewCfg {
+  static constexpr int kRows = 16;                     // query rows of a CTA
+  static constexpr int kWarps = 4;                     // each 32 keys of a tile
+  static constexpr int kThreads = 32 * (kWarps + 1);   // and one that loads
+  static constexpr int kKT = 32 * kWarps;
+  static constexpr int kTileBytes = kKT * kD * 2;
+  static constexpr int kStages = kD == 32 ? 4 : 3;
+  static constexpr int kQBytes = kRows * kD * 2;
+  static constexpr int kPitch = kD + 4;
+  static constexpr int kPartBytes = kWarps * kRows * kPitch * 4;  // over the ring
+  static constexpr int kRing = 2 * kStages * kTileBytes;
+  static_assert(kPartBytes <= kRing, "partial rows fit over the ring");
+  static constexpr int kSmem = kRing + kQBytes;
 };
 
 // Byte offset of 16-byte piece c of row r in a tile of kChunks pieces a row,
@@ -159,18 +176,100 @@ struct RowState {
   }
 };
 
-template <bool kBf16, int kD, int kWM, bool kBias>
-__global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_constant__ CrossParams p, int row_tiles,
+// The end of a kernel whose threads left, for kRows rows and each of kWK key
+// warps, (max, sum) in ml [kWK][kRows] and the unscaled partial O in part
+// [kWK][kRows][kD + 4]: adds the warps' rows up, and with splits > 1 those of
+// the cluster's CTAs (each sums a share of the rows over all of them, in rank
+// order), and writes the output.  wgt: [kWK][kRows], kWK > 1 only.
+template <bool kBf16, int kD, int kRows, int kWK, int kN>
+__device__ __forceinline__ void join_rows(const CrossParams& p, float* part, float2* ml, float* wgt, int row0, int b,
+                                          int kvh, int split, int splits, float to_log2) {
+  constexpr int kPitch = kD + 4;
+  const int tid = threadIdx.x;
+  __syncthreads();
+  if constexpr (kWK > 1) {
+    // the weight of each warp's partial row against the row's maximum
+    if (tid < kRows) {
+      float m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWK; ++w) m = fmaxf(m, ml[w * kRows + tid].x);
+      const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int w = 0; w < kWK; ++w) {
+        const float f = ex2((ml[w * kRows + tid].x - base) * to_log2);
+        wgt[w * kRows + tid] = f;
+        l = fmaf(f, ml[w * kRows + tid].y, l);
+      }
+      ml[tid] = make_float2(m, l);
+    }
+    __syncthreads();
+    // one partial tile per CTA
+    for (int i = tid; i < kRows * kD / 4; i += kN) {
+      const int r = i / (kD / 4), c = (i % (kD / 4)) * 4;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWK; ++w) {
+        const float f = wgt[w * kRows + r];
+        const float4 x = *reinterpret_cast<const float4*>(part + (w * kRows + r) * kPitch + c);
+        a.x = fmaf(f, x.x, a.x);
+        a.y = fmaf(f, x.y, a.y);
+        a.z = fmaf(f, x.z, a.z);
+        a.w = fmaf(f, x.w, a.w);
+      }
+      *reinterpret_cast<float4*>(part + r * kPitch + c) = a;
+    }
+  }
+  if (splits > 1) cluster_sync();
+  else if (kWK > 1) __syncthreads();
+  // Rows to the output, 8 elements a thread.
+  const int out_chunks = p.head_dim / 8;
+  const uint32_t part_s = smem_u32(part), ml_s = smem_u32(ml);
+  for (int i = tid + kN * split; i < kRows * out_chunks; i += kN * splits) {
+    const int r = i / out_chunks, c = (i % out_chunks) * 8;
+    if (row0 + r >= p.rows) break;
+    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f;
+    if (splits > 1) {
+      float m = -INFINITY;
+      for (int w = 0; w < splits; ++w) m = fmaxf(m, ld_cluster_f2(mapa_shared(ml_s + r * 8, w)).x);
+      const float base = m == -INFINITY ? 0.f : m;
+      for (int w = 0; w < splits; ++w) {
+        const float2 s = ld_cluster_f2(mapa_shared(ml_s + r * 8, w));
+        const float f = ex2((s.x - base) * to_log2);
+        l = fmaf(f, s.y, l);
+        const uint32_t src = mapa_shared(part_s + (r * kPitch + c) * 4, w);
+        const float4 x = ld_cluster_f4(src), y = ld_cluster_f4(src + 16);
+        const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = fmaf(f, v[e], o[e]);
+      }
+    } else {
+      l = ml[r].y;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = part[r * kPitch + c + e];
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays NaN
+    const int row = row0 + r, q = row / p.group;
+    uint4 w4;
+    w4.x = pack2<kBf16>(o[0] * inv, o[1] * inv);
+    w4.y = pack2<kBf16>(o[2] * inv, o[3] * inv);
+    w4.z = pack2<kBf16>(o[4] * inv, o[5] * inv);
+    w4.w = pack2<kBf16>(o[6] * inv, o[7] * inv);
+    *reinterpret_cast<uint4*>(p.o + b * p.ob + q * p.os + static_cast<int64_t>(kvh * p.group + row - q * p.group) * p.oh +
+                              c) = w4;
+  }
+  if (splits > 1) cluster_sync();  // the others may still read this CTA's partial rows
+}
+
+template <bool kBf16, int kD, bool kBias>
+__global__ void __launch_bounds__(kThreads) cross_rows_kernel(const __grid_constant__ CrossParams p, int row_tiles,
                                                              int splits) {
-  using Cf = Cfg<kD, kWM>;
-  constexpr int kKW = Cf::kKW, kKT = Cf::kKT, kWK = Cf::kWK, kCh = Cf::kChunks, kStages = Cf::kStages;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float2 ml[kWK][Cf::kRows];  // (max, sum) of each row, by key warp; [0] then holds the CTA's
-  __shared__ float wgt[kWK][Cf::kRows];
+  using Cf = RowsCfg<kD>;
+  constexpr int kKT = Cf::kKT, kCh = Cf::kChunks, kStages = Cf::kStages;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ float2 ml[Cf::kRows];  // (max, sum) of each row
   const uint32_t sq = smem_u32(smem), ring = sq + Cf::kQBytes;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int wm = kWM == 4 ? warp : 0, wk = kWM == 4 ? 0 : warp;
   const int split = blockIdx.x % splits, item = blockIdx.x / splits;
   const int rt = item % row_tiles, bh = item / row_tiles;
   const int kvh = bh % p.kv_heads, b = bh / p.kv_heads;
@@ -194,15 +293,13 @@ __global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_consta
   }
   cp_async_commit();
 
-  // Tile t into its ring slot: by the whole CTA, or by each key warp its own
-  // keys (then only that warp waits for them).
+  // Tile t into its ring slot.
   auto load = [&](int t) {
     const uint32_t sk = ring + (t % kStages) * 2 * Cf::kTileBytes, sv = sk + Cf::kTileBytes;
-    constexpr int kCopies = kKW * kCh / (kWM == 4 ? kThreads : 32);
 #pragma unroll 4
-    for (int i = 0; i < kCopies; ++i) {
-      const int idx = (kWM == 4 ? tid : lane) + i * (kWM == 4 ? kThreads : 32);
-      const int r = wk * kKW + idx / kCh, c = idx % kCh;
+    for (int i = 0; i < kKT * kCh / kThreads; ++i) {
+      const int idx = tid + i * kThreads;
+      const int r = idx / kCh, c = idx % kCh;
       const int key = t * kKT + r;
       bool ok = key < len && c * 8 < p.head_dim;
       if (mg && ok) ok = mg[key] != 0;
@@ -228,7 +325,7 @@ __global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_consta
   if (kBias) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = min(row0 + wm * 16 + (lane >> 2) + 8 * h, p.rows - 1);
+      const int r = min(row0 + warp * 16 + (lane >> 2) + 8 * h, p.rows - 1);
       brow[h] = p.bias + b * p.bb + static_cast<int64_t>(kvh * p.group + r % p.group) * p.bh + (r / p.group) * p.bs;
     }
   }
@@ -237,24 +334,22 @@ __global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_consta
   __syncthreads();
 #pragma unroll
   for (int kk = 0; kk < kD / 16; ++kk) {
-    const int r = wm * 16 + (lane & 15);
+    const int r = warp * 16 + (lane & 15);
     ldsm_x4(sq + tile_at<kCh>(r, kk * 2 + (lane >> 4)), qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3]);
   }
 
   for (int t = t0; t < t1; ++t) {
     cp_async_wait<kStages - 2>();
-    if (kWM == 4) __syncthreads();
-    else __syncwarp();
+    __syncthreads();
     if (t + kStages - 1 < t1) load(t + kStages - 1);  // into the slot of tile t - 1, which all have left
     cp_async_commit();
     const uint32_t sk = ring + (t % kStages) * 2 * Cf::kTileBytes, sv = sk + Cf::kTileBytes;
-    const int key0 = t * kKT + wk * kKW;
-    if (key0 >= len) continue;
+    const int key0 = t * kKT;
 
-    float bias[kBias ? kKW / 8 : 1][4];
+    float bias[kBias ? kKT / 8 : 1][4];
     if (kBias) {
 #pragma unroll
-      for (int j = 0; j < kKW / 8; ++j) {
+      for (int j = 0; j < kKT / 8; ++j) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int key = key0 + j * 8 + (lane & 3) * 2 + (e & 1);
@@ -262,14 +357,14 @@ __global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_consta
         }
       }
     }
-    float s[kKW / 8][4];
+    float s[kKT / 8][4];
 #pragma unroll
-    for (int j = 0; j < kKW / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+    for (int j = 0; j < kKT / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < kD / 16; ++kk) {
 #pragma unroll
-      for (int jp = 0; jp < kKW / 16; ++jp) {  // pairs of 8-key blocks
-        const int r = wk * kKW + jp * 16 + (lane & 7) + (lane >> 4) * 8;
+      for (int jp = 0; jp < kKT / 16; ++jp) {  // pairs of 8-key blocks
+        const int r = jp * 16 + (lane & 7) + (lane >> 4) * 8;
         uint32_t b0, b1, b2, b3;
         ldsm_x4(sk + tile_at<kCh>(r, kk * 2 + ((lane >> 3) & 1)), b0, b1, b2, b3);
         mma16816<kBf16>(s[2 * jp], qf[kk], b0, b1);
@@ -278,13 +373,13 @@ __global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_consta
     }
     if (kBias) {
 #pragma unroll
-      for (int j = 0; j < kKW / 8; ++j)
+      for (int j = 0; j < kKT / 8; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[j][e] = fmaf(s[j][e], p.scale, bias[kBias ? j : 0][e]);
     }
-    if (mg || key0 + kKW > len) {
+    if (mg || key0 + kKT > len) {
 #pragma unroll
-      for (int j = 0; j < kKW / 8; ++j) {
+      for (int j = 0; j < kKT / 8; ++j) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int key = key0 + j * 8 + (lane & 3) * 2 + e;
@@ -292,10 +387,10 @@ __global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_consta
         }
       }
     }
-    st.template softmax<kKW>(s, to_log2, kBf16);
+    st.template softmax<kKT>(s, to_log2, kBf16);
     // O += P V, P rounded to the operands' type
 #pragma unroll
-    for (int kk = 0; kk < kKW / 16; ++kk) {
+    for (int kk = 0; kk < kKT / 16; ++kk) {
       uint32_t pa[4];
       pa[0] = pack2<kBf16>(s[2 * kk][0], s[2 * kk][1]);
       pa[1] = pack2<kBf16>(s[2 * kk][2], s[2 * kk][3]);
@@ -303,7 +398,7 @@ __global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_consta
       pa[3] = pack2<kBf16>(s[2 * kk + 1][2], s[2 * kk + 1][3]);
 #pragma unroll
       for (int jp = 0; jp < kD / 16; ++jp) {  // pairs of 8-wide column blocks
-        const int r = wk * kKW + kk * 16 + (lane & 15);
+        const int r = kk * 16 + (lane & 15);
         uint32_t b0, b1, b2, b3;
         ldsm_x4_t(sv + tile_at<kCh>(r, jp * 2 + (lane >> 4)), b0, b1, b2, b3);
         mma16816<kBf16>(st.acc[2 * jp], pa, b0, b1);
@@ -317,104 +412,209 @@ __global__ void __launch_bounds__(kThreads) cross_mma_kernel(const __grid_consta
   cp_async_wait<0>();
   __syncthreads();
   float* part = reinterpret_cast<float*>(smem + Cf::kQBytes);
-  const int r_lo = wm * 16 + (lane >> 2);
+  const int r_lo = warp * 16 + (lane >> 2);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float l = st.l[h];
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if ((lane & 3) == 0) ml[wk][r_lo + 8 * h] = make_float2(st.m[h], l);
-    float* dst = part + (wk * Cf::kRows + r_lo + 8 * h) * Cf::kOPitch + (lane & 3) * 2;
+    if ((lane & 3) == 0) ml[r_lo + 8 * h] = make_float2(st.m[h], l);
+    float* dst = part + (r_lo + 8 * h) * Cf::kPitch + (lane & 3) * 2;
 #pragma unroll
     for (int j = 0; j < kD / 8; ++j)
       *reinterpret_cast<float2*>(dst + j * 8) = make_float2(st.acc[j][2 * h], st.acc[j][2 * h + 1]);
   }
+  join_rows<kBf16, kD, Cf::kRows, 1, kThreads>(p, part, ml, nullptr, row0, b, kvh, split, splits, to_log2);
+}
+
+// Up to 16 rows of a key head: K and V are read once and little is done with
+// them, so what counts is that loads never pause.  One warp fetches 128-key
+// tiles by TMA into a ring; four compute, each on 32 keys of every tile with a
+// running maximum of its own, and are added up at the end.
+template <bool kBf16, int kD, bool kBias>
+__global__ void __launch_bounds__(FewCfg<kD>::kThreads)
+    cross_few_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                     const __grid_constant__ CrossParams p, const KvShare share, int row_tiles, int splits) {
+  using Cf = FewCfg<kD>;
+  constexpr int kCh = kD / 8, kStages = Cf::kStages, kTile = Cf::kTileBytes, kHalves = kD == 128 ? 2 : 1;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ uint64_t bars[2 * kStages];
+  __shared__ float2 ml[Cf::kWarps * Cf::kRows];
+  __shared__ float wgt[Cf::kWarps * Cf::kRows];
+  __shared__ int abort_flag_s;
+  uint64_t* full = bars;
+  uint64_t* empty = bars + kStages;
+  volatile int* abort_flag = &abort_flag_s;
+  const uint32_t ring = smem_u32(smem), sq = ring + Cf::kRing;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int split = blockIdx.x % splits, item = blockIdx.x / splits;
+  const int rt = item % row_tiles, bh = item / row_tiles;
+  const int kvh = bh % p.kv_heads, b = bh / p.kv_heads;
+  const int row0 = rt * Cf::kRows;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], Cf::kWarps);
+    }
+    const bool aligned = (ring & 1023u) == 0;  // the swizzled layouts need it
+    abort_flag_s = aligned ? 0 : 1;
+    if (!aligned) atomicCAS(&g_dev_error, 0u, static_cast<unsigned>(kErrTmaWait));
+    fence_barrier_init();
+  }
+  const int len = cross_len(p, b);
+  const int n_tiles = (len + Cf::kKT - 1) / Cf::kKT;
+  const int t0 = static_cast<int>(static_cast<int64_t>(n_tiles) * split / splits);
+  const int t1 = static_cast<int>(static_cast<int64_t>(n_tiles) * (split + 1) / splits);
   __syncthreads();
-  // The weight of each key warp's partial row against the row's maximum over
-  // this CTA, and over the cluster.
-  if (kWK > 1 || splits > 1) {
-    if (tid < Cf::kRows) {
-      float m = -INFINITY, l = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWK; ++w) m = fmaxf(m, ml[w][tid].x);
-      const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int w = 0; w < kWK; ++w) {
-        const float f = ex2((ml[w][tid].x - base) * to_log2);
-        wgt[w][tid] = f;
-        l = fmaf(f, ml[w][tid].y, l);
+  const bool run = *abort_flag == 0;
+  // with a bias the scores are in natural units (its lowest finite values
+  // would overflow in base 2), without one they stay unscaled dot products
+  const float to_log2 = kBias ? kLog2e : p.scale_log2;
+
+  if (warp == Cf::kWarps) {
+    for (int t = t0; run && t < t1; ++t) {
+      const int st = (t - t0) % kStages;
+      if (!mbar_wait_warp(&empty[st], (((t - t0) / kStages) & 1) ^ 1, kErrStageFree, abort_flag)) break;
+      if (elect_one()) {
+        uint8_t* dst = smem + st * 2 * kTile;
+        mbar_arrive_expect_tx(&full[st], 2 * kTile);
+        for (int h = 0; h < kHalves; ++h) {
+          tma_load_4d(dst + h * (kTile / 2), &tk, &full[st], h * 64, t * Cf::kKT, kvh * share.kh, b * share.kb);
+          tma_load_4d(dst + kTile + h * (kTile / 2), &tv, &full[st], h * 64, t * Cf::kKT, kvh * share.vh, b * share.vb);
+        }
       }
-      ml[0][tid] = make_float2(m, l);
+      __syncwarp();
     }
-    if (kWK == 1) cluster_sync();
-    else __syncthreads();
-  }
-  if (kWK > 1 && splits > 1) {
-    // one partial tile per CTA for the others to read
-    for (int i = tid; i < Cf::kRows * kD / 4; i += kThreads) {
-      const int r = i / (kD / 4), c = (i % (kD / 4)) * 4;
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kWK; ++w) {
-        const float f = wgt[w][r];
-        const float4 x = *reinterpret_cast<const float4*>(part + (w * Cf::kRows + r) * Cf::kOPitch + c);
-        a.x = fmaf(f, x.x, a.x);
-        a.y = fmaf(f, x.y, a.y);
-        a.z = fmaf(f, x.z, a.z);
-        a.w = fmaf(f, x.w, a.w);
-      }
-      *reinterpret_cast<float4*>(part + r * Cf::kOPitch + c) = a;
+  } else {
+    // byte offset of piece c of row r in a tile as the copies lay it: for
+    // D = 128 two halves of 128-byte rows
+    auto at = [](int r, int c) {
+      return kD == 128 ? (c >> 3) * (kTile / 2) + tile_at<8>(r, c & 7) : tile_at<kD == 128 ? 8 : kCh>(r, c);
+    };
+    // the queries, by this warp alone: each warp writes the same values
+    for (int i = lane; i < Cf::kRows * kCh; i += 32) {
+      const int r = i / kCh, c = i % kCh, row = row0 + r;
+      const bool ok = row < p.rows && c * 8 < p.head_dim;
+      const int q = ok ? row / p.group : 0, h = ok ? row - q * p.group : 0;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (ok) w = *reinterpret_cast<const uint4*>(p.q + b * p.qb + q * p.qs + (kvh * p.group + h) * p.qh + c * 8);
+      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(sq + tile_at<kCh>(r, c)), "r"(w.x), "r"(w.y),
+                   "r"(w.z), "r"(w.w)
+                   : "memory");
     }
-    cluster_sync();
-  }
-  // Rows to the output, 8 elements a thread; with a cluster each CTA sums a
-  // share of them over all CTAs, in rank order.
-  const int out_chunks = p.head_dim / 8;
-  const uint32_t part_s = smem_u32(part), ml_s = smem_u32(&ml[0][0]);
-  for (int i = tid + kThreads * split; i < Cf::kRows * out_chunks; i += kThreads * splits) {
-    const int r = i / out_chunks, c = (i % out_chunks) * 8;
-    if (row0 + r >= p.rows) break;
-    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f;
-    if (splits > 1) {
-      float m = -INFINITY;
-      for (int w = 0; w < splits; ++w) m = fmaxf(m, ld_cluster_f2(mapa_shared(ml_s + r * 8, w)).x);
-      const float base = m == -INFINITY ? 0.f : m;
-      for (int w = 0; w < splits; ++w) {
-        const float2 s = ld_cluster_f2(mapa_shared(ml_s + r * 8, w));
-        const float f = ex2((s.x - base) * to_log2);
-        l = fmaf(f, s.y, l);
-        const uint32_t src = mapa_shared(part_s + (r * Cf::kOPitch + c) * 4, w);
-        const float4 x = ld_cluster_f4(src), y = ld_cluster_f4(src + 16);
-        o[0] = fmaf(f, x.x, o[0]);
-        o[1] = fmaf(f, x.y, o[1]);
-        o[2] = fmaf(f, x.z, o[2]);
-        o[3] = fmaf(f, x.w, o[3]);
-        o[4] = fmaf(f, y.x, o[4]);
-        o[5] = fmaf(f, y.y, o[5]);
-        o[6] = fmaf(f, y.z, o[6]);
-        o[7] = fmaf(f, y.w, o[7]);
-      }
-    } else {
-      l = ml[0][r].y;
+    __syncwarp();
+    uint32_t qf[kD / 16][4];
 #pragma unroll
-      for (int w = 0; w < kWK; ++w) {
-        const float f = kWK > 1 ? wgt[w][r] : 1.f;
-        const float* src = part + (w * Cf::kRows + r) * Cf::kOPitch + c;
+    for (int kk = 0; kk < kD / 16; ++kk)
+      ldsm_x4(sq + tile_at<kCh>(lane & 15, kk * 2 + (lane >> 4)), qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3]);
+    const uint8_t* mg = p.key_mask ? p.key_mask + b * p.mask_stride : nullptr;
+    const float* brow[2] = {nullptr, nullptr};
+    if (kBias) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = fmaf(f, src[e], o[e]);
+      for (int h = 0; h < 2; ++h) {
+        const int r = min(row0 + (lane >> 2) + 8 * h, p.rows - 1);
+        brow[h] = p.bias + b * p.bb + (kvh * p.group + r % p.group) * p.bh + (r / p.group) * p.bs;
       }
     }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays NaN
-    const int row = row0 + r;
-    uint4 w4;
-    w4.x = pack2<kBf16>(o[0] * inv, o[1] * inv);
-    w4.y = pack2<kBf16>(o[2] * inv, o[3] * inv);
-    w4.z = pack2<kBf16>(o[4] * inv, o[5] * inv);
-    w4.w = pack2<kBf16>(o[6] * inv, o[7] * inv);
-    *reinterpret_cast<uint4*>(p.o + b * p.ob + (row / p.group) * p.os +
-                              static_cast<int64_t>(kvh * p.group + row % p.group) * p.oh + c) = w4;
+    RowState<kD> rs;
+    rs.clear();
+    for (int t = t0; run && t < t1; ++t) {
+      const int st = (t - t0) % kStages;
+      const int key0 = t * Cf::kKT + warp * 32;
+      const uint32_t on = __ballot_sync(0xffffffffu, key0 + lane < len && (!mg || mg[key0 + lane] != 0));
+      float bias[kBias ? 4 : 1][4];
+      if (kBias) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + j * 8 + (lane & 3) * 2 + (e & 1);
+            bias[kBias ? j : 0][e] = key < len ? __ldg(brow[e >> 1] + key) : 0.f;
+          }
+        }
+      }
+      if (!mbar_wait_warp(&full[st], ((t - t0) / kStages) & 1, kErrTmaWait, abort_flag)) break;
+      const uint32_t sk = ring + st * 2 * kTile, sv = sk + kTile;
+      if (on != 0) {
+        if (on != 0xffffffffu) {
+          // V of keys that do not count: 0 * NaN would reach the sums
+          if (!(on >> lane & 1)) {
+#pragma unroll
+            for (int c = 0; c < kCh; ++c)
+              asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(sv + at(warp * 32 + lane, c)), "r"(0)
+                           : "memory");
+          }
+          __syncwarp();
+        }
+        float s[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < kD / 16; ++kk) {
+#pragma unroll
+          for (int jp = 0; jp < 2; ++jp) {  // pairs of 8-key blocks
+            const int r = warp * 32 + jp * 16 + (lane & 7) + (lane >> 4) * 8;
+            uint32_t b0, b1, b2, b3;
+            ldsm_x4(sk + at(r, kk * 2 + ((lane >> 3) & 1)), b0, b1, b2, b3);
+            mma16816<kBf16>(s[2 * jp], qf[kk], b0, b1);
+            mma16816<kBf16>(s[2 * jp + 1], qf[kk], b2, b3);
+          }
+        }
+        if (kBias) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][e] = fmaf(s[j][e], p.scale, bias[kBias ? j : 0][e]);
+        }
+        if (on != 0xffffffffu) {
+          const uint32_t mine = on >> ((lane & 3) * 2);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (!(mine >> (j * 8) & 1)) s[j][0] = s[j][2] = -INFINITY;
+            if (!(mine >> (j * 8 + 1) & 1)) s[j][1] = s[j][3] = -INFINITY;
+          }
+        }
+        rs.template softmax<32>(s, to_log2, kBf16);
+        // O += P V, P rounded to the operands' type
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          uint32_t pa[4];
+          pa[0] = pack2<kBf16>(s[2 * kk][0], s[2 * kk][1]);
+          pa[1] = pack2<kBf16>(s[2 * kk][2], s[2 * kk][3]);
+          pa[2] = pack2<kBf16>(s[2 * kk + 1][0], s[2 * kk + 1][1]);
+          pa[3] = pack2<kBf16>(s[2 * kk + 1][2], s[2 * kk + 1][3]);
+#pragma unroll
+          for (int jp = 0; jp < kD / 16; ++jp) {  // pairs of 8-wide column blocks
+            const int r = warp * 32 + kk * 16 + (lane & 15);
+            uint32_t b0, b1, b2, b3;
+            ldsm_x4_t(sv + at(r, jp * 2 + (lane >> 4)), b0, b1, b2, b3);
+            mma16816<kBf16>(rs.acc[2 * jp], pa, b0, b1);
+            mma16816<kBf16>(rs.acc[2 * jp + 1], pa, b2, b3);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+    // (the ring is read by others until here, and filled no more)
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * Cf::kWarps) : "memory");
+    float* part = reinterpret_cast<float*>(smem) + warp * Cf::kRows * Cf::kPitch;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float l = rs.l[h];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      const int r = (lane >> 2) + 8 * h;
+      if ((lane & 3) == 0) ml[warp * Cf::kRows + r] = make_float2(rs.m[h], l);
+      float* dst = part + r * Cf::kPitch + (lane & 3) * 2;
+#pragma unroll
+      for (int j = 0; j < kD / 8; ++j)
+        *reinterpret_cast<float2*>(dst + j * 8) = make_float2(rs.acc[j][2 * h], rs.acc[j][2 * h + 1]);
+    }
   }
-  if (splits > 1) cluster_sync();  // the others may still read this CTA's partial rows
+  join_rows<kBf16, kD, Cf::kRows, Cf::kWarps, Cf::kThreads>(p, reinterpret_cast<float*>(smem), ml, wgt, row0, b, kvh,
+                                                            split, splits, to_log2);
 }
 
 // Few keys, many rows: the CTA keeps K and V of its key head in shared memory
@@ -432,7 +632,7 @@ template <bool kBf16, int kD, bool kBias>
 __global__ void __launch_bounds__(kThreads) cross_keep_kernel(const __grid_constant__ CrossParams p, int chunks) {
   using Cf = KeepCfg<kD>;
   constexpr int kCh = Cf::kChunks, kKW = 64, kWarps = kThreads / 32;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint32_t on[kMaxKeep / 32];  // bit per key that counts
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kp = (p.sk + 15) & ~15;
@@ -593,29 +793,37 @@ __global__ void __launch_bounds__(kThreads) cross_keep_kernel(const __grid_const
   }
 }
 
-template <bool kBf16, int kD, int kWM, bool kBias>
-int launch_variant(const CrossParams& p, cudaStream_t st) {
-  using Cf = Cfg<kD, kWM>;
-  const auto kernel = cross_mma_kernel<kBf16, kD, kWM, kBias>;
-  static std::atomic<uint64_t> ready{0};  // devices whose attributes are set
+// Sets a kernel's shared memory limit, once per device.
+int allow_smem(const void* kernel, int bytes, bool wide_cluster, std::atomic<uint64_t>& ready) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return kErrCuda;
   if (dev >= 64 || !(ready.load() >> dev & 1)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::kSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
+        (wide_cluster &&
+         cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess))
       return kErrCuda;
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
-  const int64_t row_tiles = (static_cast<int64_t>(p.rows) + Cf::kRows - 1) / Cf::kRows;
-  const int64_t items = row_tiles * p.kv_heads * p.batch;
-  const int key_tiles = (p.sk + Cf::kKT - 1) / Cf::kKT;
-  int splits = 1;
-  while (splits < 8 && items * splits * 2 <= 2 * num_sms() && key_tiles >= 2 * splits) splits *= 2;
+  return kOk;
+}
+
+// CTAs that share an item's keys: a power of two up to `most`, while there
+// are SMs for them (per_sm CTAs each) and two key tiles for every one.
+int key_splits(int64_t items, int key_tiles, int per_sm, int most) {
+  int n = 1;
+  while (n < most && items * n * 2 <= static_cast<int64_t>(per_sm) * num_sms() && key_tiles >= 4 * n) n *= 2;
+  return n;
+}
+
+template <class... A>
+int launch_split(void (*kernel)(A...), int64_t items, int splits, int threads, int smem, cudaStream_t st,
+                 const A&... args) {
   if (items * splits > 0x7fffffffLL) return kErrShape;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(static_cast<unsigned>(items * splits));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Cf::kSmem;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   if (splits > 1) {
@@ -626,20 +834,41 @@ int launch_variant(const CrossParams& p, cudaStream_t st) {
     cfg.numAttrs = 1;
   }
   count_launches(1);
-  return cudaLaunchKernelEx(&cfg, kernel, p, static_cast<int>(row_tiles), splits) == cudaSuccess ? kOk : kErrLaunch;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? kOk : kErrLaunch;
+}
+
+template <bool kBf16, int kD, bool kBias>
+int launch_few(const CrossParams& p, cudaStream_t st) {
+  using Cf = FewCfg<kD>;
+  static std::atomic<uint64_t> ready{0};
+  const auto kernel = cross_few_kernel<kBf16, kD, kBias>;
+  if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), Cf::kSmem, true, ready)) return rc;
+  CUtensorMap mk, mv;
+  KvShare share;
+  if (!make_kv_maps(p, kBf16 ? kBF16 : kF16, Cf::kKT, &mk, &mv, &share)) return kErrTma;
+  const int row_tiles = (p.rows + Cf::kRows - 1) / Cf::kRows;
+  const int64_t items = static_cast<int64_t>(row_tiles) * p.kv_heads * p.batch;
+  const int splits = key_splits(items, (p.sk + Cf::kKT - 1) / Cf::kKT, 200 * 1024 / Cf::kSmem, 16);
+  return launch_split(kernel, items, splits, Cf::kThreads, Cf::kSmem, st, mk, mv, p, share, row_tiles, splits);
+}
+
+template <bool kBf16, int kD, bool kBias>
+int launch_rows_any(const CrossParams& p, cudaStream_t st) {
+  using Cf = RowsCfg<kD>;
+  static std::atomic<uint64_t> ready{0};
+  const auto kernel = cross_rows_kernel<kBf16, kD, kBias>;
+  if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), Cf::kSmem, false, ready)) return rc;
+  const int row_tiles = static_cast<int>((static_cast<int64_t>(p.rows) + Cf::kRows - 1) / Cf::kRows);
+  const int64_t items = static_cast<int64_t>(row_tiles) * p.kv_heads * p.batch;
+  const int splits = key_splits(items, (p.sk + Cf::kKT - 1) / Cf::kKT, 2, 8);
+  return launch_split(kernel, items, splits, kThreads, Cf::kSmem, st, p, row_tiles, splits);
 }
 
 template <bool kBf16, int kD, bool kBias>
 int launch_keep(const CrossParams& p, cudaStream_t st) {
   const auto kernel = cross_keep_kernel<kBf16, kD, kBias>;
   static std::atomic<uint64_t> ready{0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return kErrCuda;
-  if (dev >= 64 || !(ready.load() >> dev & 1)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess)
-      return kErrCuda;
-    if (dev < 64) ready.fetch_or(1ull << dev);
-  }
+  if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), 200 * 1024, false, ready)) return rc;
   const int smem = KeepCfg<kD>::smem(p.sk);
   // as many CTAs as the SMs hold at once (about 200 registers a thread for
   // D = 128, and the shared memory), each with a share of the rows
@@ -658,9 +887,9 @@ template <bool kBf16, int kD>
 int launch_rows(const CrossParams& p, cudaStream_t st) {
   if (p.rows > 64 && p.sk <= S3_KEEP && KeepCfg<kD>::smem(p.sk) <= 100 * 1024)
     return p.bias ? launch_keep<kBf16, kD, true>(p, st) : launch_keep<kBf16, kD, false>(p, st);
-  if (p.rows <= 16)
-    return p.bias ? launch_variant<kBf16, kD, 1, true>(p, st) : launch_variant<kBf16, kD, 1, false>(p, st);
-  return p.bias ? launch_variant<kBf16, kD, 4, true>(p, st) : launch_variant<kBf16, kD, 4, false>(p, st);
+  if (p.rows <= 16 && cross_kv_maps(p))
+    return p.bias ? launch_few<kBf16, kD, true>(p, st) : launch_few<kBf16, kD, false>(p, st);
+  return p.bias ? launch_rows_any<kBf16, kD, true>(p, st) : launch_rows_any<kBf16, kD, false>(p, st);
 }
 
 }  // namespace

@@ -1,11 +1,14 @@
 // cross_attention.cuh - what the two cross-attention kernels share: the
 // checked arguments and how rows, heads and keys are numbered.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <initializer_list>
 
 #include "sam3cu_internal.h"
+#include "tma_host.cuh"
 
 namespace s3 {
 
@@ -47,10 +50,61 @@ __device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
   return v;
 }
 
+// Which dimensions of K and V a batch or its heads share: factors of the
+// coordinates, 0 or 1.
+struct KvShare {
+  int kb, kh, vb, vh;
+};
+
+// One dimension of a tensor map; one of stride 0 (shared data) or a single
+// element becomes one of extent 1 (*mul 0).
+struct TensorDim {
+  int64_t extent, stride;
+  int* mul;
+};
+// A tensor [d2][d1][d0][head_dim] of 16-bit elements by element strides, boxes
+// of box[2] x box[1] x box[0] rows of 64 elements (128-byte swizzle), or of 32
+// (64-byte swizzle) for head_dim <= 32; what lies past head_dim reads zeros.
+inline bool make_cross_map(CUtensorMap* m, const void* base, int dtype, int head_dim, const TensorDim (&d)[3],
+                           const int (&box)[3]) {
+  EncodeTiledFn fn = get_encode_tiled();
+  if (!fn) return false;
+  const bool small = head_dim <= 32;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), 1, 1, 1};
+  cuuint64_t strides[3] = {16, 16, 16};
+  cuuint32_t bx[4] = {small ? 32u : 64u, 1, 1, 1}, es[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 3; ++i) {
+    bx[i + 1] = static_cast<cuuint32_t>(box[i]);
+    if (d[i].mul) *d[i].mul = d[i].stride != 0;
+    if (d[i].stride == 0) continue;
+    dims[i + 1] = static_cast<cuuint64_t>(d[i].extent);
+    strides[i] = static_cast<cuuint64_t>(d[i].stride) * 2;
+  }
+  return fn(m, dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+            const_cast<void*>(base), dims, strides, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            small ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+inline bool make_kv_maps(const CrossParams& p, int dtype, int keys, CUtensorMap* mk, CUtensorMap* mv, KvShare* share) {
+  const TensorDim dk[3] = {{p.sk, p.ks, nullptr}, {p.kv_heads, p.kh, &share->kh}, {p.batch, p.kb, &share->kb}};
+  const TensorDim dv[3] = {{p.sk, p.vs, nullptr}, {p.kv_heads, p.vh, &share->vh}, {p.batch, p.vb, &share->vb}};
+  const int box[3] = {keys, 1, 1};
+  return make_cross_map(mk, p.k, dtype, p.head_dim, dk, box) && make_cross_map(mv, p.v, dtype, p.head_dim, dv, box);
+}
+// Whether tensor maps can describe K and V: strides below 2^40 bytes, and no
+// key shared (stride 0 cannot be part of a box).
+inline bool cross_kv_maps(const CrossParams& p) {
+  constexpr int64_t kMost = 1ll << 39;
+  for (int64_t x : {p.kb, p.ks, p.kh, p.vb, p.vs, p.vh})
+    if (x >= kMost) return false;
+  return p.sk > 0 && (p.sk == 1 || (p.ks != 0 && p.vs != 0));
+}
+
 int launch_cross_mma(const CrossParams& p, int dtype, cudaStream_t st);
 // cross_attention_sm100.cu: whether the tensor maps can describe the call.
 bool cross_tc_takes(const CrossParams& p);
 int launch_cross_tc(const CrossParams& p, int dtype, cudaStream_t st);
 unsigned int dev_error_cross();
+unsigned int dev_error_cross_few();
 
 }  // namespace s3

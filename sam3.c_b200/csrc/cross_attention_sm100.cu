@@ -79,7 +79,8 @@ struct TcParams {
   int n_items;    // items_x * kv_heads * batch
   int tiles;      // 128-row tiles of an item: 1 or 2
   int splits;     // CTAs of the cluster that share an item's keys (then one item a CTA)
-  int kmul_b, kmul_h, vmul_b, vmul_h, qmul_b;  // 0: that dimension is shared
+  int qmul_b;     // 0: the batch shares its queries
+  KvShare kv;
 };
 
 // One work item: up to two query tiles of a (batch, key head) and the key
@@ -244,8 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (elect_one()) {
         mbar_arrive_expect_tx(&k_full[st], kTile);
         for (int h = 0; h < Cf::kHalves; ++h)
-          tma_load_4d(sK(st) + h * (kTile / 2), &tk, &k_full[st], h * 64, row, it.kvh * prm.kmul_h,
-                      it.b * prm.kmul_b);
+          tma_load_4d(sK(st) + h * (kTile / 2), &tk, &k_full[st], h * 64, row, it.kvh * prm.kv.kh,
+                      it.b * prm.kv.kb);
       }
       __syncwarp();
       if (c.j == 0) {
@@ -268,8 +269,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (elect_one()) {
         mbar_arrive_expect_tx(&v_full[st], kTile);
         for (int h = 0; h < Cf::kHalves; ++h)
-          tma_load_4d(sV(st) + h * (kTile / 2), &tv, &v_full[st], h * 64, row, it.kvh * prm.vmul_h,
-                      it.b * prm.vmul_b);
+          tma_load_4d(sV(st) + h * (kTile / 2), &tv, &v_full[st], h * 64, row, it.kvh * prm.kv.vh,
+                      it.b * prm.kv.vb);
       }
       __syncwarp();
     }
@@ -553,31 +554,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   cluster_sync();  // the others may still read this CTA's partial rows
 }
 
-// One tensor as [d2][d1][d0][head_dim] with element strides; a dimension of
-// stride 0 (shared data) or one element becomes one of extent 1 (*mul 0).
-struct Dim {
-  int64_t extent, stride;
-  int* mul;
-};
-bool make_map(CUtensorMap* m, const void* base, int dtype, int head_dim, int box_d, const Dim (&d)[3],
-              const int (&box)[3], CUtensorMapSwizzle swz) {
-  EncodeTiledFn fn = get_encode_tiled();
-  if (!fn) return false;
-  cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), 1, 1, 1};
-  cuuint64_t strides[3] = {16, 16, 16};
-  cuuint32_t bx[4] = {static_cast<cuuint32_t>(box_d), 1, 1, 1}, es[4] = {1, 1, 1, 1};
-  for (int i = 0; i < 3; ++i) {
-    bx[i + 1] = static_cast<cuuint32_t>(box[i]);
-    if (d[i].mul) *d[i].mul = d[i].stride != 0;
-    if (d[i].stride == 0) continue;
-    dims[i + 1] = static_cast<cuuint64_t>(d[i].extent);
-    strides[i] = static_cast<cuuint64_t>(d[i].stride) * 2;
-  }
-  return fn(m, dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-            const_cast<void*>(base), dims, strides, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <bool kBf16, int kD, bool kMask>
 int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TcParams& prm,
                    int64_t ctas, cudaStream_t st) {
@@ -622,14 +598,10 @@ int launch_typed(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap
 }  // namespace
 
 bool cross_tc_takes(const CrossParams& p) {
-  if (p.bias) return false;
-  // a tensor map's stride is below 2^40 bytes, and where it is 0 the
-  // dimension cannot be part of a box
-  const int64_t s[] = {p.qb, p.qs, p.qh, p.kb, p.ks, p.kh, p.vb, p.vs, p.vh};
-  for (int64_t x : s)
-    if (x >= (1ll << 39)) return false;
-  if ((p.sq > 1 && p.qs == 0) || (p.kv_heads * p.group > 1 && p.qh == 0)) return false;
-  return p.sk > 0 && (p.sk == 1 || (p.ks != 0 && p.vs != 0));
+  if (p.bias || !cross_kv_maps(p)) return false;
+  constexpr int64_t kMost = 1ll << 39;
+  if (p.qb >= kMost || p.qs >= kMost || p.qh >= kMost) return false;
+  return (p.sq == 1 || p.qs != 0) && (p.kv_heads * p.group == 1 || p.qh != 0);
 }
 
 int launch_cross_tc(const CrossParams& p, int dtype, cudaStream_t st) {
@@ -651,17 +623,11 @@ int launch_cross_tc(const CrossParams& p, int dtype, cudaStream_t st) {
   // 2048 keys, D = 64: 29 / 63 / 203 us against 37 / 71 / 208 with a CTA each).
   // Long ones have a CTA each, dealt out as SMs come free (lengths differ).
   if (prm.splits == 1 && key_tiles <= 16) ctas = std::min<int64_t>(ctas, num_sms());
-  const int box_d = p.head_dim <= 32 ? 32 : 64;
-  const CUtensorMapSwizzle swz = box_d == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
   CUtensorMap mq, mk, mv;
-  const Dim dq[3] = {{static_cast<int64_t>(p.kv_heads) * p.group, p.qh, nullptr}, {p.sq, p.qs, nullptr},
-                     {p.batch, p.qb, &prm.qmul_b}};
-  const Dim dk[3] = {{p.sk, p.ks, nullptr}, {p.kv_heads, p.kh, &prm.kmul_h}, {p.batch, p.kb, &prm.kmul_b}};
-  const Dim dv[3] = {{p.sk, p.vs, nullptr}, {p.kv_heads, p.vh, &prm.vmul_h}, {p.batch, p.vb, &prm.vmul_b}};
-  const int bq[3] = {p.group, prm.qpt, 1}, bk[3] = {kKV, 1, 1};
-  if (!make_map(&mq, p.q, dtype, p.head_dim, box_d, dq, bq, swz) ||
-      !make_map(&mk, p.k, dtype, p.head_dim, box_d, dk, bk, swz) ||
-      !make_map(&mv, p.v, dtype, p.head_dim, box_d, dv, bk, swz))
+  const TensorDim dq[3] = {{static_cast<int64_t>(p.kv_heads) * p.group, p.qh, nullptr}, {p.sq, p.qs, nullptr},
+                           {p.batch, p.qb, &prm.qmul_b}};
+  const int bq[3] = {p.group, prm.qpt, 1};
+  if (!make_cross_map(&mq, p.q, dtype, p.head_dim, dq, bq) || !make_kv_maps(p, dtype, kKV, &mk, &mv, &prm.kv))
     return kErrTma;
   if (p.head_dim <= 32) return launch_typed<32>(mq, mk, mv, prm, dtype, ctas, st);
   if (p.head_dim <= 64) return launch_typed<64>(mq, mk, mv, prm, dtype, ctas, st);
