@@ -43,6 +43,9 @@ S3_DEV_ERROR_ACCESSOR(dev_error_cross_few)
 
 namespace {
 
+#ifndef S3_RPS
+#define S3_RPS 4
+#endif
 #ifndef S3_KEEP
 #define S3_KEEP 256
 #endif
@@ -91,17 +94,20 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 // kD: head_dim rounded up to 32, 64 or 128 (the copies fill the rest with
 // zeros).
-template <int kD>
+template <int kD, bool kBias>
 struct RowsCfg {
   static constexpr int kRows = 64;                     // query rows of a CTA, 16 to a warp
   static constexpr int kKT = 64;                       // keys of a tile
   static constexpr int kChunks = kD / 8;               // 16-byte pieces of a row
   static constexpr int kTileBytes = kKT * kD * 2;      // K or V
-  static constexpr int kStages = kD == 32 ? 4 : kD == 64 ? 3 : 2;
+  static constexpr int kBiasPitch = kKT + 4;           // floats of a bias row
+  static constexpr int kBiasBytes = kBias ? kRows * kBiasPitch * 4 : 0;
+  static constexpr int kStageBytes = 2 * kTileBytes + kBiasBytes;
+  static constexpr int kStages = kD == 32 && !kBias ? 4 : kD == 128 && !kBias ? 2 : 3;
   static constexpr int kQBytes = kRows * kD * 2;
   static constexpr int kPitch = kD + 4;                // floats of a partial row
   static constexpr int kPartBytes = kRows * kPitch * 4;  // over the ring
-  static constexpr int kRing = 2 * kStages * kTileBytes;
+  static constexpr int kRing = kStages * kStageBytes;
   static constexpr int kSmem = kQBytes + (kRing > kPartBytes ? kRing : kPartBytes);
 };
 template <int kD>
@@ -144,10 +150,12 @@ struct RowState {
   }
   // Scores to P, against the maximum with them in it; sum and O rescaled.
   // f16 P are times 2^14, which cancels in O / sum: below 2^-14 the type has
-  // no full precision left.
-  template <int kKeys>
-  __device__ __forceinline__ void softmax(float (&s)[kKeys / 8][4], float to_log2, bool bf) {
-    const float shift = bf ? 0.f : 14.f;
+  // no full precision left.  kApart: the maximum is taken off before the
+  // factor (scores with a bias, whose product with it could overflow).
+  template <int kKeys, bool kBf16, bool kApart>
+  __device__ __forceinline__ void softmax(float (&s)[kKeys / 8][4], float to_log2) {
+    const float shift = kBf16 ? 0.f : 14.f;
+    float top[2], corr[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float mx = -INFINITY;
@@ -155,22 +163,43 @@ struct RowState {
       for (int j = 0; j < kKeys / 8; ++j) mx = max3(mx, s[j][2 * h], s[j][2 * h + 1]);
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float m_new = fmaxf(m[h], mx);
-      const float base = m_new == -INFINITY ? 0.f : m_new;  // nothing counted yet: every p is 0
-      const float corr = ex2((m[h] - base) * to_log2);
-      m[h] = m_new;
-      float sum = 0.f;
+      top[h] = fmaxf(m[h], mx);
+    }
+    const bool grew = __any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float base = top[h] == -INFINITY ? 0.f : top[h];  // nothing counted yet: every p is 0
+      corr[h] = ex2((m[h] - base) * to_log2);
+      m[h] = top[h];
+      const uint64_t c2 = f2pack(to_log2, to_log2);
+      const float k = kApart ? shift : fmaf(-base, to_log2, shift);
+      const uint64_t k2 = f2pack(k, k), b2 = f2pack(-base, -base);
+      uint64_t sum2 = f2pack(0.f, 0.f);
 #pragma unroll
       for (int j = 0; j < kKeys / 8; ++j) {
-        s[j][2 * h] = ex2(fmaf(s[j][2 * h] - base, to_log2, shift));
-        s[j][2 * h + 1] = ex2(fmaf(s[j][2 * h + 1] - base, to_log2, shift));
-        sum += s[j][2 * h] + s[j][2 * h + 1];
+        uint64_t x = f2pack(s[j][2 * h], s[j][2 * h + 1]);
+        if (kApart) x = fadd2(x, b2);
+        float e0, e1;
+        f2unpack(ffma2(x, c2, k2), e0, e1);
+        s[j][2 * h] = ex2(e0);
+        s[j][2 * h + 1] = ex2(e1);
+        sum2 = fadd2(sum2, f2pack(s[j][2 * h], s[j][2 * h + 1]));
       }
-      l[h] = fmaf(l[h], corr, sum);
+      float s0, s1;
+      f2unpack(sum2, s0, s1);
+      l[h] = fmaf(l[h], corr[h], s0 + s1);
+    }
+    if (grew) {
+      const uint64_t c2[2] = {f2pack(corr[0], corr[0]), f2pack(corr[1], corr[1])};
 #pragma unroll
       for (int j = 0; j < kD / 8; ++j) {
-        acc[j][2 * h] *= corr;
-        acc[j][2 * h + 1] *= corr;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float a0, a1;
+          f2unpack(fmul2(f2pack(acc[j][2 * h], acc[j][2 * h + 1]), c2[h]), a0, a1);
+          acc[j][2 * h] = a0;
+          acc[j][2 * h + 1] = a1;
+        }
       }
     }
   }
@@ -262,11 +291,12 @@ __device__ __forceinline__ void join_rows(const CrossParams& p, float* part, flo
 
 template <bool kBf16, int kD, bool kBias>
 __global__ void __launch_bounds__(kThreads) cross_rows_kernel(const __grid_constant__ CrossParams p, int row_tiles,
-                                                             int splits) {
-  using Cf = RowsCfg<kD>;
+                                                              int splits, int bias_step) {
+  using Cf = RowsCfg<kD, kBias>;
   constexpr int kKT = Cf::kKT, kCh = Cf::kChunks, kStages = Cf::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ float2 ml[Cf::kRows];  // (max, sum) of each row
+  __shared__ const float* brow[kBias ? Cf::kRows : 1];
   const uint32_t sq = smem_u32(smem), ring = sq + Cf::kQBytes;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -295,7 +325,7 @@ __global__ void __launch_bounds__(kThreads) cross_rows_kernel(const __grid_const
 
   // Tile t into its ring slot.
   auto load = [&](int t) {
-    const uint32_t sk = ring + (t % kStages) * 2 * Cf::kTileBytes, sv = sk + Cf::kTileBytes;
+    const uint32_t sk = ring + (t % kStages) * Cf::kStageBytes, sv = sk + Cf::kTileBytes;
 #pragma unroll 4
     for (int i = 0; i < kKT * kCh / kThreads; ++i) {
       const int idx = tid + i * kThreads;
@@ -308,7 +338,31 @@ __global__ void __launch_bounds__(kThreads) cross_rows_kernel(const __grid_const
       cp_async16(sk + tile_at<kCh>(r, c), kg + at * p.ks + cc, ok);
       cp_async16(sv + tile_at<kCh>(r, c), vg + at * p.vs + cc, ok);
     }
+    if constexpr (kBias) {
+      // the tile's bias, a row by 16 lanes of 4 keys; bias_step 4: its rows
+      // start on 16 bytes, 1: key by key
+      const uint32_t sb = sv + Cf::kTileBytes;
+#pragma unroll 2
+      for (int r = tid / 16; r < Cf::kRows; r += kThreads / 16) {
+        const float* src = brow[kBias ? r : 0];
+        const int c = tid % 16 * 4, key = t * kKT + c;
+        const uint32_t dst = sb + (r * Cf::kBiasPitch + c) * 4;
+        if (bias_step == 4) {
+          cp_async16(dst, src + (key < len ? key : 0), key < len);  // (sk is a multiple of 4)
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) cp_async4(dst + 4 * e, src + (key + e < len ? key + e : 0), key + e < len);
+        }
+      }
+    }
   };
+  if constexpr (kBias) {
+    if (tid < Cf::kRows) {
+      const int row = min(row0 + tid, p.rows - 1), q = row / p.group;
+      brow[tid] = p.bias + b * p.bb + static_cast<int64_t>(kvh * p.group + row - q * p.group) * p.bh + q * p.bs;
+    }
+    __syncthreads();
+  }
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) {
     if (t0 + i < t1) load(t0 + i);
@@ -321,15 +375,6 @@ __global__ void __launch_bounds__(kThreads) cross_rows_kernel(const __grid_const
   // with a bias the scores are in natural units (its lowest finite values
   // would overflow in base 2), without one they stay unscaled dot products
   const float to_log2 = kBias ? kLog2e : p.scale_log2;
-  const float* brow[2] = {nullptr, nullptr};
-  if (kBias) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = min(row0 + warp * 16 + (lane >> 2) + 8 * h, p.rows - 1);
-      brow[h] = p.bias + b * p.bb + static_cast<int64_t>(kvh * p.group + r % p.group) * p.bh + (r / p.group) * p.bs;
-    }
-  }
-
   cp_async_wait<kStages - 1>();  // the queries
   __syncthreads();
 #pragma unroll
@@ -343,20 +388,9 @@ __global__ void __launch_bounds__(kThreads) cross_rows_kernel(const __grid_const
     __syncthreads();
     if (t + kStages - 1 < t1) load(t + kStages - 1);  // into the slot of tile t - 1, which all have left
     cp_async_commit();
-    const uint32_t sk = ring + (t % kStages) * 2 * Cf::kTileBytes, sv = sk + Cf::kTileBytes;
+    const uint32_t sk = ring + (t % kStages) * Cf::kStageBytes, sv = sk + Cf::kTileBytes;
     const int key0 = t * kKT;
 
-    float bias[kBias ? kKT / 8 : 1][4];
-    if (kBias) {
-#pragma unroll
-      for (int j = 0; j < kKT / 8; ++j) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = key0 + j * 8 + (lane & 3) * 2 + (e & 1);
-          bias[kBias ? j : 0][e] = key < len ? __ldg(brow[e >> 1] + key) : 0.f;
-        }
-      }
-    }
     float s[kKT / 8][4];
 #pragma unroll
     for (int j = 0; j < kKT / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
@@ -371,11 +405,19 @@ __global__ void __launch_bounds__(kThreads) cross_rows_kernel(const __grid_const
         mma16816<kBf16>(s[2 * jp + 1], qf[kk], b2, b3);
       }
     }
-    if (kBias) {
+    if constexpr (kBias) {
 #pragma unroll
-      for (int j = 0; j < kKT / 8; ++j)
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t sb = sv + Cf::kTileBytes +
+                            ((warp * 16 + (lane >> 2) + 8 * h) * Cf::kBiasPitch + (lane & 3) * 2) * 4;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] = fmaf(s[j][e], p.scale, bias[kBias ? j : 0][e]);
+        for (int j = 0; j < kKT / 8; ++j) {
+          float x, y;
+          asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(x), "=f"(y) : "r"(sb + j * 32) : "memory");
+          f2unpack(ffma2(f2pack(s[j][2 * h], s[j][2 * h + 1]), f2pack(p.scale, p.scale), f2pack(x, y)), s[j][2 * h],
+                   s[j][2 * h + 1]);
+        }
+      }
     }
     if (mg || key0 + kKT > len) {
 #pragma unroll
@@ -387,7 +429,7 @@ __global__ void __launch_bounds__(kThreads) cross_rows_kernel(const __grid_const
         }
       }
     }
-    st.template softmax<kKT>(s, to_log2, kBf16);
+    st.template softmax<kKT, kBf16, kBias>(s, to_log2);
     // O += P V, P rounded to the operands' type
 #pragma unroll
     for (int kk = 0; kk < kKT / 16; ++kk) {
@@ -575,7 +617,7 @@ __global__ void __launch_bounds__(FewCfg<kD>::kThreads)
             if (!(mine >> (j * 8 + 1) & 1)) s[j][1] = s[j][3] = -INFINITY;
           }
         }
-        rs.template softmax<32>(s, to_log2, kBf16);
+        rs.template softmax<32, kBf16, kBias>(s, to_log2);
         // O += P V, P rounded to the operands' type
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
@@ -739,7 +781,7 @@ __global__ void __launch_bounds__(kThreads) cross_keep_kernel(const __grid_const
           if (!(mine_on >> (j * 8 + 1) & 1)) s[j][1] = s[j][3] = -INFINITY;
         }
       }
-      st.template softmax<kKW>(s, to_log2, kBf16);
+      st.template softmax<kKW, kBf16, kBias>(s, to_log2);
       // O += P V, P rounded to the operands' type
 #pragma unroll
       for (int kk = 0; kk < kKW / 16; ++kk) {
@@ -854,14 +896,17 @@ int launch_few(const CrossParams& p, cudaStream_t st) {
 
 template <bool kBf16, int kD, bool kBias>
 int launch_rows_any(const CrossParams& p, cudaStream_t st) {
-  using Cf = RowsCfg<kD>;
+  using Cf = RowsCfg<kD, kBias>;
   static std::atomic<uint64_t> ready{0};
   const auto kernel = cross_rows_kernel<kBf16, kD, kBias>;
   if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), Cf::kSmem, false, ready)) return rc;
   const int row_tiles = static_cast<int>((static_cast<int64_t>(p.rows) + Cf::kRows - 1) / Cf::kRows);
   const int64_t items = static_cast<int64_t>(row_tiles) * p.kv_heads * p.batch;
-  const int splits = key_splits(items, (p.sk + Cf::kKT - 1) / Cf::kKT, 2, 8);
-  return launch_split(kernel, items, splits, kThreads, Cf::kSmem, st, p, row_tiles, splits);
+  const int per_sm = std::min(S3_RPS, 200 * 1024 / Cf::kSmem);
+  const int splits = key_splits(items, (p.sk + Cf::kKT - 1) / Cf::kKT, per_sm, 8);
+  const bool wide = p.bias && (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0 && p.sk % 4 == 0 && p.bb % 4 == 0 &&
+                    p.bh % 4 == 0 && p.bs % 4 == 0;
+  return launch_split(kernel, items, splits, kThreads, Cf::kSmem, st, p, row_tiles, splits, wide ? 4 : 1);
 }
 
 template <bool kBf16, int kD, bool kBias>
