@@ -43,15 +43,6 @@ S3_DEV_ERROR_ACCESSOR(dev_error_cross_few)
 
 namespace {
 
-#ifndef S3_RPS
-#define S3_RPS 4
-#endif
-#ifndef S3_KEEP
-#define S3_KEEP 256
-#endif
-#ifndef S3_TCK
-#define S3_TCK 256
-#endif
 constexpr int kThreads = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxKeep = 2048;  // keys that cross_keep_kernel may hold
@@ -673,7 +664,7 @@ struct KeepCfg {
 template <bool kBf16, int kD, bool kBias>
 __global__ void __launch_bounds__(kThreads) cross_keep_kernel(const __grid_constant__ CrossParams p, int chunks) {
   using Cf = KeepCfg<kD>;
-  constexpr int kCh = Cf::kChunks, kKW = 64, kWarps = kThreads / 32;
+  constexpr int kCh = Cf::kChunks, kKW = 32, kWarps = kThreads / 32;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint32_t on[kMaxKeep / 32];  // bit per key that counts
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -761,8 +752,7 @@ __global__ void __launch_bounds__(kThreads) cross_keep_kernel(const __grid_const
           }
         }
       }
-      const uint64_t bits = static_cast<uint64_t>(on[k0 / 32]) |
-                            (k0 + 32 < kp ? static_cast<uint64_t>(on[k0 / 32 + 1]) << 32 : 0ull);
+      const uint32_t bits = on[k0 / 32];
 #pragma unroll
       for (int j = 0; j < kKW / 8; ++j) {
         if (kBias && j * 8 < n) {
@@ -773,8 +763,8 @@ __global__ void __launch_bounds__(kThreads) cross_keep_kernel(const __grid_const
           }
         }
       }
-      if (bits != ~0ull) {
-        const uint64_t mine_on = bits >> ((lane & 3) * 2);
+      if (bits != ~0u) {
+        const uint32_t mine_on = bits >> ((lane & 3) * 2);
 #pragma unroll
         for (int j = 0; j < kKW / 8; ++j) {
           if (!(mine_on >> (j * 8) & 1)) s[j][0] = s[j][2] = -INFINITY;
@@ -902,7 +892,7 @@ int launch_rows_any(const CrossParams& p, cudaStream_t st) {
   if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), Cf::kSmem, false, ready)) return rc;
   const int row_tiles = static_cast<int>((static_cast<int64_t>(p.rows) + Cf::kRows - 1) / Cf::kRows);
   const int64_t items = static_cast<int64_t>(row_tiles) * p.kv_heads * p.batch;
-  const int per_sm = std::min(S3_RPS, 200 * 1024 / Cf::kSmem);
+  const int per_sm = std::min(4, 200 * 1024 / Cf::kSmem);
   const int splits = key_splits(items, (p.sk + Cf::kKT - 1) / Cf::kKT, per_sm, 8);
   const bool wide = p.bias && (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0 && p.sk % 4 == 0 && p.bb % 4 == 0 &&
                     p.bh % 4 == 0 && p.bs % 4 == 0;
@@ -914,11 +904,15 @@ int launch_keep(const CrossParams& p, cudaStream_t st) {
   const auto kernel = cross_keep_kernel<kBf16, kD, kBias>;
   static std::atomic<uint64_t> ready{0};
   if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), 200 * 1024, false, ready)) return rc;
+  static const int regs = [&] {
+    cudaFuncAttributes fa;
+    return cudaFuncGetAttributes(&fa, kernel) == cudaSuccess ? fa.numRegs : 255;
+  }();
   const int smem = KeepCfg<kD>::smem(p.sk);
-  // as many CTAs as the SMs hold at once (about 200 registers a thread for
-  // D = 128, and the shared memory), each with a share of the rows
+  // as many CTAs as the SMs hold at once, each with a share of the rows (one
+  // more per SM than fits makes a second wave: 36 -> 50 us for image to text)
   const int64_t bh = static_cast<int64_t>(p.kv_heads) * p.batch;
-  const int per_sm = std::min(kD == 128 ? 2 : kD == 64 ? 4 : 6, 200 * 1024 / smem);
+  const int per_sm = std::max(1, std::min(65536 / ((regs + 7) / 8 * 8 * kThreads), 224 * 1024 / (smem + 1024)));
   const int tiles = (p.rows + 15) / 16;
   int64_t chunks = std::max<int64_t>(1, static_cast<int64_t>(per_sm) * num_sms() / bh);
   chunks = std::min<int64_t>(chunks, (tiles + kThreads / 32 - 1) / (kThreads / 32));
@@ -930,7 +924,7 @@ int launch_keep(const CrossParams& p, cudaStream_t st) {
 
 template <bool kBf16, int kD>
 int launch_rows(const CrossParams& p, cudaStream_t st) {
-  if (p.rows > 64 && p.sk <= S3_KEEP && KeepCfg<kD>::smem(p.sk) <= 100 * 1024)
+  if (p.rows > 64 && p.sk <= 256 && KeepCfg<kD>::smem(p.sk) <= 100 * 1024)
     return p.bias ? launch_keep<kBf16, kD, true>(p, st) : launch_keep<kBf16, kD, false>(p, st);
   if (p.rows <= 16 && cross_kv_maps(p))
     return p.bias ? launch_few<kBf16, kD, true>(p, st) : launch_few<kBf16, kD, false>(p, st);
@@ -1011,6 +1005,12 @@ extern "C" int sam3cu_cross_attention(const struct sam3cu_cross_attention_args* 
     p.bs = a->bias_strides[2];
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (cross_tc_takes(p) && p.rows > 64 && p.sk > S3_TCK) return launch_cross_tc(p, a->dtype, st);
+  // Which kernel: tcgen05 for many rows, except over few keys where heads are
+  // small or the whole call is (4 x 8 heads x 5184 queries, D = 32: 77 keys 17
+  // us kept in shared memory, 25 us on tcgen05, 256 keys 36 and 31; D = 64, 77
+  // keys: 42 and 29; 8 heads x 300 queries, D = 64, 77 keys: 5.3 and 7.9).
+  const bool small = p.sk <= 128 && (p.head_dim <= 32 || static_cast<int64_t>(p.rows) * p.kv_heads * p.batch <=
+                                                             128ll * num_sms());
+  if (p.rows > 64 && !small && cross_tc_takes(p)) return launch_cross_tc(p, a->dtype, st);
   return launch_cross_mma(p, a->dtype, st);
 }

@@ -611,12 +611,16 @@ int launch_cross_tc(const CrossParams& p, int dtype, cudaStream_t st) {
   prm.qpt = kQ / p.group;
   const int64_t row_tiles = (static_cast<int64_t>(p.sq) + prm.qpt - 1) / prm.qpt;
   const int64_t heads = static_cast<int64_t>(p.kv_heads) * p.batch;
-  prm.tiles = 2;
-  prm.splits = 1;
+  const int key_tiles = (p.sk + kKV - 1) / kKV;
+  // Two query tiles to a CTA; one, where even then there are SMs to spare, and
+  // the keys over the CTAs of a cluster while there still are (with at least
+  // four key tiles each).
+  prm.tiles = heads * row_tiles <= num_sms() ? 1 : 2;
   prm.items_x = static_cast<int>((row_tiles + prm.tiles - 1) / prm.tiles);
   if (heads * prm.items_x > 0x3fffffffLL) return kErrShape;
   prm.n_items = static_cast<int>(heads * prm.items_x);
-  const int key_tiles = (p.sk + kKV - 1) / kKV;
+  prm.splits = 1;
+  while (prm.splits < 8 && prm.n_items * 2ll * prm.splits <= num_sms() && key_tiles >= 8 * prm.splits) prm.splits *= 2;
   int64_t ctas = static_cast<int64_t>(prm.n_items) * prm.splits;
   // Short items: one CTA per SM that walks them, so that an item's first loads
   // and S overlap the epilogue before it (4 x 8 heads x 5184 queries, 77 / 512 /
