@@ -12,9 +12,8 @@
 
 using namespace s3;
 
+namespace s3 {
 namespace {
-
-cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
 
 // The library's own stream-ordered pool for per-call temporaries (the
 // 16-bit copies of a Q8_0 weight and of F32 activations): its release
@@ -45,10 +44,18 @@ cudaMemPool_t call_pool() {
   return pools[dev];
 }
 
+}  // namespace
+
 cudaError_t pool_alloc(void** p, size_t n, cudaStream_t st) {
   cudaMemPool_t pool = call_pool();
   return pool ? cudaMallocFromPoolAsync(p, n, pool, st) : cudaMallocAsync(p, n, st);
 }
+
+}  // namespace s3
+
+namespace {
+
+cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
 
 int linear_common(const void* x, int x_dtype, const void* w, const int8_t* q, const float* sc, const float* bias,
                   const float* residual, void* y, int y_dtype, int M, int K, int N, int act, void* stream) {

@@ -196,51 +196,70 @@ struct RowState {
   }
 };
 
-// The end of a kernel whose threads left, for kRows rows and each of kWK key
-// warps, (max, sum) in ml [kWK][kRows] and the unscaled partial O in part
-// [kWK][kRows][kD + 4]: adds the warps' rows up, and with splits > 1 those of
-// the cluster's CTAs (each sums a share of the rows over all of them, in rank
-// order), and writes the output.  wgt: [kWK][kRows], kWK > 1 only.
-template <bool kBf16, int kD, int kRows, int kWK, int kN>
-__device__ __forceinline__ void join_rows(const CrossParams& p, float* part, float2* ml, float* wgt, int row0, int b,
-                                          int kvh, int split, int splits, float to_log2) {
+// 8 elements of an output row, scaled by what they were summed with.
+template <bool kBf16>
+__device__ __forceinline__ void store_row(const CrossParams& p, int b, int kvh, int row, int c, const float (&o)[8],
+                                          float l) {
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays NaN
+  const int q = row / p.group;
+  uint4 w4;
+  w4.x = pack2<kBf16>(o[0] * inv, o[1] * inv);
+  w4.y = pack2<kBf16>(o[2] * inv, o[3] * inv);
+  w4.z = pack2<kBf16>(o[4] * inv, o[5] * inv);
+  w4.w = pack2<kBf16>(o[6] * inv, o[7] * inv);
+  *reinterpret_cast<uint4*>(p.o + b * p.ob + q * p.os + static_cast<int64_t>(kvh * p.group + row - q * p.group) * p.oh +
+                            c) = w4;
+}
+
+// Adds up what the key warps of a CTA left for its kRows rows: (max, sum) in ml
+// [kWK][kRows] and the unscaled partial O in part [kWK][kRows][kD + 4]; the
+// sums take the place of the first warp's.  wgt: [kWK][kRows].
+template <int kD, int kRows, int kWK, int kN>
+__device__ __forceinline__ void join_warps(float* part, float2* ml, float* wgt, float to_log2) {
   constexpr int kPitch = kD + 4;
   const int tid = threadIdx.x;
   __syncthreads();
-  if constexpr (kWK > 1) {
-    // the weight of each warp's partial row against the row's maximum
-    if (tid < kRows) {
-      float m = -INFINITY, l = 0.f;
+  // the weight of each warp's partial row against the row's maximum
+  if (tid < kRows) {
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWK; ++w) m = fmaxf(m, ml[w * kRows + tid].x);
-      const float base = m == -INFINITY ? 0.f : m;
+    for (int w = 0; w < kWK; ++w) m = fmaxf(m, ml[w * kRows + tid].x);
+    const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-      for (int w = 0; w < kWK; ++w) {
-        const float f = ex2((ml[w * kRows + tid].x - base) * to_log2);
-        wgt[w * kRows + tid] = f;
-        l = fmaf(f, ml[w * kRows + tid].y, l);
-      }
-      ml[tid] = make_float2(m, l);
+    for (int w = 0; w < kWK; ++w) {
+      const float f = ex2((ml[w * kRows + tid].x - base) * to_log2);
+      wgt[w * kRows + tid] = f;
+      l = fmaf(f, ml[w * kRows + tid].y, l);
     }
-    __syncthreads();
-    // one partial tile per CTA
-    for (int i = tid; i < kRows * kD / 4; i += kN) {
-      const int r = i / (kD / 4), c = (i % (kD / 4)) * 4;
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kWK; ++w) {
-        const float f = wgt[w * kRows + r];
-        const float4 x = *reinterpret_cast<const float4*>(part + (w * kRows + r) * kPitch + c);
-        a.x = fmaf(f, x.x, a.x);
-        a.y = fmaf(f, x.y, a.y);
-        a.z = fmaf(f, x.z, a.z);
-        a.w = fmaf(f, x.w, a.w);
-      }
-      *reinterpret_cast<float4*>(part + r * kPitch + c) = a;
-    }
+    ml[tid] = make_float2(m, l);
   }
+  __syncthreads();
+  for (int i = tid; i < kRows * kD / 4; i += kN) {
+    const int r = i / (kD / 4), c = (i % (kD / 4)) * 4;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWK; ++w) {
+      const float f = wgt[w * kRows + r];
+      const float4 x = *reinterpret_cast<const float4*>(part + (w * kRows + r) * kPitch + c);
+      a.x = fmaf(f, x.x, a.x);
+      a.y = fmaf(f, x.y, a.y);
+      a.z = fmaf(f, x.z, a.z);
+      a.w = fmaf(f, x.w, a.w);
+    }
+    *reinterpret_cast<float4*>(part + r * kPitch + c) = a;
+  }
+}
+
+// The end of a kernel that left ml [kRows] and part [kRows][kD + 4]: the rows to
+// the output, with splits > 1 added up over the cluster's CTAs (each takes a
+// share of the rows over all of them, in rank order).
+template <bool kBf16, int kD, int kRows, int kN>
+__device__ __forceinline__ void join_cluster(const CrossParams& p, float* part, float2* ml, int row0, int b, int kvh,
+                                             int split, int splits, float to_log2) {
+  constexpr int kPitch = kD + 4;
+  const int tid = threadIdx.x;
   if (splits > 1) cluster_sync();
-  else if (kWK > 1) __syncthreads();
+  else __syncthreads();
   // Rows to the output, 8 elements a thread.
   const int out_chunks = p.head_dim / 8;
   const uint32_t part_s = smem_u32(part), ml_s = smem_u32(ml);
@@ -267,15 +286,7 @@ __device__ __forceinline__ void join_rows(const CrossParams& p, float* part, flo
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] = part[r * kPitch + c + e];
     }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays NaN
-    const int row = row0 + r, q = row / p.group;
-    uint4 w4;
-    w4.x = pack2<kBf16>(o[0] * inv, o[1] * inv);
-    w4.y = pack2<kBf16>(o[2] * inv, o[3] * inv);
-    w4.z = pack2<kBf16>(o[4] * inv, o[5] * inv);
-    w4.w = pack2<kBf16>(o[6] * inv, o[7] * inv);
-    *reinterpret_cast<uint4*>(p.o + b * p.ob + q * p.os + static_cast<int64_t>(kvh * p.group + row - q * p.group) * p.oh +
-                              c) = w4;
+    store_row<kBf16>(p, b, kvh, row0 + r, c, o, l);
   }
   if (splits > 1) cluster_sync();  // the others may still read this CTA's partial rows
 }
@@ -457,7 +468,7 @@ __global__ void __launch_bounds__(kThreads) cross_rows_kernel(const __grid_const
     for (int j = 0; j < kD / 8; ++j)
       *reinterpret_cast<float2*>(dst + j * 8) = make_float2(st.acc[j][2 * h], st.acc[j][2 * h + 1]);
   }
-  join_rows<kBf16, kD, Cf::kRows, 1, kThreads>(p, part, ml, nullptr, row0, b, kvh, split, splits, to_log2);
+  join_cluster<kBf16, kD, Cf::kRows, kThreads>(p, part, ml, row0, b, kvh, split, splits, to_log2);
 }
 
 // Up to 16 rows of a key head: K and V are read once and little is done with
@@ -467,7 +478,7 @@ __global__ void __launch_bounds__(kThreads) cross_rows_kernel(const __grid_const
 template <bool kBf16, int kD, bool kBias>
 __global__ void __launch_bounds__(FewCfg<kD>::kThreads)
     cross_few_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                     const __grid_constant__ CrossParams p, const KvShare share, int row_tiles, int splits) {
+                     const __grid_constant__ CrossParams p, const KvShare share, int row_tiles, int splits, float* ws) {
   using Cf = FewCfg<kD>;
   constexpr int kCh = kD / 8, kStages = Cf::kStages, kTile = Cf::kTileBytes, kHalves = kD == 128 ? 2 : 1;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -646,8 +657,71 @@ __global__ void __launch_bounds__(FewCfg<kD>::kThreads)
         *reinterpret_cast<float2*>(dst + j * 8) = make_float2(rs.acc[j][2 * h], rs.acc[j][2 * h + 1]);
     }
   }
-  join_rows<kBf16, kD, Cf::kRows, Cf::kWarps, Cf::kThreads>(p, reinterpret_cast<float*>(smem), ml, wgt, row0, b, kvh,
-                                                            split, splits, to_log2);
+  float* part = reinterpret_cast<float*>(smem);
+  join_warps<kD, Cf::kRows, Cf::kWarps, Cf::kThreads>(part, ml, wgt, to_log2);
+  if (ws) {
+    // to cross_join_kernel: this CTA's (max, sum) and partial rows
+    __syncthreads();
+    float* dst = ws + static_cast<int64_t>(blockIdx.x) * Cf::kRows * (kD + 2);
+    for (int i = tid; i < Cf::kRows * kD / 4; i += Cf::kThreads)
+      *reinterpret_cast<float4*>(dst + i * 4) =
+          *reinterpret_cast<const float4*>(part + i / (kD / 4) * Cf::kPitch + i % (kD / 4) * 4);
+    if (tid < Cf::kRows) *reinterpret_cast<float2*>(dst + Cf::kRows * kD + tid * 2) = ml[tid];
+    return;
+  }
+  join_cluster<kBf16, kD, Cf::kRows, Cf::kThreads>(p, part, ml, row0, b, kvh, split, splits, to_log2);
+}
+
+// Adds up the partial rows that cross_few_kernel left in its workspace, a CTA
+// per row: 8 groups of threads take every 8th split, then are added up in order.
+template <bool kBf16, int kD>
+__global__ void __launch_bounds__(kD) cross_join_kernel(const __grid_constant__ CrossParams p, int row_tiles,
+                                                        int splits, const float* ws, float to_log2) {
+  constexpr int kRows = FewCfg<kD>::kRows, kSlab = kRows * (kD + 2), kCh = kD / 8;
+  __shared__ float top[kD / 32];
+  __shared__ float part[8][kD + 1];  // and the group's sum of weights
+  const int r = blockIdx.x % kRows, item = blockIdx.x / kRows, rt = item % row_tiles, bh = item / row_tiles;
+  const int row = rt * kRows + r;
+  if (row >= p.rows) return;
+  const int tid = threadIdx.x, c = tid % kCh * 8, group = tid / kCh;
+  const float* src = ws + static_cast<int64_t>(item) * splits * kSlab;
+  const float* ml = src + kRows * kD + r * 2;
+  float m = -INFINITY;
+  for (int w = tid; w < splits; w += kD) m = fmaxf(m, ml[static_cast<int64_t>(w) * kSlab]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (tid % 32 == 0) top[tid / 32] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kD / 32; ++i) m = fmaxf(m, top[i]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int w = group; w < splits; w += 8) {
+    const int64_t at = static_cast<int64_t>(w) * kSlab;
+    const float2 s = *reinterpret_cast<const float2*>(ml + at);
+    const float4 x = *reinterpret_cast<const float4*>(src + at + r * kD + c);
+    const float4 y = *reinterpret_cast<const float4*>(src + at + r * kD + c + 4);
+    const float f = ex2((s.x - base) * to_log2);
+    l = fmaf(f, s.y, l);
+    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = fmaf(f, v[e], o[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) part[group][c + e] = o[e];
+  if (tid % kCh == 0) part[group][kD] = l;
+  __syncthreads();
+  if (group == 0 && c < p.head_dim) {
+    l = part[0][kD];
+#pragma unroll
+    for (int g = 1; g < 8; ++g) {
+      l += part[g][kD];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] += part[g][c + e];
+    }
+    store_row<kBf16>(p, bh / p.kv_heads, bh % p.kv_heads, row, c, o, l);
+  }
 }
 
 // Few keys, many rows: the CTA keeps K and V of its key head in shared memory
@@ -839,17 +913,9 @@ int allow_smem(const void* kernel, int bytes, bool wide_cluster, std::atomic<uin
   return kOk;
 }
 
-// CTAs that share an item's keys: a power of two up to `most`, while there
-// are SMs for them (per_sm CTAs each) and two key tiles for every one.
-int key_splits(int64_t items, int key_tiles, int per_sm, int most) {
-  int n = 1;
-  while (n < most && items * n * 2 <= static_cast<int64_t>(per_sm) * num_sms() && key_tiles >= 4 * n) n *= 2;
-  return n;
-}
-
 template <class... A>
 int launch_split(void (*kernel)(A...), int64_t items, int splits, int threads, int smem, cudaStream_t st,
-                 const A&... args) {
+                 bool cluster, const A&... args) {
   if (items * splits > 0x7fffffffLL) return kErrShape;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
@@ -858,7 +924,7 @@ int launch_split(void (*kernel)(A...), int64_t items, int splits, int threads, i
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
-  if (splits > 1) {
+  if (cluster && splits > 1) {
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = splits;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
@@ -880,8 +946,35 @@ int launch_few(const CrossParams& p, cudaStream_t st) {
   if (!make_kv_maps(p, kBf16 ? kBF16 : kF16, Cf::kKT, &mk, &mv, &share)) return kErrTma;
   const int row_tiles = (p.rows + Cf::kRows - 1) / Cf::kRows;
   const int64_t items = static_cast<int64_t>(row_tiles) * p.kv_heads * p.batch;
-  const int splits = key_splits(items, (p.sk + Cf::kKT - 1) / Cf::kKT, 200 * 1024 / Cf::kSmem, 16);
-  return launch_split(kernel, items, splits, Cf::kThreads, Cf::kSmem, st, mk, mv, p, share, row_tiles, splits);
+  static std::atomic<int> active[17];
+  const int key_tiles = (p.sk + Cf::kKT - 1) / Cf::kKT;
+  // Few items over long states: a cluster of 16 CTAs for each leaves SMs idle
+  // (and only 7 such clusters fit where a CTA takes most of an SM).  From 16 MB
+  // of K and V on the keys are split over all SMs, and a second launch adds the
+  // parts up out of a workspace: 8 items, 235 MB: 59 -> 44 us; 1 item, 34 MB: 31 -> 15 us.
+  const int64_t slots = static_cast<int64_t>(200 * 1024 / Cf::kSmem) * num_sms();
+  const int64_t kv_bytes = 4ll * p.sk * p.head_dim * p.kv_heads * p.batch;
+  if (items <= slots / 3 && kv_bytes >= (16ll << 20)) {
+    const int splits = static_cast<int>(std::min<int64_t>(slots / items, key_tiles / 4));
+    float* ws = nullptr;
+    const size_t bytes = static_cast<size_t>(items) * splits * Cf::kRows * (kD + 2) * 4;
+    if (splits > 1 && pool_alloc(reinterpret_cast<void**>(&ws), bytes, st) == cudaSuccess) {
+      int rc = launch_split(kernel, items, splits, Cf::kThreads, Cf::kSmem, st, false, mk, mv, p, share, row_tiles,
+                            splits, ws);
+      if (!rc) {
+        count_launches(1);
+        cross_join_kernel<kBf16, kD><<<static_cast<unsigned>(items * Cf::kRows), kD, 0, st>>>(
+            p, row_tiles, splits, ws, kBias ? kLog2e : p.scale_log2);
+        if (cudaGetLastError() != cudaSuccess) rc = kErrLaunch;
+      }
+      cudaFreeAsync(ws, st);
+      return rc;
+    }
+    cudaGetLastError();
+  }
+  const int splits = cluster_splits(kernel, Cf::kThreads, Cf::kSmem, items, key_tiles, 2, 16, active);
+  return launch_split(kernel, items, splits, Cf::kThreads, Cf::kSmem, st, true, mk, mv, p, share, row_tiles, splits,
+                      static_cast<float*>(nullptr));
 }
 
 template <bool kBf16, int kD, bool kBias>
@@ -892,11 +985,11 @@ int launch_rows_any(const CrossParams& p, cudaStream_t st) {
   if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), Cf::kSmem, false, ready)) return rc;
   const int row_tiles = static_cast<int>((static_cast<int64_t>(p.rows) + Cf::kRows - 1) / Cf::kRows);
   const int64_t items = static_cast<int64_t>(row_tiles) * p.kv_heads * p.batch;
-  const int per_sm = std::min(4, 200 * 1024 / Cf::kSmem);
-  const int splits = key_splits(items, (p.sk + Cf::kKT - 1) / Cf::kKT, per_sm, 8);
+  static std::atomic<int> active[17];
+  const int splits = cluster_splits(kernel, kThreads, Cf::kSmem, items, (p.sk + Cf::kKT - 1) / Cf::kKT, 4, 8, active);
   const bool wide = p.bias && (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0 && p.sk % 4 == 0 && p.bb % 4 == 0 &&
                     p.bh % 4 == 0 && p.bs % 4 == 0;
-  return launch_split(kernel, items, splits, kThreads, Cf::kSmem, st, p, row_tiles, splits, wide ? 4 : 1);
+  return launch_split(kernel, items, splits, kThreads, Cf::kSmem, st, true, p, row_tiles, splits, wide ? 4 : 1);
 }
 
 template <bool kBf16, int kD, bool kBias>

@@ -4,6 +4,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <initializer_list>
 
@@ -98,6 +99,38 @@ inline bool cross_kv_maps(const CrossParams& p) {
   for (int64_t x : {p.kb, p.ks, p.kh, p.vb, p.vs, p.vh})
     if (x >= kMost) return false;
   return p.sk > 0 && (p.sk == 1 || (p.ks != 0 && p.vs != 0));
+}
+
+// CTAs of a cluster that share an item's keys: the most, up to `most` (<= 16),
+// of which all items' clusters run at once and each has `tiles_each` key tiles.
+// (Clusters are placed within a GPC: 16 items of 8 are two waves, 15 fit.)
+// active: the kernel's own table of what fits, filled as it is asked.
+template <class K>
+int cluster_splits(K kernel, int threads, int smem, int64_t items, int key_tiles, int tiles_each, int most,
+                   std::atomic<int> (&active)[17]) {
+  for (int n = most; n > 1; --n) {
+    if (key_tiles < tiles_each * n || items * n > 2 * num_sms()) continue;
+    int fit = active[n].load();
+    if (!fit) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(n);
+      cfg.blockDim = dim3(threads);
+      cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = n;
+      at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg) != cudaSuccess || fit < 1) {
+        cudaGetLastError();
+        fit = -1;
+      }
+      active[n].store(fit);
+    }
+    if (items <= fit) return n;
+  }
+  return 1;
 }
 
 int launch_cross_mma(const CrossParams& p, int dtype, cudaStream_t st);

@@ -555,8 +555,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <bool kBf16, int kD, bool kMask>
-int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TcParams& prm,
-                   int64_t ctas, cudaStream_t st) {
+int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, TcParams& prm, int key_tiles,
+                   cudaStream_t st) {
   const auto kernel = cross_tc_kernel<kBf16, kD, kMask>;
   static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
   int dev = 0;
@@ -566,6 +566,14 @@ int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
       return kErrCuda;
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
+  static std::atomic<int> active[17];
+  prm.splits = cluster_splits(kernel, kThreads, Cfg<kD>::kSmem, prm.n_items, key_tiles, 4, 8, active);
+  // Short items: one CTA per SM that walks them, so that an item's first loads
+  // and S overlap the epilogue before it (4 x 8 heads x 5184 queries, 77 / 512 /
+  // 2048 keys, D = 64: 29 / 63 / 203 us against 37 / 71 / 208 with a CTA each).
+  // Long ones have a CTA each, dealt out as SMs come free (lengths differ).
+  int64_t ctas = static_cast<int64_t>(prm.n_items) * prm.splits;
+  if (prm.splits == 1 && key_tiles <= 16) ctas = std::min<int64_t>(ctas, num_sms());
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
@@ -585,14 +593,14 @@ int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
 }
 
 template <int kD>
-int launch_typed(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TcParams& prm,
-                 int dtype, int64_t ctas, cudaStream_t st) {
+int launch_typed(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, TcParams& prm, int dtype,
+                 int key_tiles, cudaStream_t st) {
   const bool mask = prm.c.key_mask != nullptr;  // (lengths alone need none of it)
   if (dtype == kBF16)
-    return mask ? launch_variant<true, kD, true>(mq, mk, mv, prm, ctas, st)
-                : launch_variant<true, kD, false>(mq, mk, mv, prm, ctas, st);
-  return mask ? launch_variant<false, kD, true>(mq, mk, mv, prm, ctas, st)
-              : launch_variant<false, kD, false>(mq, mk, mv, prm, ctas, st);
+    return mask ? launch_variant<true, kD, true>(mq, mk, mv, prm, key_tiles, st)
+                : launch_variant<true, kD, false>(mq, mk, mv, prm, key_tiles, st);
+  return mask ? launch_variant<false, kD, true>(mq, mk, mv, prm, key_tiles, st)
+              : launch_variant<false, kD, false>(mq, mk, mv, prm, key_tiles, st);
 }
 
 }  // namespace
@@ -620,22 +628,15 @@ int launch_cross_tc(const CrossParams& p, int dtype, cudaStream_t st) {
   if (heads * prm.items_x > 0x3fffffffLL) return kErrShape;
   prm.n_items = static_cast<int>(heads * prm.items_x);
   prm.splits = 1;
-  while (prm.splits < 8 && prm.n_items * 2ll * prm.splits <= num_sms() && key_tiles >= 8 * prm.splits) prm.splits *= 2;
-  int64_t ctas = static_cast<int64_t>(prm.n_items) * prm.splits;
-  // Short items: one CTA per SM that walks them, so that an item's first loads
-  // and S overlap the epilogue before it (4 x 8 heads x 5184 queries, 77 / 512 /
-  // 2048 keys, D = 64: 29 / 63 / 203 us against 37 / 71 / 208 with a CTA each).
-  // Long ones have a CTA each, dealt out as SMs come free (lengths differ).
-  if (prm.splits == 1 && key_tiles <= 16) ctas = std::min<int64_t>(ctas, num_sms());
   CUtensorMap mq, mk, mv;
   const TensorDim dq[3] = {{static_cast<int64_t>(p.kv_heads) * p.group, p.qh, nullptr}, {p.sq, p.qs, nullptr},
                            {p.batch, p.qb, &prm.qmul_b}};
   const int bq[3] = {p.group, prm.qpt, 1};
   if (!make_cross_map(&mq, p.q, dtype, p.head_dim, dq, bq) || !make_kv_maps(p, dtype, kKV, &mk, &mv, &prm.kv))
     return kErrTma;
-  if (p.head_dim <= 32) return launch_typed<32>(mq, mk, mv, prm, dtype, ctas, st);
-  if (p.head_dim <= 64) return launch_typed<64>(mq, mk, mv, prm, dtype, ctas, st);
-  return launch_typed<128>(mq, mk, mv, prm, dtype, ctas, st);
+  if (p.head_dim <= 32) return launch_typed<32>(mq, mk, mv, prm, dtype, key_tiles, st);
+  if (p.head_dim <= 64) return launch_typed<64>(mq, mk, mv, prm, dtype, key_tiles, st);
+  return launch_typed<128>(mq, mk, mv, prm, dtype, key_tiles, st);
 }
 
 }  // namespace s3

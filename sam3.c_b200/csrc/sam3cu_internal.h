@@ -1,6 +1,7 @@
 // sam3cu_internal.h - declarations shared by the library's translation units.
 #pragma once
 #include <cuda_runtime.h>
+#include <cstddef>
 #include <cstdint>
 
 namespace s3 {
@@ -26,6 +27,9 @@ struct EpiParams;
 int num_sms();
 // Add `delta` to the library-wide kernel launch counter; returns the new value.
 uint64_t count_launches(int64_t delta);
+// Stream-ordered memory for one call, from a pool of the library's own (freed
+// with cudaFreeAsync on the same stream).
+cudaError_t pool_alloc(void** p, size_t n, cudaStream_t st);
 int launch_q8_quantize(const float* src, void* blocks, int64_t n, cudaStream_t st);
 unsigned int dev_error_gemm();
 unsigned int dev_error_attn();

@@ -257,6 +257,24 @@ def test_long_and_many(cuda, b, sq, sk, hq, hkv, hd, dt):
     _check(*_make(b, sq, sk, hq, hkv, hd, dt, seed=12))
 
 
+@pytest.mark.parametrize("hd,dt", [(32, "f16"), (64, "bf16"), (128, "f16")])
+@pytest.mark.parametrize("sq,hq,hkv", [(1, 8, 2), (16, 1, 1), (5, 8, 1)])
+def test_few_rows_over_long_states(cuda, hd, dt, sq, hq, hkv):
+    """Keys split over all SMs and joined by a second launch: lengths (an empty
+    sequence among them), a mask that leaves whole splits out, a bias."""
+    import torch
+    sk = (24 << 20) // (4 * hd * hkv * 3) // 8 * 8 + 13
+    q, k, v = _make(3, sq, sk, hq, hkv, hd, dt, seed=sq)
+    _check(q, k, v)
+    o = _check(q, k, v, k_lens=torch.tensor([sk, 0, 700], dtype=torch.int32, device="cuda"))
+    assert bool((o[1] == 0).all())
+    mask = torch.zeros(3, sk, dtype=torch.bool, device="cuda")
+    mask[0, -1] = True
+    mask[1, 100:sk // 2: 3] = True
+    _check(q, k, v, key_mask=mask)
+    _check(q, k, v, bias=torch.randn(1, hq, 1, sk, device="cuda"))
+
+
 @pytest.mark.parametrize("sq", [1, 300])
 def test_offsets_past_32_bits(cuda, sq):
     """Rows that begin beyond 2^32 bytes into the states (and 2^31 elements)."""
@@ -281,25 +299,25 @@ def test_same_answer_every_time(cuda, sq):
         assert torch.equal(sam3cu.cross_attention(q, k, v), first)
 
 
-@pytest.mark.parametrize("sq", [2, 300])
-def test_captured_graphs_and_streams(cuda, sq):
+@pytest.mark.parametrize("sq,sk", [(2, 3000), (300, 3000), (2, 30000)])
+def test_captured_graphs_and_streams(cuda, sq, sk):
     """Two captured graphs replayed at once on two streams, with new inputs
     and new lengths, against plain calls."""
     import torch
     import sam3cu
     sets = []
     for i in range(2):
-        q, k, v = _make(2, sq, 3000, 4, 2, 64, "bf16", seed=20 + i)
-        lens = torch.tensor([3000, 5], dtype=torch.int32, device="cuda")
+        q, k, v = _make(2, sq, sk, 4, 2, 64, "bf16", seed=20 + i)
+        lens = torch.tensor([sk, 5], dtype=torch.int32, device="cuda")
         out, st, g = torch.empty_like(q), torch.cuda.Stream(), torch.cuda.CUDAGraph()
         torch.cuda.synchronize()
         with torch.cuda.graph(g, stream=st):
             sam3cu.cross_attention(q, k, v, k_lens=lens, out=out)
         sets.append((q, k, v, lens, out, st, g))
     for i, (q, k, v, lens, out, st, g) in enumerate(sets):
-        for x, y in zip((q, k, v), _make(2, sq, 3000, 4, 2, 64, "bf16", seed=30 + i)):
+        for x, y in zip((q, k, v), _make(2, sq, sk, 4, 2, 64, "bf16", seed=30 + i)):
             x.copy_(y)
-        lens.copy_(torch.tensor([17 + i, 2900], dtype=torch.int32))
+        lens.copy_(torch.tensor([17 + i, sk - 100], dtype=torch.int32))
     torch.cuda.synchronize()
     for _ in range(4):
         for q, k, v, lens, out, st, g in sets:
