@@ -906,8 +906,10 @@ int allow_smem(const void* kernel, int bytes, bool wide_cluster, std::atomic<uin
   if (dev >= 64 || !(ready.load() >> dev & 1)) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
         (wide_cluster &&
-         cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess))
+         cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)) {
+      cudaGetLastError();
       return kErrCuda;
+    }
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   return kOk;
@@ -932,7 +934,9 @@ int launch_split(void (*kernel)(A...), int64_t items, int splits, int threads, i
     cfg.numAttrs = 1;
   }
   count_launches(1);
-  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? kOk : kErrLaunch;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess) return kOk;
+  cudaGetLastError();  // the next call's own check must not see it
+  return kErrLaunch;
 }
 
 template <bool kBf16, int kD, bool kBias>
@@ -1037,6 +1041,18 @@ int launch_cross_mma(const CrossParams& p, int dtype, cudaStream_t st) {
 
 using namespace s3;
 
+namespace {
+
+// A first call sets kernels' attributes and makes the pool; while another or
+// this thread captures in the strict mode such calls end the capture.
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+}  // namespace
+
 extern "C" int sam3cu_cross_attention(const struct sam3cu_cross_attention_args* a, void* stream) {
   if (!a) return SAM3CU_EINVAL;
   if (a->dtype != SAM3CU_BF16 && a->dtype != SAM3CU_F16) return SAM3CU_EDTYPE;
@@ -1098,6 +1114,7 @@ extern "C" int sam3cu_cross_attention(const struct sam3cu_cross_attention_args* 
     p.bs = a->bias_strides[2];
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const RelaxedCapture relaxed;
   // Which kernel: tcgen05 for many rows, except over few keys where heads are
   // small or the whole call is (4 x 8 heads x 5184 queries, D = 32: 77 keys 17
   // us kept in shared memory, 25 us on tcgen05, 256 keys 36 and 31; D = 64, 77

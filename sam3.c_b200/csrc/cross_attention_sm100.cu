@@ -562,8 +562,10 @@ int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return kErrCuda;
   if (dev >= 64 || !(ready.load() >> dev & 1)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<kD>::kSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<kD>::kSmem) != cudaSuccess) {
+      cudaGetLastError();
       return kErrCuda;
+    }
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   static std::atomic<int> active[17];
@@ -589,7 +591,9 @@ int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
     cfg.numAttrs = 1;
   }
   count_launches(1);
-  return cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, prm) == cudaSuccess ? kOk : kErrLaunch;
+  if (cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, prm) == cudaSuccess) return kOk;
+  cudaGetLastError();  // the next call's own check must not see it
+  return kErrLaunch;
 }
 
 template <int kD>

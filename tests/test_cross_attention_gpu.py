@@ -230,10 +230,12 @@ def test_scale(cuda):
     _check(q, k, v, scale=1e-3)
 
 
-def test_no_keys(cuda):
+@pytest.mark.parametrize("sq", [1, 5, 300])
+def test_no_keys(cuda, sq):
     import sam3cu
-    q, k, v = _make(2, 5, 0, 2, 2, 64, "bf16")
+    q, k, v = _make(2, sq, 0, 2, 2, 64, "bf16")
     assert bool((sam3cu.cross_attention(q, k, v) == 0).all())
+    assert sam3cu.cross_attention(q[:, :0], k, v).shape == (2, 0, 2, 64)
 
 
 def test_nan_query_stays_in_its_row(cuda):
@@ -327,6 +329,65 @@ def test_captured_graphs_and_streams(cuda, sq, sk):
     for q, k, v, lens, out, st, g in sets:
         assert torch.equal(out, sam3cu.cross_attention(q, k, v, k_lens=lens))
         _check(q, k, v, k_lens=lens)
+
+
+def test_first_call_may_be_captured():
+    """In a fresh process the first call of each kernel is one that a graph
+    captures (each takes its attributes, tables and pool on first use)."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import sys
+sys.path.insert(0, %r)
+import torch, sam3cu
+sam3cu.init(0)
+f = sam3cu.RopeFreqs(64)
+for sq, sk in ((1, 200), (1, 40000), (40, 300), (300, 77), (300, 2000)):
+    q = torch.randn(1, sq, 4, 64, device="cuda").bfloat16()
+    k = torch.randn(1, sk, 4, 64, device="cuda").bfloat16()
+    v = torch.randn(1, sk, 4, 64, device="cuda").bfloat16()
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        y = sam3cu.cross_attention(sam3cu.rope_pos(q, f), k, v)
+    g.replay()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, sam3cu.cross_attention(sam3cu.rope_pos(q, f), k, v)), (sq, sk)
+    assert sam3cu.device_error() == 0
+print("done")
+""" % os.path.join(root, "sam3.c_b200")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
+
+
+def test_two_threads(cuda):
+    """Calls from two host threads, each on a stream of its own."""
+    import threading
+
+    import torch
+    import sam3cu
+    sets = [_make(1, sq, 3000, 4, 2, 64, "bf16", seed=sq) for sq in (2, 300)]
+    want = [sam3cu.cross_attention(*s) for s in sets]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        torch.cuda.set_device(0)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got = sam3cu.cross_attention(*sets[i])
+            torch.cuda.current_stream().synchronize()
+            if not torch.equal(got, want[i]):
+                wrong.append(i)
+    threads = [threading.Thread(target=work, args=(i % 2,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_wrapper_refusals(cuda):
