@@ -94,7 +94,9 @@ struct RowsCfg {
   static constexpr int kBiasPitch = kKT + 4;           // floats of a bias row
   static constexpr int kBiasBytes = kBias ? kRows * kBiasPitch * 4 : 0;
   static constexpr int kStageBytes = 2 * kTileBytes + kBiasBytes;
-  static constexpr int kStages = kD == 32 && !kBias ? 4 : kD == 128 && !kBias ? 2 : 3;
+  // (with a bias two, so that more CTAs fit: 201 x 5184 x 8 heads of 32, batch 4:
+  // 53 us, three stages 66)
+  static constexpr int kStages = kBias ? 2 : kD == 32 ? 4 : kD == 128 ? 2 : 3;
   static constexpr int kQBytes = kRows * kD * 2;
   static constexpr int kPitch = kD + 4;                // floats of a partial row
   static constexpr int kPartBytes = kRows * kPitch * 4;  // over the ring
@@ -986,11 +988,11 @@ int launch_rows_any(const CrossParams& p, cudaStream_t st) {
   using Cf = RowsCfg<kD, kBias>;
   static std::atomic<uint64_t> ready{0};
   const auto kernel = cross_rows_kernel<kBf16, kD, kBias>;
-  if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), Cf::kSmem, false, ready)) return rc;
+  if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), Cf::kSmem, true, ready)) return rc;
   const int row_tiles = static_cast<int>((static_cast<int64_t>(p.rows) + Cf::kRows - 1) / Cf::kRows);
   const int64_t items = static_cast<int64_t>(row_tiles) * p.kv_heads * p.batch;
   static std::atomic<int> active[17];
-  const int splits = cluster_splits(kernel, kThreads, Cf::kSmem, items, (p.sk + Cf::kKT - 1) / Cf::kKT, 4, 8, active);
+  const int splits = cluster_splits(kernel, kThreads, Cf::kSmem, items, (p.sk + Cf::kKT - 1) / Cf::kKT, 8, 16, active);
   const bool wide = p.bias && (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0 && p.sk % 4 == 0 && p.bb % 4 == 0 &&
                     p.bh % 4 == 0 && p.bs % 4 == 0;
   return launch_split(kernel, items, splits, kThreads, Cf::kSmem, st, true, p, row_tiles, splits, wide ? 4 : 1);

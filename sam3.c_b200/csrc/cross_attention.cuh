@@ -109,7 +109,7 @@ template <class K>
 int cluster_splits(K kernel, int threads, int smem, int64_t items, int key_tiles, int tiles_each, int most,
                    std::atomic<int> (&active)[17]) {
   for (int n = most; n > 1; --n) {
-    if (key_tiles < tiles_each * n || items * n > 2 * num_sms()) continue;
+    if (key_tiles < tiles_each * n || items * n > 4 * num_sms()) continue;
     int fit = active[n].load();
     if (!fit) {
       cudaLaunchConfig_t cfg = {};

@@ -566,6 +566,9 @@ int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
       cudaGetLastError();
       return kErrCuda;
     }
+    // a build that spills is not run: see the softmax's registers
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess || fa.localSizeBytes != 0) return kErrLaunch;
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   static std::atomic<int> active[17];
