@@ -313,12 +313,25 @@ class RopeFreqs:
         return self._c.amplitude
 
 
+# torch's own functions, looked up once: an import statement or a Stream object
+# in every call costs as much as the launch
+_cuda_device = _cuda_stream = _torch_empty_like = _torch_contiguous = _torch_int64 = None
+
+
+def _bind():
+    global _cuda_device, _cuda_stream, _torch_empty_like, _torch_contiguous, _torch_int64
+    import torch
+    _torch_empty_like, _torch_contiguous, _torch_int64 = torch.empty_like, torch.contiguous_format, torch.int64
+    _cuda_device, _cuda_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _here(x):
     """The device index of x, which must be the current device's: the calls
     launch there, on its current stream."""
-    import torch
     dev = x.get_device()
-    if dev < 0 or dev != torch._C._cuda_getDevice():
+    if dev >= 0 and _cuda_device is None:
+        _bind()
+    if dev < 0 or dev != _cuda_device():
         raise ValueError(f"tensors must be on the current CUDA device, not on {x.device}")
     return dev
 
@@ -327,17 +340,6 @@ def _like(t, x, shape, dev, what):
     if t.dtype != x.dtype or t.get_device() != dev or t.shape != shape or (t.stride(-1) != 1 and shape[-1] > 1):
         raise ValueError(f"{what} must be a {x.dtype} tensor of shape {tuple(shape)} on {x.device} with contiguous "
                          f"last dimension")
-
-
-def _empty_like(x):
-    import torch
-    return torch.empty_like(x, memory_format=torch.contiguous_format)
-
-
-def _raw_stream(dev):
-    """The current stream's handle (the public form makes a Stream object, 3 us a call)."""
-    import torch
-    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _head_param(t, head_dim, dev, what):
@@ -355,7 +357,7 @@ def _head_view(x, out, q, dev, gamma, beta, what):
         raise ValueError("q and k must be [batch, seq, heads, head_dim], alike but in heads")
     _like(x, q, shape, dev, what)
     if out is None:
-        out = _empty_like(x)
+        out = _torch_empty_like(x, memory_format=_torch_contiguous)
     else:
         _like(out, q, shape, dev, "the output of " + what)
     xb, xs, xh, _ = x.stride()
@@ -366,11 +368,10 @@ def _head_view(x, out, q, dev, gamma, beta, what):
 
 def _positions(positions, batch, seq, dev):
     """Pointer and batch stride of int64 positions [seq], [1, seq] or [batch, seq]."""
-    import torch
     if positions is None:
         return None, 0
     shape = positions.shape
-    if positions.dtype != torch.int64 or positions.get_device() != dev or len(shape) not in (1, 2) \
+    if positions.dtype != _torch_int64 or positions.get_device() != dev or len(shape) not in (1, 2) \
             or shape[-1] != seq or (seq > 1 and positions.stride(-1) != 1):
         raise ValueError("positions must be int64 [batch, seq] or [seq] on the inputs' device, contiguous along seq")
     if len(shape) == 1 or shape[0] == 1:
@@ -393,7 +394,7 @@ def rope_pos(q, freqs: RopeFreqs, positions=None, start: int = 0, k=None, out=No
     batch, seq, _, head_dim = q.shape
     pos, stride = _positions(positions, batch, seq, dev)
     check(lib().sam3cu_rope_pos(qv, kv, dtype_code(q), batch, seq, head_dim, pos, stride, start, freqs.ptr,
-                                _raw_stream(dev)), "sam3cu_rope_pos")
+                                _cuda_stream(dev)), "sam3cu_rope_pos")
     return out if k is None else (out, k_out)
 
 
@@ -414,7 +415,7 @@ def qk_norm_rope(q, k, q_gamma=None, k_gamma=None, q_beta=None, k_beta=None, nor
         table = freqs.ptr
         pos, stride = _positions(positions, batch, seq, dev)
     check(lib().sam3cu_qk_norm_rope(qv, kv, dtype_code(q), batch, seq, head_dim, norm, eps, pos, stride, start, table,
-                                    _raw_stream(dev)), "sam3cu_qk_norm_rope")
+                                    _cuda_stream(dev)), "sam3cu_qk_norm_rope")
     return out if k is None else (out, k_out)
 
 
@@ -428,7 +429,6 @@ def cross_attention(q, k, v, k_lens=None, key_mask=None, bias=None, scale: float
     added to the scaled scores, of a shape that broadcasts to [batch, q_heads,
     sq, sk] (its last dimension sk); scale 0: 1/sqrt(head_dim).  A query left
     without keys gives zeros."""
-    import torch
     dev = _here(q)
     qshape, kshape = q.shape, k.shape
     if len(qshape) != 4 or len(kshape) != 4 or kshape[0] != qshape[0] or kshape[3] != qshape[3]:
@@ -439,10 +439,12 @@ def cross_attention(q, k, v, k_lens=None, key_mask=None, bias=None, scale: float
     _like(k, q, kshape, dev, "k")
     _like(v, q, kshape, dev, "v")
     if out is None:
-        out = _empty_like(q)
+        out = _torch_empty_like(q, memory_format=_torch_contiguous)
     else:
         _like(out, q, qshape, dev, "out")
     lens = mask = bptr = mask_stride = bb = bh = bq = 0
+    if k_lens is not None or key_mask is not None or bias is not None:
+        import torch
     if k_lens is not None:
         if k_lens.dtype != torch.int32 or k_lens.shape != (batch,) or k_lens.get_device() != dev \
                 or not k_lens.is_contiguous():
@@ -472,7 +474,7 @@ def cross_attention(q, k, v, k_lens=None, key_mask=None, bias=None, scale: float
     args = _CROSS_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qb, qs, qh, kb, ks, kh, vb, vs,
                             vh, ob, os_, oh, dtype_code(q), batch, sq, sk, q_heads, kv_heads, head_dim, scale, lens,
                             mask, mask_stride, bptr, bb, bh, bq)
-    check(lib().sam3cu_cross_attention(args, _raw_stream(dev)), "sam3cu_cross_attention")
+    check(lib().sam3cu_cross_attention(args, _cuda_stream(dev)), "sam3cu_cross_attention")
     return out
 
 
