@@ -1,24 +1,32 @@
 // cross_attention.cu - attention of queries over states of another length,
-// for few query rows or few keys (and the entry point of both kernels).
+// for few query rows, few keys or a bias (and the entry point, which sends the
+// rest to cross_attention_sm100.cu).
 //
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(s_j - max s),
 //   s_j = scale q.k_j + bias_j, over the keys that count
 //
-// One pass over the keys with the running maximum and sum of each row.  With
-// few rows to a key head the call reads K and V once and does little with
-// them, with few keys it reads Q and writes O: HBM bounds both, and what
-// matters is that enough loads are under way on every SM.  So:
-//   * a warp computes 16 rows with m16n8k16 MMAs (fp32 accumulate); K and V
-//     tiles come by 16-byte cp.async through a ring in shared memory;
-//   * up to 16 rows: every warp of the CTA walks key tiles of its own (no
-//     CTA barrier in the loop); more: the CTA's four warps take 16 rows each
-//     of 64 and share the tiles;
-//   * where that leaves SMs idle the keys are split over the CTAs of a
-//     cluster, which exchange (max, sum, partial O) through distributed
-//     shared memory: no workspace, no second launch, a fixed order of sums.
-// A key that does not count is not read at all: its K and V rows are
-// zero-filled by the copy (so what they hold cannot reach the sums as 0 * NaN)
-// and its score is -inf.
+// One pass over the keys with the running maximum and sum of each row; a warp
+// computes 16 rows with m16n8k16 MMAs (fp32 accumulate).  With few rows to a
+// key head a call reads K and V once and does little with them, with few keys
+// it reads Q and writes O: HBM bounds both, and what matters is that enough
+// loads are under way on every SM.  Three kernels:
+//   * cross_few_kernel, up to 16 rows of a key head: one warp fetches 128-key
+//     tiles by TMA, four compute.  2 x 4 key heads of 128 under 32, one query,
+//     65521 keys with lengths: 44 us, 0.80 of the measured copy rate;
+//   * cross_keep_kernel, few keys: K and V stay in shared memory, the warps
+//     walk the rows.  4 x 8 heads of 32, 5184 rows, 77 keys: 17 us;
+//   * cross_rows_kernel, the rest: 64 rows to a CTA, 16 to a warp, K, V and the
+//     bias through a ring of cp.async.  4 x 8 heads of 32, 201 rows, 5184 keys
+//     with a bias: 53 us, 0.45 of the copy rate for reading the bias once (the
+//     scores' arithmetic on the legacy tensor path and the exponentials bound
+//     it).
+// Where that leaves SMs idle the keys are split over the CTAs of a cluster,
+// which exchange (max, sum, partial O) through distributed shared memory: no
+// workspace, no second launch, a fixed order of sums.  Few items over long
+// states need more CTAs than a cluster has: those leave their parts in a
+// workspace, which cross_join_kernel adds up, in a fixed order too.
+// A key that does not count is never multiplied: its score is -inf, and its V
+// row becomes zeros (so what it holds cannot reach the sums as 0 * NaN).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -45,7 +53,7 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaxKeep = 2048;  // keys that cross_keep_kernel may hold
+constexpr int kMaxKeep = 256;  // keys that cross_keep_kernel may hold
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -591,6 +599,7 @@ __global__ void __launch_bounds__(FewCfg<kD>::kThreads)
               asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(sv + at(warp * 32 + lane, c)), "r"(0)
                            : "memory");
           }
+          fence_proxy_async_smem();  // before the next copy into this slot
           __syncwarp();
         }
         float s[4][4];
@@ -1023,7 +1032,7 @@ int launch_keep(const CrossParams& p, cudaStream_t st) {
 
 template <bool kBf16, int kD>
 int launch_rows(const CrossParams& p, cudaStream_t st) {
-  if (p.rows > 64 && p.sk <= 256 && KeepCfg<kD>::smem(p.sk) <= 100 * 1024)
+  if (p.rows > 64 && p.sk <= kMaxKeep && KeepCfg<kD>::smem(p.sk) <= 100 * 1024)
     return p.bias ? launch_keep<kBf16, kD, true>(p, st) : launch_keep<kBf16, kD, false>(p, st);
   if (p.rows <= 16 && cross_kv_maps(p))
     return p.bias ? launch_few<kBf16, kD, true>(p, st) : launch_few<kBf16, kD, false>(p, st);

@@ -1,4 +1,4 @@
-// cross_attention.cuh - what the two cross-attention kernels share: the
+// cross_attention.cuh - what the cross-attention kernels share: the
 // checked arguments and how rows, heads and keys are numbered.
 #pragma once
 #include <cuda.h>
