@@ -322,7 +322,8 @@ def _bind():
     global _cuda_device, _cuda_stream, _torch_empty_like, _torch_contiguous, _torch_int64
     import torch
     _torch_empty_like, _torch_contiguous, _torch_int64 = torch.empty_like, torch.contiguous_format, torch.int64
-    _cuda_device, _cuda_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    _cuda_stream = torch._C._cuda_getCurrentRawStream
+    _cuda_device = torch._C._cuda_getDevice  # last: another thread looks at it alone
 
 
 def _here(x):
