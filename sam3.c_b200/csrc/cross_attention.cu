@@ -99,8 +99,7 @@ struct RowsCfg {
   static constexpr int kKT = 64;                       // keys of a tile
   static constexpr int kChunks = kD / 8;               // 16-byte pieces of a row
   static constexpr int kTileBytes = kKT * kD * 2;      // K or V
-  static constexpr int kBiasPitch = kKT + 4;           // floats of a bias row
-  static constexpr int kBiasBytes = kBias ? kRows * kBiasPitch * 4 : 0;
+  static constexpr int kBiasBytes = kBias ? kRows * kKT * 4 : 0;
   static constexpr int kStageBytes = 2 * kTileBytes + kBiasBytes;
   // (with a bias two, so that more CTAs fit: 201 x 5184 x 8 heads of 32, batch 4:
   // 53 us, three stages 66)
@@ -352,13 +351,15 @@ __global__ void __launch_bounds__(kThreads) cross_rows_kernel(const __grid_const
     }
     if constexpr (kBias) {
       // the tile's bias, a row by 16 lanes of 4 keys; bias_step 4: its rows
-      // start on 16 bytes, 1: key by key
+      // start on 16 bytes, 1: key by key.  Piece c of row r lies at c ^ 2 (r % 4),
+      // so that the 8-byte reads of four rows touch all banks (rows with 4
+      // floats between them: two reads to a bank, 53 us on the case above).
       const uint32_t sb = sv + Cf::kTileBytes;
 #pragma unroll 2
       for (int r = tid / 16; r < Cf::kRows; r += kThreads / 16) {
         const float* src = brow[kBias ? r : 0];
-        const int c = tid % 16 * 4, key = t * kKT + c;
-        const uint32_t dst = sb + (r * Cf::kBiasPitch + c) * 4;
+        const int key = t * kKT + tid % 16 * 4;
+        const uint32_t dst = sb + r * kKT * 4 + ((tid % 16) ^ (2 * (r & 3))) * 16;
         if (bias_step == 4) {
           cp_async16(dst, src + (key < len ? key : 0), key < len);  // (sk is a multiple of 4)
         } else {
@@ -420,12 +421,12 @@ __global__ void __launch_bounds__(kThreads) cross_rows_kernel(const __grid_const
     if constexpr (kBias) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t sb = sv + Cf::kTileBytes +
-                            ((warp * 16 + (lane >> 2) + 8 * h) * Cf::kBiasPitch + (lane & 3) * 2) * 4;
+        const uint32_t sb = sv + Cf::kTileBytes + (warp * 16 + (lane >> 2) + 8 * h) * kKT * 4 + (lane & 3) * 8;
+        const uint32_t swz = (lane >> 2 & 3) * 32;
 #pragma unroll
         for (int j = 0; j < kKT / 8; ++j) {
           float x, y;
-          asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(x), "=f"(y) : "r"(sb + j * 32) : "memory");
+          asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(x), "=f"(y) : "r"(sb + ((j * 32) ^ swz)) : "memory");
           f2unpack(ffma2(f2pack(s[j][2 * h], s[j][2 * h + 1]), f2pack(p.scale, p.scale), f2pack(x, y)), s[j][2 * h],
                    s[j][2 * h + 1]);
         }
