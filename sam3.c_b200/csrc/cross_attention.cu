@@ -17,9 +17,8 @@
 //     walk the rows.  4 x 8 heads of 32, 5184 rows, 77 keys: 17 us;
 //   * cross_rows_kernel, the rest: 64 rows to a CTA, 16 to a warp, K, V and the
 //     bias through a ring of cp.async.  4 x 8 heads of 32, 201 rows, 5184 keys
-//     with a bias: 53 us, 0.45 of the copy rate for reading the bias once (the
-//     scores' arithmetic on the legacy tensor path and the exponentials bound
-//     it).
+//     with a bias: 50 us, 0.48 of the copy rate for reading the bias once
+//     (shared memory bounds it: every 16 rows read all of K and V there).
 // Where that leaves SMs idle the keys are split over the CTAs of a cluster,
 // which exchange (max, sum, partial O) through distributed shared memory: no
 // workspace, no second launch, a fixed order of sums.  Few items over long
@@ -102,7 +101,7 @@ struct RowsCfg {
   static constexpr int kBiasBytes = kBias ? kRows * kKT * 4 : 0;
   static constexpr int kStageBytes = 2 * kTileBytes + kBiasBytes;
   // (with a bias two, so that more CTAs fit: 201 x 5184 x 8 heads of 32, batch 4:
-  // 53 us, three stages 66)
+  // three stages 66 us, two 53, and 50 since the bias rows are permuted)
   static constexpr int kStages = kBias ? 2 : kD == 32 ? 4 : kD == 128 ? 2 : 3;
   static constexpr int kQBytes = kRows * kD * 2;
   static constexpr int kPitch = kD + 4;                // floats of a partial row
@@ -353,7 +352,8 @@ __global__ void __launch_bounds__(kThreads) cross_rows_kernel(const __grid_const
       // the tile's bias, a row by 16 lanes of 4 keys; bias_step 4: its rows
       // start on 16 bytes, 1: key by key.  Piece c of row r lies at c ^ 2 (r % 4),
       // so that the 8-byte reads of four rows touch all banks (rows with 4
-      // floats between them: two reads to a bank, 53 us on the case above).
+      // floats between them: two reads to a bank, 53 us instead of 50 for the
+      // case at kStages).
       const uint32_t sb = sv + Cf::kTileBytes;
 #pragma unroll 2
       for (int r = tid / 16; r < Cf::kRows; r += kThreads / 16) {
