@@ -109,6 +109,30 @@ __device__ __forceinline__ void st_piece(void* p, int64_t i, const uint64_t* h) 
   *reinterpret_cast<uint4*>(static_cast<char*>(p) + i * (T == kF32 ? 4 : 2)) = w;
 }
 
+// Element of the head that piece i (of kp elements) of lane `slot` starts at,
+// where the pieces are spread over the `slots` lanes of a head.
+__host__ __device__ constexpr int spread_piece(int kp, int slots, int slot, int i) {
+  return kp * slot + i * kp * slots;
+}
+// A group has as many lanes as the next power of two; those behind the head's
+// hold no piece of it.  Their offsets are those of the first lanes' next
+// pieces, so they must not store what the lanes of a group share.
+__host__ __device__ constexpr bool holds_piece(int slots, int slot) { return slot < slots; }
+// Whether the lanes that store pieces store each element of a head once.
+constexpr bool one_writer_each(int kp) {
+  for (int slots = 1; slots <= kMaxDim / 16; ++slots) {
+    int lanes = 1;
+    while (lanes < slots) lanes *= 2;
+    int writers[2 * kMaxDim] = {};
+    for (int slot = 0; slot < lanes; ++slot)
+      for (int e = 0; holds_piece(slots, slot) && e < 16; ++e) ++writers[spread_piece(kp, slots, slot, e / kp) + e % kp];
+    for (int e = 0; e < 2 * kMaxDim; ++e)
+      if (writers[e] != (e < 16 * slots)) return false;
+  }
+  return true;
+}
+static_assert(one_writer_each(Raw<kF32>::kP) && one_writer_each(Raw<kBF16>::kP), "two lanes store one element");
+
 // Heads of a lane under way: 32 bytes each, 64 for F32.
 template <int T, int kRot>
 constexpr int ring_depth() {
@@ -200,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, kRot == 2 ? 2 : kVecCtas) rotary_vec
     } else if (half) {  // behind the rotated part
       off[i] = 16 * rslots + R::kP * (slot - rslots) + i * R::kP * (slots - rslots);
     } else {
-      off[i] = R::kP * slot + i * R::kP * slots;
+      off[i] = spread_piece(R::kP, slots, slot, i);
     }
     turned = turned || (kRot && off[i] < 2 * p.f.n_pairs);
   }
@@ -209,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, kRot == 2 ? 2 : kVecCtas) rotary_vec
   const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / kG) + tid / kG;
   const int64_t token = p.slices > 1 ? item / p.slices : item;
   const int slice = p.slices > 1 ? static_cast<int>(item - token * p.slices) : 0;
-  const bool have = slot < slots && token < p.tokens;
+  const bool have = holds_piece(slots, slot) && token < p.tokens;
   const int h0 = slice * p.per_slice;
   const int h1 = min(p.heads, h0 + p.per_slice);
   int64_t b, s;
@@ -297,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, kRot == 2 ? 2 : kVecCtas) rotary_vec
         float sum = a + c;
 #pragma unroll
         for (int o = kG / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float mean = slot < slots ? -sum * n : 0.f;
+        const float mean = holds_piece(slots, slot) ? -sum * n : 0.f;
         const uint64_t m2 = f2pack(mean, mean);
 #pragma unroll
         for (int i = 0; i < 8; ++i) h2[i] = fadd2(h2[i], m2);
@@ -312,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, kRot == 2 ? 2 : kVecCtas) rotary_vec
       for (int o = kG / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
       const float inv = rsqrtf(fmaf(sq, n, p.eps));
       const uint64_t i2 = f2pack(inv, inv);
-      if (slot < slots) {
+      if (holds_piece(slots, slot)) {
         const float(&af)[2][kNorm ? 16 * kG : 1] = affine[kNorm && k ? 1 : 0];
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
@@ -336,8 +360,10 @@ __global__ void __launch_bounds__(kThreads, kRot == 2 ? 2 : kVecCtas) rotary_vec
       for (int i = 0; i < 8; ++i) {
         f2unpack(h2[i], f[2 * i], f[2 * i + 1]);
         const int e = off[2 * i / R::kP] + 2 * i % R::kP;
-        mine_h[e + (e >> 3)] = f[2 * i];
-        mine_h[e + 1 + (e >> 3)] = f[2 * i + 1];
+        if (holds_piece(slots, slot)) {
+          mine_h[e + (e >> 3)] = f[2 * i];
+          mine_h[e + 1 + (e >> 3)] = f[2 * i + 1];
+        }
       }
       __syncwarp();
       if (turns) {

@@ -270,3 +270,14 @@ def test_captured_and_other_stream(cuda):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, sam3cu.rope_pos(q, f, pos))
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("norm", [0, 2])
+@pytest.mark.parametrize("hd", [48, 80, 96, 112, 144, 160, 176, 192, 208, 224, 240])
+def test_exchange_with_lanes_left_over(cuda, dt, norm, hd):
+    """Halves that are not multiples of 8 elements go through shared memory;
+    where head_dim / 16 is no power of two some lanes of a group hold no part
+    of the head and must leave its words to the lanes that do."""
+    _check((3, 41, 9, hd), 5, dt, hd - 2, True, norm=norm, seed=hd)
+    _check((3, 41, 9, hd), 5, dt, hd // 2 + 2 - hd // 2 % 2, True, norm=norm, seed=hd, inplace=True)
