@@ -300,8 +300,12 @@ class RopeFreqs:
                           high_freq, amplitude)
         self._c = _RopeFreqs()
         check(lib().sam3cu_rope_freqs_init(C.byref(cfg), C.byref(self._c)), "sam3cu_rope_freqs_init")
-        self.ptr = C.addressof(self._c)
         self.rot_dim = rot_dim
+
+    @property
+    def ptr(self) -> int:
+        """Address of the table (asked each time: a copy has a table of its own)."""
+        return C.addressof(self._c)
 
     @property
     def turns(self) -> np.ndarray:

@@ -159,3 +159,21 @@ def test_wrappers_want_cuda_tensors():
         sam3cu.rope_pos(x, sam3cu.RopeFreqs(64))
     with pytest.raises(ValueError):
         sam3cu.qk_norm_rope(x, None)
+
+
+@pytest.mark.parametrize("how", ["copy", "deepcopy", "pickle"])
+def test_copied_frequencies_point_to_their_own_table(how):
+    """A copied or unpickled table (a module's deepcopy, another process) hands
+    the library its own memory, not that of the object it was made from."""
+    import copy
+    import pickle
+    f = sam3cu.RopeFreqs(64, theta=500.0)
+    g = {"copy": copy.copy, "deepcopy": copy.deepcopy, "pickle": lambda x: pickle.loads(pickle.dumps(x))}[how](f)
+    want = f.turns
+    assert g.rot_dim == 64 and np.array_equal(g.turns, want)
+    assert g.ptr == C.addressof(g._c)
+    if how != "copy":
+        assert g.ptr != f.ptr
+    del f
+    assert sam3cu._RopeFreqs.from_address(g.ptr).n_pairs == 32
+    assert np.array_equal(np.array(sam3cu._RopeFreqs.from_address(g.ptr).turns[:32]), want)
