@@ -582,7 +582,7 @@ enum sam3cu_rope_layout {
  * How the angles theta^(-2i/rot_dim) are scaled for contexts of `factor`
  * times the trained length:
  *   LINEAR  every angle divided by factor
- *   NTK     theta * factor^(rot_dim/(rot_dim-2)) in place of theta
+ *   NTK     theta * factor^(rot_dim/(rot_dim-2)) in place of theta (finite)
  *   YARN    pairs that turn more than beta_fast times over trained_len keep
  *           their angle, those that turn less than beta_slow times have it
  *           divided by factor, a ramp over the pair index between them;
@@ -608,7 +608,7 @@ struct sam3cu_rope_config {
 	double trained_len;   /* > 0, YARN and BANDS */
 	double beta_fast, beta_slow;    /* YARN (32, 1): fast > slow > 0 */
 	double low_freq, high_freq;     /* BANDS (1, 4): high > low > 0 */
-	double amplitude;     /* 0: 1, or what YARN says */
+	double amplitude;     /* 0: 1, or what YARN says; within F32 */
 };
 
 #define SAM3CU_ROPE_MAX_PAIRS 128

@@ -664,7 +664,7 @@ int sam3cu_rope_freqs_init(const struct sam3cu_rope_config* c, struct sam3cu_rop
   if (c->scaling < SAM3CU_ROPE_SCALE_NONE || c->scaling > SAM3CU_ROPE_SCALE_BANDS) return SAM3CU_EINVAL;
   // negated comparisons, so that a NaN is refused too
   if (!(c->theta > 1.0) || std::isinf(c->theta)) return SAM3CU_EINVAL;
-  if (!(c->amplitude >= 0.0) || std::isinf(c->amplitude)) return SAM3CU_EINVAL;
+  if (!(c->amplitude >= 0.0) || std::isinf(static_cast<float>(c->amplitude))) return SAM3CU_EINVAL;
   const bool yarn = c->scaling == SAM3CU_ROPE_SCALE_YARN, bands = c->scaling == SAM3CU_ROPE_SCALE_BANDS;
   if (c->scaling != SAM3CU_ROPE_SCALE_NONE && (!(c->factor >= 1.0) || std::isinf(c->factor))) return SAM3CU_EINVAL;
   if ((yarn || bands) && (!(c->trained_len > 0.0) || std::isinf(c->trained_len))) return SAM3CU_EINVAL;
@@ -676,6 +676,7 @@ int sam3cu_rope_freqs_init(const struct sam3cu_rope_config* c, struct sam3cu_rop
   const int rot = c->rot_dim;
   double theta = c->theta;
   if (c->scaling == SAM3CU_ROPE_SCALE_NTK && rot > 2) theta *= std::pow(c->factor, rot / (rot - 2.0));
+  if (std::isinf(theta)) return SAM3CU_EINVAL;
   memset(out, 0, sizeof(*out));
   out->n_pairs = rot / 2;
   out->layout = c->layout;

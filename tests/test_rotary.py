@@ -177,3 +177,18 @@ def test_copied_frequencies_point_to_their_own_table(how):
     del f
     assert sam3cu._RopeFreqs.from_address(g.ptr).n_pairs == 32
     assert np.array_equal(np.array(sam3cu._RopeFreqs.from_address(g.ptr).turns[:32]), want)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(amplitude=1e39), dict(scaling=sam3cu.ROPE_SCALE_NTK, factor=1e200, rot_dim=4),
+    dict(scaling=sam3cu.ROPE_SCALE_NTK, factor=1e10, theta=1e300)])
+def test_tables_that_do_not_fit_are_refused(bad):
+    """An amplitude past F32, a base past F64: the table would hold
+    infinities, or zeros in place of every frequency but the first."""
+    with pytest.raises(sam3cu.Sam3cuError):
+        sam3cu.RopeFreqs(**{"rot_dim": 64, **bad})
+
+
+def test_largest_tables():
+    assert np.isfinite(sam3cu.RopeFreqs(64, amplitude=3e38).amplitude)
+    assert (sam3cu.RopeFreqs(64, scaling=sam3cu.ROPE_SCALE_NTK, factor=1e6, theta=1e300).turns > 0).all()
