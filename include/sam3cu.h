@@ -649,7 +649,8 @@ struct sam3cu_head_view {
  * Rotate the heads of q and k (k NULL: q alone) by the positions of their
  * tokens: positions[b*pos_stride + s] (device int64; pos_stride 0: the same
  * for every sequence; negative positions turn backwards), or start + s where
- * positions is NULL.  The angle is formed in 64 bits, the rotation in F32.
+ * positions is NULL (start + seq - 1 must fit 64 bits).  The angle is formed
+ * in 64 bits, the rotation in F32.
  * dtype SAM3CU_F32, _F16 or _BF16; head_dim 2 .. 256, >= 2*n_pairs.  Heads
  * whose head_dim is a multiple of 16 and whose rows start on 16
  * bytes take 16-byte accesses.

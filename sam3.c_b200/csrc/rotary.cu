@@ -639,6 +639,7 @@ int rotary_common(const sam3cu_head_view* q, const sam3cu_head_view* k, int dtyp
   p.heads = static_cast<int>(heads);
   p.tokens = static_cast<int64_t>(batch) * seq;
   if (p.tokens == 0 || p.heads == 0) return SAM3CU_OK;
+  if (freqs && !positions && start > INT64_MAX - (seq - 1)) return SAM3CU_EINVAL;
   p.seq = seq;
   p.head_dim = head_dim;
   p.positions = positions;

@@ -371,9 +371,11 @@ def _head_view(x, out, q, dev, gamma, beta, what):
                                 _head_param(gamma, shape[3], dev, "gamma"), _head_param(beta, shape[3], dev, "beta"))
 
 
-def _positions(positions, batch, seq, dev):
+def _positions(positions, start, batch, seq, dev):
     """Pointer and batch stride of int64 positions [seq], [1, seq] or [batch, seq]."""
     if positions is None:
+        if not -2 ** 63 <= start < 2 ** 63:  # ctypes would drop the upper bits
+            raise ValueError("start must fit 64 bits")
         return None, 0
     shape = positions.shape
     if positions.dtype != _torch_int64 or positions.get_device() != dev or len(shape) not in (1, 2) \
@@ -397,7 +399,7 @@ def rope_pos(q, freqs: RopeFreqs, positions=None, start: int = 0, k=None, out=No
     if k is not None:
         k_out, kv = _head_view(k, k_out, q, dev, None, None, "k")
     batch, seq, _, head_dim = q.shape
-    pos, stride = _positions(positions, batch, seq, dev)
+    pos, stride = _positions(positions, start, batch, seq, dev)
     check(lib().sam3cu_rope_pos(qv, kv, dtype_code(q), batch, seq, head_dim, pos, stride, start, freqs.ptr,
                                 _cuda_stream(dev)), "sam3cu_rope_pos")
     return out if k is None else (out, k_out)
@@ -418,7 +420,7 @@ def qk_norm_rope(q, k, q_gamma=None, k_gamma=None, q_beta=None, k_beta=None, nor
     table, pos, stride = None, None, 0
     if freqs is not None:
         table = freqs.ptr
-        pos, stride = _positions(positions, batch, seq, dev)
+        pos, stride = _positions(positions, start, batch, seq, dev)
     check(lib().sam3cu_qk_norm_rope(qv, kv, dtype_code(q), batch, seq, head_dim, norm, eps, pos, stride, start, table,
                                     _cuda_stream(dev)), "sam3cu_qk_norm_rope")
     return out if k is None else (out, k_out)

@@ -192,3 +192,21 @@ def test_tables_that_do_not_fit_are_refused(bad):
 def test_largest_tables():
     assert np.isfinite(sam3cu.RopeFreqs(64, amplitude=3e38).amplitude)
     assert (sam3cu.RopeFreqs(64, scaling=sam3cu.ROPE_SCALE_NTK, factor=1e6, theta=1e300).turns > 0).all()
+
+
+def test_start_out_of_range():
+    """start + seq - 1 has to be a 64-bit position; a Python integer that is
+    none must not wrap into one."""
+    L, f = sam3cu.lib(), sam3cu.RopeFreqs(64)
+
+    def call(start, seq=2, batch=2):
+        rope = L.sam3cu_rope_pos(_view(), None, sam3cu.BF16, batch, seq, 64, None, 0, start, f.ptr, None)
+        norm = L.sam3cu_qk_norm_rope(_view(), None, sam3cu.BF16, batch, seq, 64, 1, 1e-6, None, 0, start, f.ptr, None)
+        assert rope == norm
+        return rope
+    assert call(2 ** 63 - 1) == EINVAL and call(2 ** 63 - 5, seq=7) == EINVAL
+    assert call(2 ** 63 - 1, batch=0) == 0
+    for start in (2 ** 63, 2 ** 64 + 1, -2 ** 63 - 1):
+        with pytest.raises(ValueError):
+            sam3cu._positions(None, start, 1, 1, 0)
+    assert sam3cu._positions(None, -2 ** 63, 1, 1, 0) == (None, 0)
