@@ -695,8 +695,8 @@ SAM3CU_API int sam3cu_qk_norm_rope(const struct sam3cu_head_view *q,
  * bias: device F32 [batch, q_heads, sq, sk] with strides (batch, head, query)
  * >= 0, keys contiguous, or NULL; -inf removes a key for its query (the key's
  * V still has to be finite); finite values, the lowest included, only add.
- * scale 0: 1/sqrt(head_dim).  q_heads / kv_heads <= 128.  Scores, softmax
- * and sums in F32, P rounded to dtype before P.V.
+ * scale: at most 2^127; 0: 1/sqrt(head_dim).  q_heads / kv_heads <= 128.
+ * Scores, softmax and sums in F32, P rounded to dtype before P.V.
  */
 struct sam3cu_cross_attention_args {
 	const void *q, *k, *v;

@@ -1071,7 +1071,7 @@ extern "C" int sam3cu_cross_attention(const struct sam3cu_cross_attention_args* 
   if (a->batch < 0 || a->sq < 0 || a->sk < 0 || a->q_heads < 0 || a->kv_heads < 1 || a->head_dim < 1)
     return SAM3CU_EINVAL;
   if (a->q_heads % a->kv_heads) return SAM3CU_EINVAL;
-  if (!(a->scale >= 0.f) || std::isinf(a->scale)) return SAM3CU_EINVAL;
+  if (!(a->scale >= 0.f) || std::isinf(a->scale * kLog2e)) return SAM3CU_EINVAL;
   if (a->head_dim % 8 || a->head_dim > 128) return SAM3CU_ESHAPE;
   if (a->batch == 0 || a->sq == 0 || a->q_heads == 0) return SAM3CU_OK;
   const int group = a->q_heads / a->kv_heads;
@@ -1106,7 +1106,7 @@ extern "C" int sam3cu_cross_attention(const struct sam3cu_cross_attention_args* 
   p.head_dim = a->head_dim;
   p.rows = a->sq * group;
   p.scale = a->scale > 0.f ? a->scale : 1.f / sqrtf(static_cast<float>(a->head_dim));
-  p.scale_log2 = p.scale * 1.4426950408889634f;
+  p.scale_log2 = p.scale * kLog2e;
   if (a->k_lens) {
     if (reinterpret_cast<uintptr_t>(a->k_lens) & 3) return SAM3CU_EINVAL;
     p.k_lens = a->k_lens;

@@ -210,3 +210,10 @@ def test_start_out_of_range():
         with pytest.raises(ValueError):
             sam3cu._positions(None, start, 1, 1, 0)
     assert sam3cu._positions(None, -2 ** 63, 1, 1, 0) == (None, 0)
+
+
+def test_cross_attention_scale_out_of_range():
+    """Scores are taken in base 2: scale * log2(e) has to be finite, or a score
+    of 0 becomes NaN."""
+    for scale in (3.4e38, 2.4e38):
+        assert _cross(scale=scale) == EINVAL
