@@ -962,7 +962,7 @@ int launch_few(const CrossParams& p, cudaStream_t st) {
   if (!make_kv_maps(p, kBf16 ? kBF16 : kF16, Cf::kKT, &mk, &mv, &share)) return kErrTma;
   const int row_tiles = (p.rows + Cf::kRows - 1) / Cf::kRows;
   const int64_t items = static_cast<int64_t>(row_tiles) * p.kv_heads * p.batch;
-  static std::atomic<int> active[17];
+  static ClusterTable clusters;
   const int key_tiles = (p.sk + Cf::kKT - 1) / Cf::kKT;
   // Few items over long states: a cluster of 16 CTAs for each leaves SMs idle
   // (and only 7 such clusters fit where a CTA takes most of an SM).  From 16 MB
@@ -988,7 +988,7 @@ int launch_few(const CrossParams& p, cudaStream_t st) {
     }
     cudaGetLastError();
   }
-  const int splits = cluster_splits(kernel, Cf::kThreads, Cf::kSmem, items, key_tiles, 2, 16, active);
+  const int splits = cluster_splits(kernel, Cf::kThreads, Cf::kSmem, items, key_tiles, 2, 16, clusters);
   return launch_split(kernel, items, splits, Cf::kThreads, Cf::kSmem, st, true, mk, mv, p, share, row_tiles, splits,
                       static_cast<float*>(nullptr));
 }
@@ -1001,8 +1001,8 @@ int launch_rows_any(const CrossParams& p, cudaStream_t st) {
   if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), Cf::kSmem, true, ready)) return rc;
   const int row_tiles = static_cast<int>((static_cast<int64_t>(p.rows) + Cf::kRows - 1) / Cf::kRows);
   const int64_t items = static_cast<int64_t>(row_tiles) * p.kv_heads * p.batch;
-  static std::atomic<int> active[17];
-  const int splits = cluster_splits(kernel, kThreads, Cf::kSmem, items, (p.sk + Cf::kKT - 1) / Cf::kKT, 8, 16, active);
+  static ClusterTable clusters;
+  const int splits = cluster_splits(kernel, kThreads, Cf::kSmem, items, (p.sk + Cf::kKT - 1) / Cf::kKT, 8, 16, clusters);
   const bool wide = p.bias && (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0 && p.sk % 4 == 0 && p.bb % 4 == 0 &&
                     p.bh % 4 == 0 && p.bs % 4 == 0;
   return launch_split(kernel, items, splits, kThreads, Cf::kSmem, st, true, p, row_tiles, splits, wide ? 4 : 1);

@@ -4,10 +4,10 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
-#include <atomic>
 #include <cstdint>
 #include <initializer_list>
 
+#include "cluster_table.h"
 #include "sam3cu_internal.h"
 #include "tma_host.cuh"
 
@@ -104,14 +104,15 @@ inline bool cross_kv_maps(const CrossParams& p) {
 // CTAs of a cluster that share an item's keys: the most, up to `most` (<= 16),
 // of which all items' clusters run at once and each has `tiles_each` key tiles.
 // (Clusters are placed within a GPC: 16 items of 8 are two waves, 15 fit.)
-// active: the kernel's own table of what fits, filled as it is asked.
+// table: the kernel's own, of what fits on each device.
 template <class K>
 int cluster_splits(K kernel, int threads, int smem, int64_t items, int key_tiles, int tiles_each, int most,
-                   std::atomic<int> (&active)[17]) {
+                   ClusterTable& table) {
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess) cudaGetLastError();
   for (int n = most; n > 1; --n) {
     if (key_tiles < tiles_each * n || items * n > 4 * num_sms()) continue;
-    int fit = active[n].load();
-    if (!fit) {
+    const int fit = table.fit(dev, n, [&](int* f) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(n);
       cfg.blockDim = dim3(threads);
@@ -122,12 +123,10 @@ int cluster_splits(K kernel, int threads, int smem, int64_t items, int key_tiles
       at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
       cfg.attrs = at;
       cfg.numAttrs = 1;
-      if (cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg) != cudaSuccess || fit < 1) {
-        cudaGetLastError();
-        fit = -1;
-      }
-      active[n].store(fit);
-    }
+      const cudaError_t e = cudaOccupancyMaxActiveClusters(f, kernel, &cfg);
+      if (e != cudaSuccess) cudaGetLastError();  // the next call's own check must not see it
+      return static_cast<int>(e);
+    });
     if (items <= fit) return n;
   }
   return 1;

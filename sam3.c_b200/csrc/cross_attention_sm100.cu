@@ -571,8 +571,8 @@ int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
     if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess || fa.localSizeBytes != 0) return kErrLaunch;
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
-  static std::atomic<int> active[17];
-  prm.splits = cluster_splits(kernel, kThreads, Cfg<kD>::kSmem, prm.n_items, key_tiles, 4, 8, active);
+  static ClusterTable clusters;
+  prm.splits = cluster_splits(kernel, kThreads, Cfg<kD>::kSmem, prm.n_items, key_tiles, 4, 8, clusters);
   // Short items: one CTA per SM that walks them, so that an item's first loads
   // and S overlap the epilogue before it (4 x 8 heads x 5184 queries, 77 / 512 /
   // 2048 keys, D = 64: 29 / 63 / 203 us against 37 / 71 / 208 with a CTA each).
