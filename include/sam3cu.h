@@ -164,6 +164,13 @@ SAM3CU_API int sam3cu_sdpa(const void *q, const void *k, const void *v, int64_t 
  */
 SAM3CU_API int sam3cu_selftest_wait_timeout(unsigned long long limit_ns, int *timed_out);
 
+/*
+ * on != 0: sam3cu_cross_attention computes what its tcgen05 kernel would take
+ * with the warp-MMA kernels, as it does where a compiler spilled registers of
+ * that kernel (the whole process, until called with 0).
+ */
+SAM3CU_API void sam3cu_selftest_cross_spilled(int on);
+
 /* ------------------------------------------------------------- TinyViT */
 
 /*

@@ -1015,7 +1015,9 @@ int launch_keep(const CrossParams& p, cudaStream_t st) {
   if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), 200 * 1024, false, ready)) return rc;
   static const int regs = [&] {
     cudaFuncAttributes fa;
-    return cudaFuncGetAttributes(&fa, kernel) == cudaSuccess ? fa.numRegs : 255;
+    if (cudaFuncGetAttributes(&fa, kernel) == cudaSuccess) return fa.numRegs;
+    cudaGetLastError();  // the launch's own check must not see it
+    return 255;
   }();
   const int smem = KeepCfg<kD>::smem(p.sk);
   // as many CTAs as the SMs hold at once, each with a share of the rows (one
@@ -1133,6 +1135,9 @@ extern "C" int sam3cu_cross_attention(const struct sam3cu_cross_attention_args* 
   // keys: 42 and 29; 8 heads x 300 queries, D = 64, 77 keys: 5.3 and 7.9).
   const bool small = p.sk <= 128 && (p.head_dim <= 32 || static_cast<int64_t>(p.rows) * p.kv_heads * p.batch <=
                                                              128ll * num_sms());
-  if (p.rows > 64 && !small && cross_tc_takes(p)) return launch_cross_tc(p, a->dtype, st);
+  if (p.rows > 64 && !small && cross_tc_takes(p)) {
+    const int rc = launch_cross_tc(p, a->dtype, st);
+    if (rc != kCrossTcSpills) return rc;
+  }
   return launch_cross_mma(p, a->dtype, st);
 }

@@ -135,6 +135,10 @@ int cluster_splits(K kernel, int threads, int smem, int64_t items, int key_tiles
 int launch_cross_mma(const CrossParams& p, int dtype, cudaStream_t st);
 // cross_attention_sm100.cu: whether the tensor maps can describe the call.
 bool cross_tc_takes(const CrossParams& p);
+// Launches, or returns kCrossTcSpills where the compiler spilled registers of
+// the kernel: launch_cross_mma takes every call that this one takes.
+constexpr int kCrossTcSpills = 1;
+void cross_tc_as_if_spilled(bool on);  // for the self test
 int launch_cross_tc(const CrossParams& p, int dtype, cudaStream_t st);
 unsigned int dev_error_cross();
 unsigned int dev_error_cross_few();

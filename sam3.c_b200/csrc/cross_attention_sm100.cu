@@ -554,11 +554,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   cluster_sync();  // the others may still read this CTA's partial rows
 }
 
+std::atomic<bool> as_if_spilled{false};
+
 template <bool kBf16, int kD, bool kMask>
 int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, TcParams& prm, int key_tiles,
                    cudaStream_t st) {
   const auto kernel = cross_tc_kernel<kBf16, kD, kMask>;
   static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+  static std::atomic<int> spills{-1};     // of this build: see the softmax's registers
+  if (spills.load() < 0) {
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess) {
+      cudaGetLastError();
+      return kErrCuda;
+    }
+    spills.store(fa.localSizeBytes != 0);
+  }
+  if (spills.load() || as_if_spilled.load()) return kCrossTcSpills;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return kErrCuda;
   if (dev >= 64 || !(ready.load() >> dev & 1)) {
@@ -566,9 +578,6 @@ int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
       cudaGetLastError();
       return kErrCuda;
     }
-    // a build that spills is not run: see the softmax's registers
-    cudaFuncAttributes fa;
-    if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess || fa.localSizeBytes != 0) return kErrLaunch;
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   static ClusterTable clusters;
@@ -611,6 +620,8 @@ int launch_typed(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap
 }
 
 }  // namespace
+
+void cross_tc_as_if_spilled(bool on) { as_if_spilled.store(on); }
 
 bool cross_tc_takes(const CrossParams& p) {
   if (p.bias || !cross_kv_maps(p)) return false;

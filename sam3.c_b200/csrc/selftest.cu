@@ -5,11 +5,15 @@
 // hangs the GPU and the context stays usable.  This entry point proves that
 // path on demand: one CTA waits on an mbarrier that nothing ever arrives on,
 // with a short limit, and must come back with the error recorded.
+//
+// sam3cu_selftest_cross_spilled makes cross attention take the way that it
+// takes where the compiler spilled its tcgen05 kernel.
 #include <cuda_runtime.h>
 
 #include <cstdint>
 
 #include "../../include/sam3cu.h"
+#include "cross_attention.cuh"
 #include "sam3cu_internal.h"
 #include "sm100_ptx.cuh"
 
@@ -55,3 +59,5 @@ extern "C" int sam3cu_selftest_wait_timeout(unsigned long long limit_ns, int* ti
   if (rc == SAM3CU_OK) *timed_out = (h == 1 && err == kErrSelfTest) ? 1 : 0;
   return rc;
 }
+
+extern "C" void sam3cu_selftest_cross_spilled(int on) { s3::cross_tc_as_if_spilled(on != 0); }

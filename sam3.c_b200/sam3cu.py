@@ -37,7 +37,7 @@ EXPORTS = (
     "sam3cu_tvit_expand_bias", "sam3cu_tvit_window_attention",
     "sam3cu_tvit_block_create", "sam3cu_tvit_block_forward", "sam3cu_tvit_block_destroy",
     "sam3cu_tvit_mbconv_create", "sam3cu_tvit_mbconv_forward", "sam3cu_tvit_mbconv_destroy",
-    "sam3cu_selftest_wait_timeout",
+    "sam3cu_selftest_wait_timeout", "sam3cu_selftest_cross_spilled",
     "sam3cu_tinyvit_create", "sam3cu_tinyvit_encode", "sam3cu_tinyvit_grid", "sam3cu_tinyvit_destroy",
     "sam3cu_sam3_check", "sam3cu_sam3_find", "sam3cu_vit_create_from_sam3", "sam3cu_vit_get_config",
     "sam3cu_neck_create", "sam3cu_neck_forward", "sam3cu_neck_forward_async", "sam3cu_neck_out_size",
@@ -115,6 +115,8 @@ def lib():
         L.sam3cu_tvit_mbconv_forward.argtypes = [vp, vp, i32, i32, i32, vp]
         L.sam3cu_tvit_mbconv_destroy.argtypes = [vp]
         L.sam3cu_selftest_wait_timeout.argtypes = [C.c_ulonglong, C.POINTER(C.c_int)]
+        L.sam3cu_selftest_cross_spilled.argtypes = [i32]
+        L.sam3cu_selftest_cross_spilled.restype = None
         L.sam3cu_tinyvit_create.restype = vp
         L.sam3cu_tinyvit_create.argtypes = [vp, vp, i32, i32, C.POINTER(C.c_int)]
         L.sam3cu_tinyvit_encode.argtypes = [vp, vp, i32, vp, i32]

@@ -412,3 +412,22 @@ def test_wrapper_refusals(cuda):
             sam3cu.cross_attention(**{**dict(q=q, k=k, v=v), **bad})
     with pytest.raises(KeyError):
         sam3cu.cross_attention(q.double(), k.double(), v.double())
+
+
+@pytest.mark.parametrize("hd,dt", [(32, "f16"), (64, "bf16"), (128, "f16")])
+@pytest.mark.parametrize("sq,sk", [(130, 300), (1000, 200), (300, 3000)])
+def test_without_the_tcgen05_kernel(cuda, hd, dt, sq, sk):
+    """Where a compiler spilled that kernel the warp-MMA ones take its calls."""
+    import torch
+    import sam3cu
+    q, k, v = _make(2, sq, sk, 6, 3, hd, dt, seed=hd)
+    lens = torch.tensor([sk, sk // 3], dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    mask = torch.rand(2, sk, generator=g, device="cuda") < 0.5
+    sam3cu.lib().sam3cu_selftest_cross_spilled(1)
+    try:
+        _check(q, k, v)
+        _check(q, k, v, k_lens=lens, key_mask=mask)
+    finally:
+        sam3cu.lib().sam3cu_selftest_cross_spilled(0)
+    _check(q, k, v, k_lens=lens, key_mask=mask)
