@@ -528,7 +528,8 @@ __global__ void __launch_bounds__(FewCfg<kD>::kThreads)
   const float to_log2 = kBias ? kLog2e : p.scale_log2;
 
   if (warp == Cf::kWarps) {
-    for (int t = t0; run && t < t1; ++t) {
+    int issued = 0;
+    for (int t = t0; run && t < t1; ++t, ++issued) {
       const int st = (t - t0) % kStages;
       if (!mbar_wait_warp(&empty[st], (((t - t0) / kStages) & 1) ^ 1, kErrStageFree, abort_flag)) break;
       if (elect_one()) {
@@ -541,6 +542,10 @@ __global__ void __launch_bounds__(FewCfg<kD>::kThreads)
       }
       __syncwarp();
     }
+    // The last copies are seen in, also where a wait gave up: this shared
+    // memory may be another CTA's as soon as this one ends.
+    for (int i = max(0, issued - kStages); i < issued; ++i)
+      mbar_wait_warp(&full[i % kStages], (i / kStages) & 1, kErrTmaWait, nullptr);
   } else {
     // byte offset of piece c of row r in a tile as the copies lay it: for
     // D = 128 two halves of 128-byte rows

@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using Cf = Cfg<kD>;
   constexpr int kStages = Cf::kStages, kTile = Cf::kTile;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ uint64_t bars[12 + 4 * kStages];
+  __shared__ uint64_t bars[13 + 4 * kStages];
   __shared__ float2 ml[2 * kQ];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag_s;
@@ -184,6 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* k_empty = k_full + kStages;
   uint64_t* v_full = k_empty + kStages;
   uint64_t* v_empty = v_full + kStages;
+  uint64_t* mma_done = v_empty + kStages;
   volatile int* abort_flag = &abort_flag_s;
 
   const CrossParams& p = prm.c;
@@ -211,6 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
     }
+    mbar_init(mma_done, 1);
     abort_flag_s = aligned ? 0 : 1;
     if (!aligned) atomicCAS(&g_dev_error, 0u, static_cast<unsigned>(kErrTmemAlloc));
     fence_barrier_init();
@@ -234,6 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tma_prefetch_desc(&tv);
     }
     __syncwarp();
+    int k_issued = 0, v_issued = 0, q0_issued = 0, q1_issued = 0;
     Cursor c;
     c.start(prm, first, step, split);
     for (; c.more(prm); c.next(prm, step, split)) {
@@ -249,6 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                       it.b * prm.kv.kb);
       }
       __syncwarp();
+      ++k_issued;
       if (c.j == 0) {
         bool ok = true;
         for (int t = 0; ok && t < it.tiles; ++t) {
@@ -262,6 +266,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                           it.q0 + t * prm.qpt, it.b * prm.qmul_b);
           }
           __syncwarp();
+          q0_issued += ok && t == 0;
+          q1_issued += ok && t == 1;
         }
         if (!ok) break;
       }
@@ -273,7 +279,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                       it.b * prm.kv.vb);
       }
       __syncwarp();
+      ++v_issued;
     }
+    // The last copies are seen in, also where a wait gave up: this shared
+    // memory may be another CTA's as soon as this one ends.
+    for (int i = max(0, k_issued - kStages); i < k_issued; ++i)
+      mbar_wait_warp(&k_full[i % kStages], (i / kStages) & 1, kErrTmaWait, nullptr);
+    for (int i = max(0, v_issued - kStages); i < v_issued; ++i)
+      mbar_wait_warp(&v_full[i % kStages], (i / kStages) & 1, kErrTmaWait, nullptr);
+    if (q0_issued > 0) mbar_wait_warp(&q_full[0], (q0_issued - 1) & 1, kErrTmaWait, nullptr);
+    if (q1_issued > 0) mbar_wait_warp(&q_full[1], (q1_issued - 1) & 1, kErrTmaWait, nullptr);
   } else if (warp == 1 && aligned) {
     // ------------------------------------------------------------ MMA
     const uint32_t fmt = kBf16 ? 1u : 0u;
@@ -337,6 +352,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (ahead) s.next(prm, step, split);
     }
+    // and so are the last MMAs, before TMEM is given back
+    umma_commit_warp(mma_done);
+    mbar_wait_warp(mma_done, 0, kErrAccFull, nullptr);
   } else if (warp >= 4) {
     // ------------------------------------------------ softmax + epilogue
     const int t = (warp - 4) >> 2, quarter = warp & 3;
