@@ -167,9 +167,10 @@ SAM3CU_API int sam3cu_selftest_wait_timeout(unsigned long long limit_ns, int *ti
 /*
  * on != 0: sam3cu_cross_attention computes what its tcgen05 kernel would take
  * with the warp-MMA kernels, as it does where a compiler spilled registers of
- * that kernel (the whole process, until called with 0).
+ * that kernel (the whole process, until called with 0).  Returns how many of
+ * that kernel's builds that were called so far the compiler did spill.
  */
-SAM3CU_API void sam3cu_selftest_cross_spilled(int on);
+SAM3CU_API int sam3cu_selftest_cross_spilled(int on);
 
 /* ------------------------------------------------------------- TinyViT */
 

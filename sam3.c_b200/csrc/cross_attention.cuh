@@ -138,7 +138,7 @@ bool cross_tc_takes(const CrossParams& p);
 // Launches, or returns kCrossTcSpills where the compiler spilled registers of
 // the kernel: launch_cross_mma takes every call that this one takes.
 constexpr int kCrossTcSpills = 1;
-void cross_tc_as_if_spilled(bool on);  // for the self test
+int cross_tc_as_if_spilled(bool on);  // for the self test
 int launch_cross_tc(const CrossParams& p, int dtype, cudaStream_t st);
 unsigned int dev_error_cross();
 unsigned int dev_error_cross_few();

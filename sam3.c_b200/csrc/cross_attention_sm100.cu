@@ -573,6 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 std::atomic<bool> as_if_spilled{false};
+std::atomic<int> builds_spilled{0};
 
 template <bool kBf16, int kD, bool kMask>
 int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, TcParams& prm, int key_tiles,
@@ -586,6 +587,7 @@ int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
       cudaGetLastError();
       return kErrCuda;
     }
+    if (fa.localSizeBytes != 0) builds_spilled.fetch_add(1);
     spills.store(fa.localSizeBytes != 0);
   }
   if (spills.load() || as_if_spilled.load()) return kCrossTcSpills;
@@ -639,7 +641,10 @@ int launch_typed(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap
 
 }  // namespace
 
-void cross_tc_as_if_spilled(bool on) { as_if_spilled.store(on); }
+int cross_tc_as_if_spilled(bool on) {
+  as_if_spilled.store(on);
+  return builds_spilled.load();
+}
 
 bool cross_tc_takes(const CrossParams& p) {
   if (p.bias || !cross_kv_maps(p)) return false;

@@ -60,4 +60,4 @@ extern "C" int sam3cu_selftest_wait_timeout(unsigned long long limit_ns, int* ti
   return rc;
 }
 
-extern "C" void sam3cu_selftest_cross_spilled(int on) { s3::cross_tc_as_if_spilled(on != 0); }
+extern "C" int sam3cu_selftest_cross_spilled(int on) { return s3::cross_tc_as_if_spilled(on != 0); }

@@ -116,7 +116,6 @@ def lib():
         L.sam3cu_tvit_mbconv_destroy.argtypes = [vp]
         L.sam3cu_selftest_wait_timeout.argtypes = [C.c_ulonglong, C.POINTER(C.c_int)]
         L.sam3cu_selftest_cross_spilled.argtypes = [i32]
-        L.sam3cu_selftest_cross_spilled.restype = None
         L.sam3cu_tinyvit_create.restype = vp
         L.sam3cu_tinyvit_create.argtypes = [vp, vp, i32, i32, C.POINTER(C.c_int)]
         L.sam3cu_tinyvit_encode.argtypes = [vp, vp, i32, vp, i32]

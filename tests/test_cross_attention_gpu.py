@@ -431,3 +431,16 @@ def test_without_the_tcgen05_kernel(cuda, hd, dt, sq, sk):
     finally:
         sam3cu.lib().sam3cu_selftest_cross_spilled(0)
     _check(q, k, v, k_lens=lens, key_mask=mask)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_the_tcgen05_kernel_is_not_spilled(cuda, hd, dt, masked):
+    """Each build of it is the one that runs: none was left to the warp MMAs."""
+    import torch
+    import sam3cu
+    q, k, v = _make(1, 300, 1000, 2, 2, hd, dt, seed=hd)
+    mask = torch.arange(1000, device="cuda")[None] % 3 > 0 if masked else None
+    _check(q, k, v, key_mask=mask)
+    assert sam3cu.lib().sam3cu_selftest_cross_spilled(0) == 0
