@@ -640,6 +640,7 @@ int rotary_common(const sam3cu_head_view* q, const sam3cu_head_view* k, int dtyp
   p.tokens = static_cast<int64_t>(batch) * seq;
   if (p.tokens == 0 || p.heads == 0) return SAM3CU_OK;
   if (freqs && !positions && start > INT64_MAX - (seq - 1)) return SAM3CU_EINVAL;
+  if (q->heads == 0) p.v[0] = p.v[1];  // where lanes without a head point must be memory too
   p.seq = seq;
   p.head_dim = head_dim;
   p.positions = positions;

@@ -281,3 +281,22 @@ def test_exchange_with_lanes_left_over(cuda, dt, norm, hd):
     of the head and must leave its words to the lanes that do."""
     _check((3, 41, 9, hd), 5, dt, hd - 2, True, norm=norm, seed=hd)
     _check((3, 41, 9, hd), 5, dt, hd // 2 + 2 - hd // 2 % 2, True, norm=norm, seed=hd, inplace=True)
+
+
+@pytest.mark.parametrize("norm", [0, 1, 2])
+@pytest.mark.parametrize("hd,rot", [(64, 64), (80, 20), (72, 40)])
+def test_heads_of_k_alone(cuda, norm, hd, rot):
+    """No heads of q, with and without memory of its own; the result is that
+    of the same heads taken as q's."""
+    import torch
+    import sam3cu
+    x, f = _tensor((3, 17, 5, hd), "bf16", 9), sam3cu.RopeFreqs(rot)
+    gamma = 1 + 0.1 * torch.arange(hd, device="cuda", dtype=torch.float32) / hd
+    for none in (x[:, :, :0], torch.empty(3, 17, 0, hd, device="cuda", dtype=x.dtype)):
+        if norm:
+            want = sam3cu.qk_norm_rope(x, None, gamma, norm=norm, freqs=f, start=3)
+            q, k = sam3cu.qk_norm_rope(none, x, None, gamma, norm=norm, freqs=f, start=3)
+        else:
+            want = sam3cu.rope_pos(x, f, start=3)
+            q, k = sam3cu.rope_pos(none, f, start=3, k=x)
+        assert q.shape == (3, 17, 0, hd) and torch.equal(k, want)
