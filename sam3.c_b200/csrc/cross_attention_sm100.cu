@@ -221,6 +221,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(&tmem_slot, 512);
     tmem_relinquish();
   }
+  // The copies fill qpt * group of a query tile's 128 rows.  The others become
+  // zeros, once: what another kernel left there would have a say in when their
+  // warp's rows are rescaled, and with it in how those round.
+  for (int i = threadIdx.x; i < 2 * kTile / 16; i += kThreads) {
+    const int row = i % (kTile / Cf::kHalves / 16) / (Cf::kRowBytes / 16);
+    if (row >= prm.qpt * p.group) *reinterpret_cast<uint4*>(sQ + i * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

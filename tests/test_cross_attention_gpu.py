@@ -444,3 +444,21 @@ def test_the_tcgen05_kernel_is_not_spilled(cuda, hd, dt, masked):
     mask = torch.arange(1000, device="cuda")[None] % 3 > 0 if masked else None
     _check(q, k, v, key_mask=mask)
     assert sam3cu.lib().sam3cu_selftest_cross_spilled(0) == 0
+
+
+@pytest.mark.parametrize("b,sq,sk,hq,hkv,hd,dt", [
+    (2, 1729, 1001, 20, 4, 128, "f16"), (2, 500, 1001, 6, 2, 64, "bf16"), (2, 901, 1500, 5, 1, 32, "f16")])
+def test_what_ran_before_has_no_say(cuda, b, sq, sk, hq, hkv, hd, dt):
+    """Groups that do not divide 128 leave rows of a tile without a query.
+    Whatever earlier kernels left in their shared memory, the other rows come
+    out the same, to the bit."""
+    import torch
+    import sam3cu
+    q, k, v = _make(b, sq, sk, hq, hkv, hd, dt, seed=18)
+    lens = torch.tensor([sk * 2 // 3, sk * 3 // 5], dtype=torch.int32, device="cuda")
+    first = [sam3cu.cross_attention(q, k, v, k_lens=n) for n in (None, lens)]
+    for i in range(9):
+        x = _make(1, 1000, 1000, 4, 4, hd, dt, seed=i, sharp=10.0 ** (i % 3))
+        sam3cu.cross_attention(*x)
+        for n, want in zip((None, lens), first):
+            assert torch.equal(sam3cu.cross_attention(q, k, v, k_lens=n), want)
