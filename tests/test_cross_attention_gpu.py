@@ -462,3 +462,101 @@ def test_what_ran_before_has_no_say(cuda, b, sq, sk, hq, hkv, hd, dt):
         sam3cu.cross_attention(*x)
         for n, want in zip((None, lens), first):
             assert torch.equal(sam3cu.cross_attention(q, k, v, k_lens=n), want)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("value", [(40.0, 31.25), (800.0, 640.0)])
+@pytest.mark.parametrize("sq,sk", [(1, 999), (20, 999), (150, 999), (150, 77), (300, 5000), (1, 70000)])
+def test_equal_large_scores_give_the_mean(cuda, dt, value, sq, sk):
+    """One value for all scores, 10^4 or 4 10^6: the mean of V.  The dot
+    products are sums of equal powers of two and small factors, exact in F32,
+    so every P is the same number: the rounding of P (half a step), of the
+    sums and of the output remain, and nothing for the scores."""
+    import torch
+    import sam3cu
+    q, k, v = _make(1, sq, sk, 1, 1, 64, dt, seed=7)
+    q[:], k[:] = value
+    o = sam3cu.cross_attention(q, k, v).double()
+    mean, size = v[0, :, 0].double().mean(0), v[0, :, 0].double().abs().mean(0)
+    half = torch.finfo(v.dtype).eps / 2
+    tol = half * mean.abs() + (half + 2.0 ** -18) * size
+    assert bool(((o - mean).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("sq,sk", [(1, 300), (5, 1027), (40, 517), (201, 517), (300, 129)])
+def test_bias_with_masks(cuda, hd, sq, sk):
+    """A bias beside lengths and a key mask; what it holds at keys that do not
+    count, NaN and infinities, stays out."""
+    import torch
+    import sam3cu
+    q, k, v = _make(3, sq, sk, 4, 2, hd, "bf16", seed=15)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    bias = torch.randn(3, 4, sq, sk, generator=g, device="cuda") * 2
+    bias[0, 1, 0] = -math.inf
+    mask = torch.rand(3, sk, generator=g, device="cuda") < 0.6
+    mask[1] = False
+    lens = torch.tensor([sk, sk, sk // 2], dtype=torch.int32, device="cuda")
+    o = _check(q, k, v, bias=bias, key_mask=mask, k_lens=lens)
+    assert bool((o[1] == 0).all()) and bool((o[0, 0, 1] == 0).all())
+    off = ~mask | (torch.arange(sk, device="cuda") >= lens[:, None])
+    for value in (math.nan, math.inf):
+        assert torch.equal(sam3cu.cross_attention(q, k, v, bias=bias.masked_fill(off[:, None, None], value),
+                                                  key_mask=mask, k_lens=lens), o)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("sq,sk", [(1, 400), (40, 400), (300, 400), (300, 77)])
+def test_expanded_keys_and_queries(cuda, hd, sq, sk):
+    """Stride 0 along the keys, the queries and the heads of the queries,
+    which tensor maps cannot describe."""
+    import torch
+    q, k, v = _make(2, sq, sk, 4, 4, hd, "bf16", seed=16)
+    one = k[:, :1].expand(2, sk, 4, hd)
+    _check(q, one, v)
+    _check(q, k, v[:, :1].expand(2, sk, 4, hd))
+    _check(q, one, v[:, :1].expand(2, sk, 4, hd), k_lens=torch.tensor([3, sk], dtype=torch.int32, device="cuda"))
+    _check(q[:, :1].expand(2, sq, 4, hd), k, v)
+    _check(q[:, :, :1].expand(2, sq, 4, hd), k, v)
+
+
+@pytest.mark.parametrize("b,sq,sk,hq,hkv,hd,dt", [
+    (2, 5, 300, 8, 2, 64, "bf16"), (1, 7, 4096, 8, 8, 16, "f16"), (2, 1, 65521, 32, 4, 128, "bf16"),
+    (2, 40, 5000, 4, 4, 32, "f16"), (4, 300, 77, 8, 8, 32, "bf16"), (2, 1729, 1001, 20, 4, 128, "f16"),
+    (1, 300, 9000, 2, 2, 128, "bf16"), (2, 2000, 1500, 4, 4, 64, "bf16")])
+def test_repeats_exactly(cuda, b, sq, sk, hq, hkv, hd, dt):
+    """Every kernel and every split of the keys has a fixed order of sums."""
+    import torch
+    import sam3cu
+    q, k, v = _make(b, sq, sk, hq, hkv, hd, dt, seed=17)
+    lens = torch.randint(0, sk + 1, (b,), device="cuda", dtype=torch.int32)
+    first, masked = sam3cu.cross_attention(q, k, v), sam3cu.cross_attention(q, k, v, k_lens=lens)
+    for _ in range(4):
+        assert torch.equal(sam3cu.cross_attention(q, k, v), first)
+        assert torch.equal(sam3cu.cross_attention(q, k, v, k_lens=lens), masked)
+
+
+def test_every_result_of_four_threads(cuda):
+    """Calls from four host threads, each on a stream of its own, with a
+    workspace, a cluster and the tensor cores among them: what a thread raises
+    is raised here, and every result counts."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    import torch
+    import sam3cu
+    f = sam3cu.RopeFreqs(64)
+    sets = [_make(1, sq, sk, 4, 2, 64, "bf16", seed=sq + sk) for sq, sk in ((2, 40000), (20, 3000), (300, 3000), (300, 77))]
+    want = [sam3cu.cross_attention(sam3cu.rope_pos(q, f, start=5), k, v) for q, k, v in sets]
+    torch.cuda.synchronize()
+
+    def work(i):
+        torch.cuda.set_device(0)
+        q, k, v = sets[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            wrong = torch.zeros((), device="cuda", dtype=torch.int64)
+            for _ in range(50):
+                wrong += (sam3cu.cross_attention(sam3cu.rope_pos(q, f, start=5), k, v) != want[i]).sum()
+            return int(wrong)
+    with ThreadPoolExecutor(4) as pool:
+        assert [t.result() for t in [pool.submit(work, i) for i in range(4)]] == [0] * 4
+    assert sam3cu.device_error() == 0

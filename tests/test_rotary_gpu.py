@@ -300,3 +300,53 @@ def test_heads_of_k_alone(cuda, norm, hd, rot):
             want = sam3cu.rope_pos(x, f, start=3)
             q, k = sam3cu.rope_pos(none, f, start=3, k=x)
         assert q.shape == (3, 17, 0, hd) and torch.equal(k, want)
+
+
+@pytest.mark.parametrize("norm", [0, 1])
+@pytest.mark.parametrize("hd,rot", [(64, 64), (80, 20), (72, 40)])
+def test_offsets_past_32_bits(cuda, norm, hd, rot):
+    """Tokens that begin beyond 2^32 bytes (and 2^31 elements) into the input
+    and the output, with heads of q and k side by side."""
+    import torch
+    import sam3cu
+    tokens, pitch = 1100, 1 << 21
+    f = sam3cu.RopeFreqs(rot)
+    small = _tensor((1, tokens, 4, hd), "bf16", 10)
+    big = torch.empty(tokens * pitch, dtype=torch.bfloat16, device="cuda").as_strided((1, tokens, 4, hd),
+                                                                                      (0, pitch, hd, 1))
+    out = torch.empty(tokens * pitch, dtype=torch.bfloat16, device="cuda").as_strided((1, tokens, 4, hd),
+                                                                                      (0, pitch, hd, 1))
+    big.copy_(small)
+
+    def call(x, **out):
+        if norm:
+            return sam3cu.qk_norm_rope(x[:, :, :3], x[:, :, 3:], freqs=f, start=9, **out)
+        return sam3cu.rope_pos(x[:, :, :3], f, start=9, k=x[:, :, 3:], **out)
+    want = call(small)
+    call(big, out=out[:, :, :3], k_out=out[:, :, 3:])
+    assert torch.equal(out[:, :, :3], want[0]) and torch.equal(out[:, :, 3:], want[1])
+    call(big, out=big[:, :, :3], k_out=big[:, :, 3:])
+    assert torch.equal(big[:, :, :3], want[0]) and torch.equal(big[:, :, 3:], want[1])
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("norm", [0, 1])
+def test_rows_aligned_to_an_element(cuda, dt, norm):
+    """Inputs and outputs whose rows start on one element's size only."""
+    import torch
+    import sam3cu
+    f = sam3cu.RopeFreqs(64)
+    buf, back = (torch.randn(2 * 5 * 3 * 65 + 1, device="cuda").to(_torch_dtype(dt)) for _ in range(2))
+    q, out = buf[1:].view(2, 5, 3, 65)[..., :64], back[1:].view(2, 5, 3, 65)
+    rest = out[..., 64].clone()
+    # (products and sums in another order than in the kernel of aligned rows: against the formula)
+    x, slack = q.double(), 0.0
+    if norm:
+        sam3cu.qk_norm_rope(q, None, freqs=f, start=2, out=out[..., :64])
+        x = _norm64(x, 1, None, None, 1e-6)
+        slack = (64 + 16) * 2.0 ** -23 * x.abs().amax(-1, keepdim=True) * 2
+    else:
+        sam3cu.rope_pos(q, f, start=2, out=out[..., :64])
+    ref, size = _rotate64(x, f, (torch.arange(5, device="cuda", dtype=torch.float64) + 2)[None], True)
+    _within(out[..., :64], ref, size * 2.0 ** -19 + slack)
+    assert torch.equal(out[..., 64], rest)
