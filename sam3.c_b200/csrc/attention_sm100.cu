@@ -356,9 +356,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     int sb = 0;  // S buffer of the current tile
     auto load_s = [&](float* sv, uint32_t* su, uint32_t c0, int kfirst) {
 #pragma unroll
-      for (int c = 0; c < kHalf / 32; ++c)
-        tmem_ld_32x32b_x32(tS(sb) + lane_off + c0 + c * 32, *reinterpret_cast<uint32_t(*)[32]>(su + c * 32));
-      tmem_ld_wait();
+      for (int c = 0; c < kHalf / 32; ++c) {
+        const uint32_t at = tS(sb) + lane_off + c0 + c * 32;
+        if constexpr (kBias) tmem_ld_wait_32x32b_32(at, *reinterpret_cast<float(*)[32]>(sv + c * 32));
+        else tmem_ld_32x32b_x32(at, *reinterpret_cast<uint32_t(*)[32]>(su + c * 32));
+      }
+      if constexpr (!kBias) tmem_ld_wait();
       if constexpr (kBias) {
 #pragma unroll
         for (int c = 0; c < kHalf; c += 4) {
@@ -737,9 +740,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       // set to -inf)
       auto load_s = [&](float* sv, uint32_t* su, int kfirst, int b) {
 #pragma unroll
-        for (int c = 0; c < kKV / 32; ++c)
-          tmem_ld_32x32b_x32(tS(b) + lane_off + c * 32, *reinterpret_cast<uint32_t(*)[32]>(su + c * 32));
-        tmem_ld_wait();
+        for (int c = 0; c < kKV / 32; ++c) {
+          const uint32_t at = tS(b) + lane_off + c * 32;
+          if constexpr (kBias) tmem_ld_wait_32x32b_32(at, *reinterpret_cast<float(*)[32]>(sv + c * 32));
+          else tmem_ld_32x32b_x32(at, *reinterpret_cast<uint32_t(*)[32]>(su + c * 32));
+        }
+        if constexpr (!kBias) tmem_ld_wait();
         if constexpr (kBias) {
 #pragma unroll
           for (int c = 0; c < kKV; c += 4) {
