@@ -149,9 +149,10 @@ struct RowState {
   }
   // Scores to P, against the maximum with them in it; sum and O rescaled.
   // f16 P are times 2^14, which cancels in O / sum: below 2^-14 the type has
-  // no full precision left.  kApart: the maximum is taken off before the
-  // factor (scores with a bias, whose product with it could overflow).
-  template <int kKeys, bool kBf16, bool kApart>
+  // no full precision left.  The maximum is taken off before the factor: their
+  // product would be rounded, by 4 at 2^26, and exp2 of that is past f16's
+  // range; a bias of the type's lowest value would overflow with it.
+  template <int kKeys, bool kBf16>
   __device__ __forceinline__ void softmax(float (&s)[kKeys / 8][4], float to_log2) {
     const float shift = kBf16 ? 0.f : 14.f;
     float top[2], corr[2];
@@ -171,15 +172,13 @@ struct RowState {
       corr[h] = ex2((m[h] - base) * to_log2);
       m[h] = top[h];
       const uint64_t c2 = f2pack(to_log2, to_log2);
-      const float k = kApart ? shift : fmaf(-base, to_log2, shift);
-      const uint64_t k2 = f2pack(k, k), b2 = f2pack(-base, -base);
+      const uint64_t sh2 = f2pack(shift, shift), b2 = f2pack(-base, -base);
       uint64_t sum2 = f2pack(0.f, 0.f);
 #pragma unroll
       for (int j = 0; j < kKeys / 8; ++j) {
-        uint64_t x = f2pack(s[j][2 * h], s[j][2 * h + 1]);
-        if (kApart) x = fadd2(x, b2);
+        const uint64_t x = fadd2(f2pack(s[j][2 * h], s[j][2 * h + 1]), b2);
         float e0, e1;
-        f2unpack(ffma2(x, c2, k2), e0, e1);
+        f2unpack(kBf16 ? fmul2(x, c2) : ffma2(x, c2, sh2), e0, e1);
         s[j][2 * h] = ex2(e0);
         s[j][2 * h + 1] = ex2(e1);
         sum2 = fadd2(sum2, f2pack(s[j][2 * h], s[j][2 * h + 1]));
@@ -442,7 +441,7 @@ __global__ void __launch_bounds__(kThreads) cross_rows_kernel(const __grid_const
         }
       }
     }
-    st.template softmax<kKT, kBf16, kBias>(s, to_log2);
+    st.template softmax<kKT, kBf16>(s, to_log2);
     // O += P V, P rounded to the operands' type
 #pragma unroll
     for (int kk = 0; kk < kKT / 16; ++kk) {
@@ -636,7 +635,7 @@ __global__ void __launch_bounds__(FewCfg<kD>::kThreads)
             if (!(mine >> (j * 8 + 1) & 1)) s[j][1] = s[j][3] = -INFINITY;
           }
         }
-        rs.template softmax<32, kBf16, kBias>(s, to_log2);
+        rs.template softmax<32, kBf16>(s, to_log2);
         // O += P V, P rounded to the operands' type
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
@@ -862,7 +861,7 @@ __global__ void __launch_bounds__(kThreads) cross_keep_kernel(const __grid_const
           if (!(mine_on >> (j * 8 + 1) & 1)) s[j][1] = s[j][3] = -INFINITY;
         }
       }
-      st.template softmax<kKW, kBf16, kBias>(s, to_log2);
+      st.template softmax<kKW, kBf16>(s, to_log2);
       // O += P V, P rounded to the operands' type
 #pragma unroll
       for (int kk = 0; kk < kKW / 16; ++kk) {

@@ -54,6 +54,13 @@ constexpr int kQ = 128;        // rows of a tile
 constexpr int kKV = 128;       // keys of a tile
 constexpr int kThreads = 384;
 constexpr float kRescaleLog2 = 8.f;
+// One multiply-add takes a score to its exponent, which rounds maximum * factor:
+// a row's P get a factor that cancels in O / sum, 2^-12 off 1 at most up to
+// here.  It would be 2^4 at 2^27 (past f16's range) and 2^64 at 2^31: past this
+// value the maximum is taken off the scores first.  That costs 2 x 5184 queries
+// over 20736 keys 1536 -> 1543 us where it does not happen, in this form; taken
+// off always 1595, by a branch before the exponentials 1590 - 1617.
+constexpr float kFarLog2 = 4096.f;
 // f16 P below 2^-14 loses bits: with a maximum of 2^9 there is room for a
 // factor 2^6 under 65504.  It cancels in O / sum.
 constexpr float kF16Shift = 6.f;
@@ -141,18 +148,18 @@ struct Cursor {
   }
 };
 
-// P = exp2(S sl2 - mb) of kN keys as 16-bit pairs to TMEM from column tp on,
+// P = exp2(S sl2 + add) of kN keys as 16-bit pairs to TMEM from column tp on,
 // added up into l2.
 template <bool kBf16, int kN>
-__device__ __forceinline__ void exp_store(const float (&sv)[kN], float sl2, float mb, uint32_t tp, uint64_t (&l2)[2]) {
-  const uint64_t sc2 = f2pack(sl2, sl2), nmb2 = f2pack(-mb, -mb);
+__device__ __forceinline__ void exp_store(const float (&sv)[kN], float sl2, float add, uint32_t tp, uint64_t (&l2)[2]) {
+  const uint64_t sc2 = f2pack(sl2, sl2), ad2 = f2pack(add, add);
 #pragma unroll
   for (int c0 = 0; c0 < kN; c0 += 16) {  // 16 keys -> 8 P columns
     uint32_t pk[8];
 #pragma unroll
     for (int c = c0; c < c0 + 16; c += 2) {
       float e0, e1;
-      f2unpack(ffma2(f2pack(sv[c], sv[c + 1]), sc2, nmb2), e0, e1);
+      f2unpack(ffma2(f2pack(sv[c], sv[c + 1]), sc2, ad2), e0, e1);
       const float p0 = ex2(e0), p1 = ex2(e1);
       l2[(c >> 1) & 1] = fadd2(l2[(c >> 1) & 1], f2pack(p0, p1));
       pk[(c - c0) / 2] = pack2(p0, p1, kBf16);
@@ -433,8 +440,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         masked(sv, 0, 96);
         mt = fmaxf(mt, fmaxf(max64(sv), max32(sv + 64)));
         const bool need = (mt - m_used) * sl2 > kRescaleLog2;  // false for -inf - -inf
-        if (__any_sync(0xffffffffu, need)) {
-          const float m_new = fmaxf(m_used, mt);
+        const float m_new = fmaxf(m_used, mt), top = fabsf(m_new * sl2);
+        const bool far_row = top > kFarLog2 && top < INFINITY;
+        if (__any_sync(0xffffffffu, need || far_row)) {
           const float corr = m_used == -INFINITY ? 0.f : ex2((m_used - m_new) * sl2);
           l *= corr;
           m_used = m_new;
@@ -449,16 +457,30 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tmem_st_wait();
           }
+          if (__any_sync(0xffffffffu, far_row)) {
+            const float off = far_row ? m_used : 0.f;
+#pragma unroll
+            for (int c = 0; c < 96; ++c) sv[c] -= off;
+#pragma unroll
+            for (int c = 96; c < 128; c += 8) {  // and off those that are loaded again
+              uint32_t u[8];
+              tmem_ld_wait_32x32b_x8(tS(t) + lane_off + c, u);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) - off);
+              tmem_st_32x32b_x8(tS(t) + lane_off + c, u);
+            }
+            tmem_st_wait();
+          }
         }
         // no key yet: every exponent is -inf against 0
-        const float mb = (m_used == -INFINITY ? 0.f : m_used * sl2) - (kBf16 ? 0.f : kF16Shift);
+        const float add = (m_used == -INFINITY || far_row ? 0.f : -m_used * sl2) + (kBf16 ? 0.f : kF16Shift);
         uint64_t l2[2] = {f2pack(0.f, 0.f), f2pack(0.f, 0.f)};
-        exp_store<kBf16, 96>(sv, sl2, mb, tS(t) + lane_off, l2);  // P takes the place of S
+        exp_store<kBf16, 96>(sv, sl2, add, tS(t) + lane_off, l2);  // P takes the place of S
         if (n > 96) {  // (P of keys past the last 16 is not multiplied)
           float last[32];
           tmem_ld_wait_32x32b_32(tS(t) + lane_off + 96, last);
           masked(last, 96, 32);
-          exp_store<kBf16, 32>(last, sl2, mb, tS(t) + lane_off + 48, l2);
+          exp_store<kBf16, 32>(last, sl2, add, tS(t) + lane_off + 48, l2);
         }
         float a0, a1;
         f2unpack(fadd2(l2[0], l2[1]), a0, a1);

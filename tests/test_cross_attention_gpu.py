@@ -560,3 +560,40 @@ def test_every_result_of_four_threads(cuda):
     with ThreadPoolExecutor(4) as pool:
         assert [t.result() for t in [pool.submit(work, i) for i in range(4)]] == [0] * 4
     assert sam3cu.device_error() == 0
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("sq,sk", [(1, 999), (20, 999), (150, 77), (150, 999), (1, 70000)])
+@pytest.mark.parametrize("size", [4096.0, 65024.0])
+def test_huge_scores(cuda, dt, sq, sk, size):
+    """Scores of 10^8 and 3 10^10, from finite 16-bit queries and keys, equal
+    but for keys whose score is lower by much more than F32 resolves: the
+    mean of V over the others.  (The dot products are exact: one product of
+    powers of two times 64.)"""
+    import torch
+    import sam3cu
+    q, k, v = _make(1, sq, sk, 1, 1, 64, dt, seed=19)
+    q[:], k[:] = size, size
+    k[:, ::3] = size / 2
+    o = sam3cu.cross_attention(q, k, v).double()
+    keep = torch.arange(sk, device="cuda") % 3 != 0
+    vv = v[0, keep, 0].double()
+    mean, mag = vv.mean(0), vv.abs().mean(0)
+    half = torch.finfo(v.dtype).eps / 2
+    assert bool(((o - mean).abs() <= half * mean.abs() + (half + 2.0 ** -18) * mag).all())
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("sq,sk", [(3, 500), (40, 500), (150, 77), (300, 1500)])
+def test_rows_of_large_scores_among_others(cuda, dt, hd, sq, sk):
+    """Scores around 32768 / sqrt(head_dim), 2900 to 5800, in every third row,
+    around as much below 0 in every third, small ones in the rest, with
+    lengths and a key mask."""
+    import torch
+    q, k, v = _make(2, sq, sk, 4, 2, hd, dt, seed=21)
+    k[..., 0] = 256.0
+    q[..., 0] = torch.tensor([0.0, 128.0, -128.0], device="cuda").to(q.dtype)[torch.arange(sq, device="cuda") % 3, None]
+    lens = torch.tensor([sk, sk // 2], dtype=torch.int32, device="cuda")
+    _check(q, k, v, k_lens=lens)
+    _check(q, k, v, k_lens=lens, key_mask=torch.arange(sk, device="cuda")[None] % 5 > 1)
