@@ -12,13 +12,14 @@
 // loads are under way on every SM.  Three kernels:
 //   * cross_few_kernel, up to 16 rows of a key head: one warp fetches 128-key
 //     tiles by TMA, four compute.  2 x 4 key heads of 128 under 32, one query,
-//     65521 keys with lengths: 44 us, 0.80 of the measured copy rate;
+//     65521 and 49141 keys: 45 us, 0.80 of the measured copy rate (49 us a call);
 //   * cross_keep_kernel, few keys: K and V stay in shared memory, the warps
 //     walk the rows.  4 x 8 heads of 32, 5184 rows, 77 keys: 17 us;
 //   * cross_rows_kernel, the rest: 64 rows to a CTA, 16 to a warp, K, V and the
 //     bias through a ring of cp.async.  4 x 8 heads of 32, 201 rows, 5184 keys
-//     with a bias: 50 us, 0.48 of the copy rate for reading the bias once
-//     (shared memory bounds it: every 16 rows read all of K and V there).
+//     with a bias: 50 us, 0.47 of the copy rate for reading the bias once, and 50
+//     with one bias for all heads (shared memory bounds it: every 16 rows read
+//     all of K and V there).
 // Where that leaves SMs idle the keys are split over the CTAs of a cluster,
 // which exchange (max, sum, partial O) through distributed shared memory: no
 // workspace, no second launch, a fixed order of sums.  Few items over long
@@ -100,8 +101,9 @@ struct RowsCfg {
   static constexpr int kTileBytes = kKT * kD * 2;      // K or V
   static constexpr int kBiasBytes = kBias ? kRows * kKT * 4 : 0;
   static constexpr int kStageBytes = 2 * kTileBytes + kBiasBytes;
-  // (with a bias two, so that more CTAs fit: 201 x 5184 x 8 heads of 32, batch 4:
-  // three stages 66 us, two 53, and 50 since the bias rows are permuted)
+  // (with a bias two, so that more CTAs fit: 201 x 5184 x 8 heads of 16, 32, 64
+  // and 128, batch 4: 50, 50, 72 and 114 us, with three stages 60, 60, 81 and
+  // 161; 8 x 40 rows, heads of 64: 42 and 45; 8 x 100 x 1024, heads of 64: even)
   static constexpr int kStages = kBias ? 2 : kD == 32 ? 4 : kD == 128 ? 2 : 3;
   static constexpr int kQBytes = kRows * kD * 2;
   static constexpr int kPitch = kD + 4;                // floats of a partial row
@@ -971,7 +973,8 @@ int launch_few(const CrossParams& p, cudaStream_t st) {
   // Few items over long states: a cluster of 16 CTAs for each leaves SMs idle
   // (and only 7 such clusters fit where a CTA takes most of an SM).  From 16 MB
   // of K and V on the keys are split over all SMs, and a second launch adds the
-  // parts up out of a workspace: 8 items, 235 MB: 59 -> 44 us; 1 item, 34 MB: 31 -> 15 us.
+  // parts up out of a workspace: 8 items, 235 MB: 48 -> 45 us; 4 items, 134 MB:
+  // 35 -> 31; 1 item, 34 MB: 28 -> 14, 17 MB: 17 -> 12.
   const int64_t slots = static_cast<int64_t>(200 * 1024 / Cf::kSmem) * num_sms();
   const int64_t kv_bytes = 4ll * p.sk * p.head_dim * p.kv_heads * p.batch;
   if (items <= slots / 3 && kv_bytes >= (16ll << 20)) {
@@ -1135,8 +1138,9 @@ extern "C" int sam3cu_cross_attention(const struct sam3cu_cross_attention_args* 
   const RelaxedCapture relaxed;
   // Which kernel: tcgen05 for many rows, except over few keys where heads are
   // small or the whole call is (4 x 8 heads x 5184 queries, D = 32: 77 keys 17
-  // us kept in shared memory, 25 us on tcgen05, 256 keys 36 and 31; D = 64, 77
-  // keys: 42 and 29; 8 heads x 300 queries, D = 64, 77 keys: 5.3 and 7.9).
+  // us kept in shared memory, 23 us on tcgen05, 128 keys 21 and 22, 256 keys 36
+  // and 31; D = 64, 77 keys: 28 and 26, 128 keys: 34 and 25; 8 heads x 300
+  // queries, D = 64, 77 keys: 5.3 and 6.9, 128 keys 6.2 and 6.9).
   const bool small = p.sk <= 128 && (p.head_dim <= 32 || static_cast<int64_t>(p.rows) * p.kv_heads * p.batch <=
                                                              128ll * num_sms());
   if (p.rows > 64 && !small && cross_tc_takes(p)) {

@@ -20,16 +20,23 @@
 // 2^8.  Every mbarrier wait is bounded.
 //
 // What bounds it: a 128 x 128 tile takes 1024 clocks of the exponential units
-// (16 results per clock and SM) and 16 D clocks of the tensor cores, so both at
-// D = 128 and the exponentials below.  Measured: 20/4 heads of 128, 2 x 1729
-// queries, 6001 keys with lengths 184 us, 1008 TFLOP/s (0.61 of the measured
-// GEMM rate); 2 x 16 heads of 64, 5184 queries, 20736 keys 1.47 - 1.57 ms, 560
-// - 597 TFLOP/s, the exponential units 0.53 busy: what is missing is the way
-// from S to P and back (waits, two TMEM loads, the maximum), which two warps on
-// a scheduler do not hide.  Tried without gain: S read twice in 64-column
-// halves, no maximum before the exponentials (made again where a row's P would
-// overflow): 1.59 ms; P beside S with S of the next tile made early: 1.84 ms;
-// one or two of eight exponentials by polynomial: within 4%.
+// (16 results per clock and SM) and 8 D clocks of the tensor cores (4 x 128 x
+// 128 D flops at 8192 per clock and SM): as many at D = 128, half at 64.
+// Neither is what the kernel waits for: at D = 128 both are half busy (ncu:
+// 0.51 and 0.46), at 64 the exponential units 0.51.  What is missing is the
+// way from S to P and back (waits, two TMEM loads, the maximum), which two
+// warps on a scheduler do not hide.  Measured: 20/4 heads of 128, 2 x 1729
+// queries, 6001 and 4501 keys 187 us, 992 TFLOP/s, 0.59 of the measured GEMM
+// rate (205 - 208 us, 0.54, once the card is at its power limit); 2 x 16 heads
+// of 64, 5184 queries, 20736 keys 1.54 - 1.55 ms, 570 TFLOP/s.
+//
+// Other forms, the last case, measured while the kernel was written: P beside S
+// and all 128 scores of a row in registers, so that the next S is made during
+// the softmax: 1.36 ms with one item a CTA (212 us for the first case); walking
+// several items as well, that form spilled, and with 96 + 32 scores as below it
+// took 1.84 ms.  No maximum before the exponentials (made again where a row's P
+// would overflow): 1.59 ms.  S read twice in 64-column halves: 1.87 ms.  One or
+// two of eight exponentials by polynomial: 1.51 and 1.60 ms.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -634,7 +641,8 @@ int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
   prm.splits = cluster_splits(kernel, kThreads, Cfg<kD>::kSmem, prm.n_items, key_tiles, 4, 8, clusters);
   // Short items: one CTA per SM that walks them, so that an item's first loads
   // and S overlap the epilogue before it (4 x 8 heads x 5184 queries, 77 / 512 /
-  // 2048 keys, D = 64: 29 / 63 / 203 us against 37 / 71 / 208 with a CTA each).
+  // 2048 keys, D = 64: 26 / 54 / 167 us against 36 / 64 / 176 with a CTA each;
+  // 4096 keys 320 and 327, but lengths that differ would leave SMs without work).
   // Long ones have a CTA each, dealt out as SMs come free (lengths differ).
   int64_t ctas = static_cast<int64_t>(prm.n_items) * prm.splits;
   if (prm.splits == 1 && key_tiles <= 16) ctas = std::min<int64_t>(ctas, num_sms());

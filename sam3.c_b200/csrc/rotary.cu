@@ -538,10 +538,14 @@ int launch_typed(Params& p, int rot, bool vec, cudaStream_t st) {
     const int lanes = p.head_dim / 16;
     const int g = lanes <= 1 ? 1 : lanes <= 2 ? 2 : lanes <= 4 ? 4 : lanes <= 8 ? 8 : 16;
     // Lane groups that share a token's heads (they repeat its cosines): as
-    // many as one wave of CTAs has room for.  Beyond a wave one, but two where
-    // a second wave would be mostly empty and 16 heads are left to each
-    // (41472 tokens x 32 heads of 64, 1.5 waves: 60.6 -> 56.6 us; 82944 x 20
-    // with LayerNorm, 2.9 waves: 79.2 with one, 89.6 with two).
+    // many as one wave of CTAs has room for.  Beyond a wave one, but two below two
+    // waves where 16 heads are left to each: the last CTAs end sooner.  One and
+    // two at 1.05 / 1.25 / 1.5 / 1.75 / 1.95 waves, bf16: 32 heads of 64 49 / 52 /
+    // 62 / 71 / 79 and 44 / 50 / 61 / 69 / 76 us; 48 + 16 heads of 128 89 / 103 /
+    // 122 / 137 / 153 and 86 / 97 / 115 / 133 / 146; with an RMS norm two are
+    // better by up to 13% too, but worse by 2 - 10% for 32 heads of 64 and by 2 -
+    // 6% at 1.95 waves of heads of 128.  Past two waves: 82944 tokens x 20 heads
+    // with LayerNorm, 2.9 waves, 79 with one and 90 with two.
     const bool exchange = rot % 16 && p.f.layout == SAM3CU_ROPE_HALF;
     const int per_block = kThreads / g;
     const int64_t alone = (p.tokens + per_block - 1) / per_block;

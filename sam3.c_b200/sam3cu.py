@@ -436,7 +436,7 @@ def cross_attention(q, k, v, k_lens=None, key_mask=None, bias=None, scale: float
     bool or uint8 [batch or 1, sk], True where a key counts; bias: float32,
     added to the scaled scores, of a shape that broadcasts to [batch, q_heads,
     sq, sk] (its last dimension sk); scale 0: 1/sqrt(head_dim).  A query left
-    without keys gives zeros."""
+    without keys gives zeros.  out shares no memory with an input."""
     dev = _here(q)
     qshape, kshape = q.shape, k.shape
     if len(qshape) != 4 or len(kshape) != 4 or kshape[0] != qshape[0] or kshape[3] != qshape[3]:
