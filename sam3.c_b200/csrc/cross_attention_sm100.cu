@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mt = fmaxf(mt, fmaxf(max64(sv), max32(sv + 64)));
         const bool need = (mt - m_used) * sl2 > kRescaleLog2;  // false for -inf - -inf
         const float m_new = fmaxf(m_used, mt), top = fabsf(m_new * sl2);
-        const bool far_row = top > kFarLog2 && top < INFINITY;
+        const bool far_row = top > kFarLog2 && fabsf(m_new) < INFINITY;
         if (__any_sync(0xffffffffu, need || far_row)) {
           const float corr = m_used == -INFINITY ? 0.f : ex2((m_used - m_new) * sl2);
           l *= corr;
@@ -624,8 +624,8 @@ int launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
       cudaGetLastError();
       return kErrCuda;
     }
-    if (fa.localSizeBytes != 0) builds_spilled.fetch_add(1);
-    spills.store(fa.localSizeBytes != 0);
+    const int s = fa.localSizeBytes != 0;
+    if (spills.exchange(s) < 0) builds_spilled.fetch_add(s);
   }
   if (spills.load() || as_if_spilled.load()) return kCrossTcSpills;
   int dev = 0;

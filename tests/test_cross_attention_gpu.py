@@ -597,3 +597,16 @@ def test_rows_of_large_scores_among_others(cuda, dt, hd, sq, sk):
     lens = torch.tensor([sk, sk // 2], dtype=torch.int32, device="cuda")
     _check(q, k, v, k_lens=lens)
     _check(q, k, v, k_lens=lens, key_mask=torch.arange(sk, device="cuda")[None] % 5 > 1)
+
+
+@pytest.mark.parametrize("sq,sk", [(1, 999), (20, 999), (150, 77), (300, 1500)])
+def test_scores_whose_exponents_pass_f32(cuda, sq, sk):
+    """Finite dot products whose product with the scale is none: equal scores
+    still give the mean of V."""
+    import torch
+    import sam3cu
+    q, k, v = _make(1, sq, sk, 1, 1, 64, "bf16", seed=22)
+    q[:], k[:] = 32.0, 32.0
+    o = sam3cu.cross_attention(q, k, v, scale=2.0 ** 120).double()
+    mean, mag = v[0, :, 0].double().mean(0), v[0, :, 0].double().abs().mean(0)
+    assert bool(((o - mean).abs() <= 2.0 ** -8 * mean.abs() + (2.0 ** -8 + 2.0 ** -18) * mag).all())
