@@ -610,3 +610,19 @@ def test_scores_whose_exponents_pass_f32(cuda, sq, sk):
     o = sam3cu.cross_attention(q, k, v, scale=2.0 ** 120).double()
     mean, mag = v[0, :, 0].double().mean(0), v[0, :, 0].double().abs().mean(0)
     assert bool(((o - mean).abs() <= 2.0 ** -8 * mean.abs() + (2.0 ** -8 + 2.0 ** -18) * mag).all())
+
+
+@pytest.mark.parametrize("sq", [1, 40, 300])
+def test_overlapping_rows(cuda, sq):
+    """Strides shorter than a row: keys, heads and sequences that share data
+    (windows over one buffer)."""
+    import torch
+    buf, other = (torch.randn(40000, device="cuda").bfloat16() for _ in range(2))
+    q, k, v = _make(2, sq, 300, 4, 2, 64, "bf16", seed=23)
+    _check(q, buf.as_strided((2, 300, 2, 64), (8, 16, 64, 1)), other.as_strided((2, 300, 2, 64), (24, 8, 8, 1)))
+    _check(buf.as_strided((2, sq, 4, 64), (16, 8, 24, 1)), k, v)
+
+
+@pytest.mark.parametrize("sq,sk,hd", [(300000, 5, 32), (300000, 130, 64), (1, 2000000, 16), (100, 500000, 16)])
+def test_largest_sides(cuda, sq, sk, hd):
+    _check(*_make(1, sq, sk, 1, 1, hd, "bf16", seed=24))
