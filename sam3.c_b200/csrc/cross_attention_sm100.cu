@@ -65,7 +65,7 @@ constexpr float kRescaleLog2 = 8.f;
 // a row's P get a factor that cancels in O / sum, 2^-12 off 1 at most up to
 // here.  It would be 2^4 at 2^27 (past f16's range) and 2^64 at 2^31: past this
 // value the maximum is taken off the scores first.  That costs 2 x 5184 queries
-// over 20736 keys 1536 -> 1543 us where it does not happen, in this form; taken
+// over 20736 keys 1536 -> 1546 us where it does not happen, in this form; taken
 // off always 1595, by a branch before the exponentials 1590 - 1617.
 constexpr float kFarLog2 = 4096.f;
 // f16 P below 2^-14 loses bits: with a maximum of 2^9 there is room for a
